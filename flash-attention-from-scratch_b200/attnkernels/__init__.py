@@ -17,7 +17,10 @@ Decode (one query token per sequence) over a paged KV cache:
 Additions (no counterpart in the reference): paged_decode_partials and
 merge_partials expose the split state for context parallelism across GPUs
 (see attnkernels.parallel), device_status reads the kernels' error word, and
-release_workspaces drops the decode scratch kept between calls.
+release_workspaces drops the decode scratch kept between calls. A paged cache
+held in 4 bits (paged_append_kv4, paged_read_kv4, paged_decode_kv4) and the
+eviction of cached tokens by accumulated attention weight (paged_decode_weights,
+paged_evict) are in attnkernels.kvcache.
 
 There is no CPU fallback: every function needs a B200 and the native library
 (built by flash-attention-from-scratch_b200/build.py, or on first use).
@@ -33,7 +36,9 @@ from . import _native
 
 __all__ = ["naive_attention", "flash_attention", "paged_decode", "decode_partition",
            "load_extension", "paged_decode_partials", "merge_partials", "device_status",
-           "check_device_status", "release_workspaces", "CHUNK", "WMMA_BLOCK_N"]
+           "check_device_status", "release_workspaces", "CHUNK", "WMMA_BLOCK_N",
+           "kv4_row_bytes", "paged_append_kv4", "paged_read_kv4", "paged_decode_kv4",
+           "paged_decode_weights", "paged_evict"]
 
 # Decode partitions are multiples of this many tokens (attnkernels/__init__.py:29).
 CHUNK = 256
@@ -266,3 +271,7 @@ def check_device_status(device=None):
         raise RuntimeError(f"block table holds an id outside the cache (site {site})")
     if code != _native.DEVICE_OK:
         raise RuntimeError(f"attention kernel error code {code} (site {site})")
+
+
+from .kvcache import (kv4_row_bytes, paged_append_kv4, paged_decode_kv4,  # noqa: E402
+                      paged_decode_weights, paged_evict, paged_read_kv4)

@@ -47,6 +47,19 @@ SIGNATURES = {
     "attn_merge_partials": (_int, [_vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _vp, _vp]),
     "attn_paged_decode_noalloc": (_int, [_vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64,
                                          _i64, _i64, _i64, _i64, _f32, _i64, _vp]),
+    "attn_paged_decode_weights_workspace_bytes": (_size, [_i64, _i64, _i64, _i64, _i64, _i64]),
+    "attn_paged_decode_weights": (_int, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64,
+                                         _i64, _i64, _i64, _i64, _f32, _i64, _vp, _size, _vp]),
+    "attn_paged_evict": (_int, [ctypes.POINTER(_vp), ctypes.POINTER(_i64), _int, _vp, _vp, _vp, _vp,
+                                _vp, _vp, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64,
+                                _i64, _vp]),
+    "attn_kv4_row_bytes": (_i64, [_i64]),
+    "attn_kv4_append": (_int, [_vp, _vp, _int, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64,
+                               _i64, _i64, _i64, _i64, _vp]),
+    "attn_kv4_read": (_int, [_vp, _vp, _vp, _vp, _vp, _int, _i64, _i64, _i64, _i64, _i64, _vp]),
+    "attn_kv4_decode_workspace_bytes": (_size, [_i64, _i64, _i64, _i64, _i64, _i64, _int]),
+    "attn_kv4_decode": (_int, [_vp, _int, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64,
+                               _i64, _i64, _i64, _i64, _f32, _i64, _vp, _size, _vp]),
     "attn_device_status": (_int, [_u32p, _u32p]),
     "attn_selftest_wait_timeout": (_int, [ctypes.c_uint64, _vp]),
     "attn_selftest_exp2": (_int, [_vp, _vp, _vp, _vp, _i64, _vp]),
@@ -151,6 +164,18 @@ class _StreamWorkspaces:
 _decode_ws = _StreamWorkspaces()
 
 
+def _call_workspace(nbytes: int, device: torch.device, stream: int) -> torch.Tensor:
+    """The stream's kept scratch, or, while a graph is captured, scratch of the
+    capture's own: a graph must not hold an address that a later call may give
+    back, nor share it with another graph."""
+    if torch.cuda.is_current_stream_capturing():
+        return _workspace(nbytes, device)
+    return _decode_ws.get(nbytes, device, stream)
+
+
+_DTYPES = {torch.float16: 0, torch.bfloat16: 1}  # ATTN_FP16, ATTN_BF16
+
+
 class Extension:
     """The reference extension's functions, running the sm_100a kernels."""
 
@@ -244,6 +269,69 @@ class Extension:
                 slots, flags, int(world), int(rank), int(epoch) & 0xFFFFFFFF, int(rows),
                 int(head_dim), int(slot_stride), _ptr(out), _stream(out.device)))
         return out
+
+    def paged_decode_weights(self, q, kc, vc, bt, ctx, max_ctx, weights, scale, partition):
+        out = torch.empty_like(q)
+        B, H, Hkv, D, bs, nblk, maxb = self._decode_sizes(q, kc, bt)
+        with _on(q.device):
+            stream = _stream(q.device)
+            ws = _call_workspace(
+                self.lib.attn_paged_decode_weights_workspace_bytes(B, H, Hkv, D, max_ctx,
+                                                                   partition), q.device, stream)
+            _check(self.lib.attn_paged_decode_weights(
+                _ptr(q), _ptr(kc), _ptr(vc), _ptr(bt), _ptr(ctx), _ptr(out), _ptr(weights), B, H,
+                Hkv, D, bs, nblk, maxb, max_ctx, scale, partition, _ptr(ws), ws.numel(), stream))
+        return out
+
+    # ------------------------------------------------- 4-bit cache, eviction
+    def kv4_append(self, k, v, kc, vc, slots, weights):
+        T, Hkv, D = k.shape
+        with _on(k.device):
+            _check(self.lib.attn_kv4_append(
+                _ptr(k), _ptr(v), _DTYPES[k.dtype], _ptr(kc), _ptr(vc), _ptr(slots),
+                _ptr(weights), T, Hkv, D, k.stride(0), k.stride(1), v.stride(0), v.stride(1),
+                kc.shape[2], kc.shape[0], _stream(k.device)))
+
+    def kv4_read(self, kc, vc, slots, head_dim, dtype):
+        T = slots.shape[0]
+        k, v = (torch.empty(T, kc.shape[1], head_dim, dtype=dtype, device=kc.device)
+                for _ in range(2))
+        with _on(kc.device):
+            _check(self.lib.attn_kv4_read(
+                _ptr(kc), _ptr(vc), _ptr(slots), _ptr(k), _ptr(v), _DTYPES[dtype], T, kc.shape[1],
+                head_dim, kc.shape[2], kc.shape[0], _stream(kc.device)))
+        return k, v
+
+    def kv4_decode(self, q, kc, vc, bt, ctx, max_ctx, weights, scale, partition):
+        out = torch.empty_like(q)
+        B, H, Hkv, D, bs, nblk, maxb = self._decode_sizes(q, kc, bt)
+        with _on(q.device):
+            stream = _stream(q.device)
+            ws = _call_workspace(
+                self.lib.attn_kv4_decode_workspace_bytes(B, H, Hkv, D, max_ctx, partition,
+                                                         int(weights is not None)),
+                q.device, stream)
+            _check(self.lib.attn_kv4_decode(
+                _ptr(q), _DTYPES[q.dtype], _ptr(kc), _ptr(vc), _ptr(bt), _ptr(ctx), _ptr(out),
+                _ptr(weights), B, H, Hkv, D, bs, nblk, maxb, max_ctx, scale, partition, _ptr(ws),
+                ws.numel(), stream))
+        return out
+
+    def paged_evict(self, caches, row_bytes, weights, bt, ctx, max_ctx, new_bt, keep, recent,
+                    sinks):
+        nblk, Hkv, bs = weights.shape
+        B = bt.shape[0]
+        i32 = dict(dtype=torch.int32, device=weights.device)
+        new_lens = torch.empty(B, **i32)
+        kept = torch.empty(B, Hkv, keep, **i32)
+        n = len(caches)
+        with _on(weights.device):
+            _check(self.lib.attn_paged_evict(
+                (_vp * n)(*(c.data_ptr() for c in caches)), (_i64 * n)(*row_bytes), n,
+                _ptr(weights), _ptr(bt), _ptr(ctx), _ptr(new_bt), _ptr(new_lens), _ptr(kept), B,
+                Hkv, bs, nblk, bt.shape[1], max_ctx, new_bt.shape[1], keep, recent, sinks,
+                _stream(weights.device)))
+        return new_lens, kept
 
     # -------------------------------------------------------------- status
     def device_status(self, device=None):

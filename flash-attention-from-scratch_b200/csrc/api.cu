@@ -224,6 +224,40 @@ int check_decode(const char* name, const DecodeArgs& a) {
   return ATTN_OK;
 }
 
+int check_weights(const char* name, const float* weights) {
+  if (weights == nullptr || (reinterpret_cast<uintptr_t>(weights) & 3u) != 0)
+    return fail(ATTN_ERR_INVALID, "%s: weights must be a 4-byte aligned pointer", name);
+  return ATTN_OK;
+}
+
+int check_kv4(const char* name, int dtype, int64_t head_dim, const void* k_cache,
+              const void* v_cache) {
+  if (dtype != ATTN_FP16 && dtype != ATTN_BF16)
+    return fail(ATTN_ERR_UNSUPPORTED, "%s: dtype must be ATTN_FP16 or ATTN_BF16", name);
+  if (head_dim != 64 && head_dim != 128)
+    return fail(ATTN_ERR_UNSUPPORTED, "%s: head_dim must be 64 or 128, got %lld", name,
+                static_cast<long long>(head_dim));
+  if (k_cache == nullptr || v_cache == nullptr || !aligned16(k_cache) || !aligned16(v_cache))
+    return fail(ATTN_ERR_INVALID, "%s: caches must be 16-byte aligned pointers", name);
+  return ATTN_OK;
+}
+
+int check_kv4_copy(const char* name, const void* k, const void* v, const int64_t* slots,
+                   int64_t tokens, int64_t hkv, int64_t head_dim, int64_t bs, int64_t num_blocks) {
+  if (k == nullptr || v == nullptr || slots == nullptr)
+    return fail(ATTN_ERR_INVALID, "%s: null tensor pointer", name);
+  if (!aligned16(k) || !aligned16(v))
+    return fail(ATTN_ERR_INVALID, "%s: k and v must be 16-byte aligned", name);
+  if (tokens < 0 || hkv <= 0 || bs <= 0 || num_blocks < 0)
+    return fail(ATTN_ERR_INVALID, "%s: negative or zero size", name);
+  if (tokens > 0x7fffffffLL || hkv > 0x10000 || bs > 0x10000 || num_blocks > 0x7fffffffLL ||
+      tokens * hkv > 0x7fffffffLL)
+    return fail(ATTN_ERR_UNSUPPORTED,
+                "%s: tokens * num_kv_heads and num_blocks must fit in 31 bits (num_kv_heads and "
+                "block_size <= 65536)", name);
+  return ATTN_OK;
+}
+
 }  // namespace
 }  // namespace fab
 
@@ -396,6 +430,232 @@ int attn_paged_decode_noalloc(const void* q, const void* k_cache, const void* v_
   cudaError_t e = paged_decode_static_scratch(a, ctx, &err);
   if (!err.empty()) return fail(ATTN_ERR_WORKSPACE, "%s", err.c_str());
   if (e != cudaSuccess) return cuda_fail(e, "paged_decode_noalloc launch");
+  return ATTN_OK;
+}
+
+size_t attn_paged_decode_weights_workspace_bytes(int64_t batch, int64_t num_heads,
+                                                 int64_t num_kv_heads, int64_t head_dim,
+                                                 int64_t max_context_len, int64_t partition) {
+  if (batch <= 0 || num_heads <= 0 || num_kv_heads <= 0 || head_dim <= 0 || partition <= 0 ||
+      max_context_len < 0)
+    return 0;
+  return decode_weights_workspace_bytes(batch, num_heads, num_kv_heads, head_dim, max_context_len,
+                                        partition);
+}
+
+int attn_paged_decode_weights(const void* q, const void* k_cache, const void* v_cache,
+                              const int32_t* block_tables, const int32_t* context_lens, void* out,
+                              float* weights, int64_t batch, int64_t num_heads,
+                              int64_t num_kv_heads, int64_t head_dim, int64_t block_size,
+                              int64_t num_blocks, int64_t max_blocks_per_seq,
+                              int64_t max_context_len, float scale, int64_t partition,
+                              void* workspace, size_t workspace_bytes, void* stream) {
+  DecodeArgs a{q, k_cache, v_cache, block_tables, context_lens, out, nullptr, nullptr, nullptr,
+               batch, num_heads, num_kv_heads, head_dim, block_size, num_blocks,
+               max_blocks_per_seq, max_context_len, partition, scale, workspace, workspace_bytes,
+               weights};
+  int rc = check_decode("paged_decode_weights", a);
+  if (rc != ATTN_OK) return rc;
+  if (out == nullptr || !aligned16(out))
+    return fail(ATTN_ERR_INVALID, "paged_decode_weights: out must be a 16-byte aligned pointer");
+  rc = check_weights("paged_decode_weights", weights);
+  if (rc != ATTN_OK) return rc;
+  const size_t need = decode_weights_workspace_bytes(batch, num_heads, num_kv_heads, head_dim,
+                                                     max_context_len, partition);
+  if (workspace_bytes < need)
+    return fail(ATTN_ERR_WORKSPACE,
+                "paged_decode_weights: workspace of %zu bytes (256-byte aligned) needed", need);
+  if (batch == 0) return ATTN_OK;
+  LaunchCtx ctx;
+  rc = device_ctx(static_cast<cudaStream_t>(stream), &ctx);
+  if (rc != ATTN_OK) return rc;
+  cudaError_t e = launch_paged_decode(a, false, ctx);
+  if (e != cudaSuccess) return cuda_fail(e, "paged_decode_weights launch");
+  return ATTN_OK;
+}
+
+int attn_paged_evict(void* const* arrays, const int64_t* row_bytes, int num_arrays, float* weights,
+                     const int32_t* block_tables, const int32_t* context_lens,
+                     const int32_t* new_block_tables, int32_t* new_lens, int32_t* kept,
+                     int64_t batch, int64_t num_kv_heads, int64_t block_size, int64_t num_blocks,
+                     int64_t max_blocks_per_seq, int64_t max_context_len, int64_t new_max_blocks,
+                     int64_t keep, int64_t recent, int64_t sinks, void* stream) {
+  const char* name = "paged_evict";
+  if (arrays == nullptr || row_bytes == nullptr || block_tables == nullptr ||
+      context_lens == nullptr || new_block_tables == nullptr || new_lens == nullptr ||
+      kept == nullptr)
+    return fail(ATTN_ERR_INVALID, "%s: null pointer", name);
+  if (num_arrays < 1 || num_arrays > kMaxEvictArrays)
+    return fail(ATTN_ERR_INVALID, "%s: 1 to %d cache arrays, got %d", name, kMaxEvictArrays,
+                num_arrays);
+  int rc = check_weights(name, weights);
+  if (rc != ATTN_OK) return rc;
+  for (int i = 0; i < num_arrays; ++i)
+    if (arrays[i] == nullptr || row_bytes[i] <= 0 || row_bytes[i] > 0x10000)
+      return fail(ATTN_ERR_INVALID, "%s: array %d needs a pointer and 1 to 65536 bytes a row", name,
+                  i);
+  if (batch < 0 || num_kv_heads <= 0 || block_size <= 0 || num_blocks < 0 ||
+      max_blocks_per_seq < 0 || max_context_len < 0 || new_max_blocks < 0)
+    return fail(ATTN_ERR_INVALID, "%s: negative or zero size", name);
+  if (keep < 0 || recent < 0 || sinks < 0 || recent > keep || sinks > keep - recent)
+    return fail(ATTN_ERR_INVALID, "%s: sinks and recent must be >= 0 and add up to keep at most",
+                name);
+  if (max_context_len > 0x7fffffffLL || max_blocks_per_seq > 0x7fffffffLL ||
+      new_max_blocks > 0x7fffffffLL || block_size > 0x10000 || num_blocks > 0x7fffffffLL ||
+      keep > 0x7fffffffLL || num_kv_heads > 0x7fffffffLL || batch > 0x7fffffffLL ||
+      batch * num_kv_heads > 0x7fffffffLL)
+    return fail(ATTN_ERR_UNSUPPORTED, "%s: sizes must fit in 31 bits (block_size <= 65536)", name);
+  if (max_context_len > max_blocks_per_seq * block_size)
+    return fail(ATTN_ERR_INVALID, "%s: max_context_len needs more than max_blocks_per_seq blocks",
+                name);
+  const int64_t most = keep < max_context_len ? keep : max_context_len;
+  if (most > new_max_blocks * block_size)
+    return fail(ATTN_ERR_INVALID, "%s: new_block_tables holds %lld blocks of %lld, too few for %lld tokens",
+                name, static_cast<long long>(new_max_blocks), static_cast<long long>(block_size),
+                static_cast<long long>(most));
+  if (batch == 0) return ATTN_OK;
+  EvictArgs a;
+  for (int i = 0; i < num_arrays; ++i) {
+    a.arrays[i] = arrays[i];
+    a.row_bytes[i] = row_bytes[i];
+  }
+  a.num_arrays = num_arrays;
+  a.weights = weights;
+  a.block_tables = block_tables;
+  a.context_lens = context_lens;
+  a.new_block_tables = new_block_tables;
+  a.new_lens = new_lens;
+  a.kept = kept;
+  a.batch = batch;
+  a.hkv = num_kv_heads;
+  a.bs = block_size;
+  a.num_blocks = num_blocks;
+  a.max_blocks = max_blocks_per_seq;
+  a.max_ctx = max_context_len;
+  a.new_max_blocks = new_max_blocks;
+  a.keep = keep;
+  a.recent = recent;
+  a.sinks = sinks;
+  LaunchCtx ctx;
+  rc = device_ctx(static_cast<cudaStream_t>(stream), &ctx);
+  if (rc != ATTN_OK) return rc;
+  cudaError_t e = launch_evict(a, ctx);
+  if (e != cudaSuccess) return cuda_fail(e, "paged_evict launch");
+  return ATTN_OK;
+}
+
+int64_t attn_kv4_row_bytes(int64_t head_dim) {
+  return head_dim == 64 || head_dim == 128 ? head_dim / 2 + head_dim / 8 : 0;
+}
+
+int attn_kv4_append(const void* k, const void* v, int dtype, void* k_cache, void* v_cache,
+                    const int64_t* slots, float* weights, int64_t tokens, int64_t num_kv_heads,
+                    int64_t head_dim, int64_t k_token_stride, int64_t k_head_stride,
+                    int64_t v_token_stride, int64_t v_head_stride, int64_t block_size,
+                    int64_t num_blocks, void* stream) {
+  const char* name = "paged_append_kv4";
+  int rc = check_kv4(name, dtype, head_dim, k_cache, v_cache);
+  if (rc == ATTN_OK)
+    rc = check_kv4_copy(name, k, v, slots, tokens, num_kv_heads, head_dim, block_size, num_blocks);
+  if (rc == ATTN_OK && weights != nullptr) rc = check_weights(name, weights);
+  if (rc != ATTN_OK) return rc;
+  if (k_token_stride % 8 != 0 || k_head_stride % 8 != 0 || v_token_stride % 8 != 0 ||
+      v_head_stride % 8 != 0)
+    return fail(ATTN_ERR_INVALID, "%s: strides must be multiples of 8 elements", name);
+  if (tokens == 0) return ATTN_OK;
+  LaunchCtx ctx;
+  rc = device_ctx(static_cast<cudaStream_t>(stream), &ctx);
+  if (rc != ATTN_OK) return rc;
+  Kv4CopyArgs a{const_cast<void*>(k), const_cast<void*>(v), dtype == ATTN_BF16,
+                {k_token_stride, v_token_stride}, {k_head_stride, v_head_stride},
+                k_cache, v_cache, slots, weights, tokens, num_kv_heads, head_dim, block_size,
+                num_blocks};
+  cudaError_t e = launch_kv4_append(a, ctx);
+  if (e != cudaSuccess) return cuda_fail(e, "paged_append_kv4 launch");
+  return ATTN_OK;
+}
+
+int attn_kv4_read(const void* k_cache, const void* v_cache, const int64_t* slots, void* k, void* v,
+                  int dtype, int64_t tokens, int64_t num_kv_heads, int64_t head_dim,
+                  int64_t block_size, int64_t num_blocks, void* stream) {
+  const char* name = "paged_read_kv4";
+  int rc = check_kv4(name, dtype, head_dim, k_cache, v_cache);
+  if (rc == ATTN_OK)
+    rc = check_kv4_copy(name, k, v, slots, tokens, num_kv_heads, head_dim, block_size, num_blocks);
+  if (rc != ATTN_OK) return rc;
+  if (tokens == 0) return ATTN_OK;
+  LaunchCtx ctx;
+  rc = device_ctx(static_cast<cudaStream_t>(stream), &ctx);
+  if (rc != ATTN_OK) return rc;
+  Kv4CopyArgs a{k, v, dtype == ATTN_BF16, {0, 0}, {0, 0}, const_cast<void*>(k_cache),
+                const_cast<void*>(v_cache), slots, nullptr, tokens, num_kv_heads, head_dim,
+                block_size, num_blocks};
+  cudaError_t e = launch_kv4_read(a, ctx);
+  if (e != cudaSuccess) return cuda_fail(e, "paged_read_kv4 launch");
+  return ATTN_OK;
+}
+
+size_t attn_kv4_decode_workspace_bytes(int64_t batch, int64_t num_heads, int64_t num_kv_heads,
+                                       int64_t head_dim, int64_t max_context_len,
+                                       int64_t partition, int with_weights) {
+  if (batch <= 0 || num_heads <= 0 || num_kv_heads <= 0 || head_dim <= 0 || partition <= 0 ||
+      max_context_len < 0)
+    return 0;
+  return kv4_decode_workspace_bytes(batch, num_heads, num_kv_heads, head_dim, max_context_len,
+                                    partition, with_weights != 0);
+}
+
+int attn_kv4_decode(const void* q, int dtype, const void* k_cache, const void* v_cache,
+                    const int32_t* block_tables, const int32_t* context_lens, void* out,
+                    float* weights, int64_t batch, int64_t num_heads, int64_t num_kv_heads,
+                    int64_t head_dim, int64_t block_size, int64_t num_blocks,
+                    int64_t max_blocks_per_seq, int64_t max_context_len, float scale,
+                    int64_t partition, void* workspace, size_t workspace_bytes, void* stream) {
+  const char* name = "paged_decode_kv4";
+  int rc = check_kv4(name, dtype, head_dim, k_cache, v_cache);
+  if (rc == ATTN_OK && weights != nullptr) rc = check_weights(name, weights);
+  if (rc != ATTN_OK) return rc;
+  if (q == nullptr || out == nullptr || block_tables == nullptr || context_lens == nullptr)
+    return fail(ATTN_ERR_INVALID, "%s: null tensor pointer", name);
+  if (!aligned16(q) || !aligned16(out))
+    return fail(ATTN_ERR_INVALID, "%s: q and out must be 16-byte aligned", name);
+  if (batch < 0 || num_heads <= 0 || num_kv_heads <= 0 || block_size <= 0 || num_blocks < 0 ||
+      max_blocks_per_seq < 0 || max_context_len < 0)
+    return fail(ATTN_ERR_INVALID, "%s: negative or zero size", name);
+  if (num_heads % num_kv_heads != 0)
+    return fail(ATTN_ERR_INVALID, "%s: num_heads must be a multiple of num_kv_heads", name);
+  if (num_heads / num_kv_heads > 8)
+    return fail(ATTN_ERR_UNSUPPORTED, "%s: num_heads / num_kv_heads must be 1 to 8", name);
+  if (partition <= 0 || partition % 256 != 0 || partition > 0x40000000LL)
+    return fail(ATTN_ERR_INVALID, "%s: partition size must be a positive multiple of 256", name);
+  if (head_dim == 64 && block_size % 2 != 0)
+    return fail(ATTN_ERR_UNSUPPORTED, "%s: head_dim 64 needs an even block_size", name);
+  if (max_context_len > 0x40000000LL || max_blocks_per_seq > 0x7fffffffLL ||
+      block_size > 0x10000 || num_blocks > 0x7fffffffLL || batch > 0x7fffffffLL ||
+      num_heads > 0x7fffffffLL || batch * num_heads > 0x7fffffffLL)
+    return fail(ATTN_ERR_UNSUPPORTED,
+                "%s: sizes must fit in 31 bits (max_context_len <= 2^30, block_size <= 65536)", name);
+  if (max_context_len > max_blocks_per_seq * block_size)
+    return fail(ATTN_ERR_INVALID, "%s: max_context_len needs more than max_blocks_per_seq blocks",
+                name);
+  if (max_context_len > 0 && num_blocks == 0)
+    return fail(ATTN_ERR_INVALID, "%s: empty cache with a non-empty context", name);
+  if (batch == 0) return ATTN_OK;
+  const size_t need = kv4_decode_workspace_bytes(batch, num_heads, num_kv_heads, head_dim,
+                                                 max_context_len, partition, weights != nullptr);
+  if (workspace == nullptr || workspace_bytes < need ||
+      (reinterpret_cast<uintptr_t>(workspace) & 255u))
+    return fail(ATTN_ERR_WORKSPACE, "%s: workspace of %zu bytes (256-byte aligned) needed", name,
+                need);
+  LaunchCtx ctx;
+  rc = device_ctx(static_cast<cudaStream_t>(stream), &ctx);
+  if (rc != ATTN_OK) return rc;
+  Kv4DecodeArgs a{q, dtype == ATTN_BF16, k_cache, v_cache, block_tables, context_lens, out, weights,
+                  batch, num_heads, num_kv_heads, head_dim, block_size, num_blocks,
+                  max_blocks_per_seq, max_context_len, partition, scale, workspace,
+                  workspace_bytes};
+  cudaError_t e = launch_kv4_decode(a, ctx);
+  if (e != cudaSuccess) return cuda_fail(e, "paged_decode_kv4 launch");
   return ATTN_OK;
 }
 

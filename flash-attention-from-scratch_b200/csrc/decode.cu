@@ -37,7 +37,7 @@
 #include <algorithm>
 #include <mutex>
 
-#include "common.cuh"
+#include "kv4.cuh"
 #include "launch.h"
 
 namespace fab {
@@ -112,6 +112,7 @@ struct DecParams {
   float* o_part;   // fp32 [batch * hq, num_splits, D]
   float* m_part;   // fp32 [batch * hq, num_splits]
   float* l_part;
+  float* scores;   // SCORED: fp32 [batch, hkv, max_ctx, G] scores in log2 units
   unsigned int* counter;  // work counter, zero at launch
   DeviceStatus* status;
   unsigned long long timeout_ns;
@@ -119,6 +120,7 @@ struct DecParams {
   int batch, hq, hkv, bs, max_blocks, partition, num_splits;
   int num_blocks;  // physical blocks in the cache: block ids outside [0, num_blocks) are rejected
   int direct_out;  // 1: a sequence with a single split writes its fp16 row directly
+  int max_ctx;     // SCORED: tokens a sequence has room for in `scores`
   float scale_log2;
 };
 
@@ -152,7 +154,17 @@ __device__ __forceinline__ void mma_16816_rows8(float& d0, float& d1, uint32_t a
       : "r"(a0), "r"(0u), "r"(a2), "r"(b0), "r"(b1), "f"(0.f));
 }
 
-template <int D, int G>
+// The maximum that a part is merged by. One whose scores are all NaN has none
+// (max skips NaN), yet is not an empty part, which the merge would drop: in a
+// call with weights it stands with 0, so that its NaN sum reaches the row.
+template <bool SCORED>
+__device__ __forceinline__ float part_max(float m, float l) {
+  return SCORED && l != l ? fmaxf(m, 0.f) : m;
+}
+
+// SCORED: every token's score is written out too, for the totals of attention
+// weights (evict.cu): 4 G bytes beside the 4 D that a token's K and V take.
+template <int D, int G, bool SCORED>
 __global__ void __launch_bounds__(DecCfg<D, G>::THREADS, 1) paged_decode_kernel(const DecParams p) {
   using C = DecCfg<D, G>;
   extern __shared__ __align__(128) uint8_t smem[];
@@ -172,7 +184,9 @@ __global__ void __launch_bounds__(DecCfg<D, G>::THREADS, 1) paged_decode_kernel(
 
   // Context lengths and the prefix sums of the splits per sequence: active
   // (sequence, split) pairs are numbered densely, v in [0, prefix[batch]).
-  for (int b = threadIdx.x; b < p.batch; b += C::THREADS) ctx_s[b] = max(p.ctx[b], 0);
+  // The scores have room for max_ctx tokens, so a longer length is cut to it there.
+  for (int b = threadIdx.x; b < p.batch; b += C::THREADS)
+    ctx_s[b] = SCORED ? min(max(p.ctx[b], 0), p.max_ctx) : max(p.ctx[b], 0);
   if (threadIdx.x < C::W * C::STAGES)
     mbar_init(reinterpret_cast<uint64_t*>(smem + C::BAR_OFF) + threadIdx.x, 1);
   if (threadIdx.x == 0) {
@@ -360,6 +374,7 @@ __global__ void __launch_bounds__(DecCfg<D, G>::THREADS, 1) paged_decode_kernel(
   uint32_t qa[C::MMA ? KS : 1][2];
   float oc[C::MMA ? NT : 1][2];
   float m_r = -INFINITY, l_r = 0.f;  // row g's running max (log2 units) and sum
+  float* sc = nullptr;               // SCORED: the scores of the stage's first token
 
   // One stage of a unit with G > 1 query heads per kv head (st: the stage's
   // ring slot, nt: its tokens, md: its unit and flags).
@@ -394,6 +409,9 @@ __global__ void __launch_bounds__(DecCfg<D, G>::THREADS, 1) paged_decode_kernel(
         const int tok = 2 * (2 * t4 + c) + n;
         s[n][c] = tok < nt ? s[n][c] * p.scale_log2 : -INFINITY;
         mx = fmaxf(mx, s[n][c]);
+        if constexpr (SCORED) {
+          if (tok < nt && g4 < G) sc[tok * G + g4] = s[n][c];
+        }
       }
     mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
     mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
@@ -446,7 +464,7 @@ __global__ void __launch_bounds__(DecCfg<D, G>::THREADS, 1) paged_decode_kernel(
 #pragma unroll
         for (int n = 0; n < NT; ++n) dst[4 * n] = make_float2(oc[n][0] * inv, oc[n][1] * inv);
         if (t4 == 0) {
-          p.m_part[pr] = m_r;
+          p.m_part[pr] = part_max<SCORED>(m_r, l_r);
           p.l_part[pr] = l_r;
         }
       }
@@ -464,6 +482,11 @@ __global__ void __launch_bounds__(DecCfg<D, G>::THREADS, 1) paged_decode_kernel(
     const int4 md = meta[slot];
     const uint8_t* st = ring + slot * C::STAGE;
     const int nt = md.w & 31;
+    if constexpr (SCORED) {
+      sc = (md.w & 32) ? p.scores + ((static_cast<size_t>(md.x) * p.hkv + md.y) * p.max_ctx +
+                                     static_cast<size_t>(md.z) * p.partition) * G
+                       : sc + kTok * G;
+    }
     if constexpr (C::MMA) {
       if (md.w & 32) {
         // q of the unit as A fragments (rows = heads; rows >= G zero), fp16 as
@@ -536,6 +559,9 @@ __global__ void __launch_bounds__(DecCfg<D, G>::THREADS, 1) paged_decode_kernel(
         dot += __shfl_xor_sync(0xffffffffu, dot, 2);
         dot += __shfl_xor_sync(0xffffffffu, dot, 1);
         s[step][g] = (t < nt) ? dot : -INFINITY;
+        if constexpr (SCORED) {
+          if (t < nt && l8 == 0) sc[t * G + g] = dot;
+        }
       }
     }
     // Online softmax over the stage's tokens (the 4 lane groups hold 4 tokens each).
@@ -626,7 +652,7 @@ __global__ void __launch_bounds__(DecCfg<D, G>::THREADS, 1) paged_decode_kernel(
             *reinterpret_cast<float2*>(dst) = make_float2(o[0], o[1]);
           }
           if (lane == 0) {
-            p.m_part[pr] = m[g];
+            p.m_part[pr] = part_max<SCORED>(m[g], l[g]);
             p.l_part[pr] = l[g];
           }
         }
@@ -667,6 +693,7 @@ struct MergeParams {
   long long o_row_stride, o_part_stride, ml_row_stride, ml_part_stride;
   int hq, partition, num_parts;
   int skip_single;  // rows with exactly one part were written by the decode kernel
+  int out_bf16;     // out16 holds bf16 instead
   __half* out16;    // fp16 [rows, D], or else the merged partial state:
   float* out_o;     // fp32 [rows, D]
   float* out_m;     // fp32 [rows]
@@ -802,7 +829,12 @@ __global__ void __launch_bounds__(256) merge_partials_kernel(const MergeParams p
   const float inv = den > 0.f ? 1.f / den : 0.f;
   if (p.out16 != nullptr) {
     __half* dst = p.out16 + row * D + lane * DV;
-    if constexpr (DV == 4) {
+    if (p.out_bf16) {
+#pragma unroll
+      for (int j = 0; j < DV; j += 2)
+        reinterpret_cast<uint32_t*>(dst)[j / 2] =
+            pack2<__nv_bfloat16>(num[j] * inv, num[j + 1] * inv);
+    } else if constexpr (DV == 4) {
       *reinterpret_cast<uint2*>(dst) =
           make_uint2(pack_half2(num[0] * inv, num[1] * inv), pack_half2(num[2] * inv, num[3] * inv));
     } else {
@@ -865,10 +897,10 @@ int64_t splits_of(int64_t max_ctx, int64_t partition) {
   return max_ctx > 0 ? (max_ctx + partition - 1) / partition : 0;
 }
 
-template <int D, int G>
+template <int D, int G, bool SCORED>
 cudaError_t launch_decode_kernel(const DecParams& prm, int64_t upper_units, const LaunchCtx& ctx) {
   using C = DecCfg<D, G>;
-  auto kern = paged_decode_kernel<D, G>;
+  auto kern = paged_decode_kernel<D, G, SCORED>;
   static std::once_flag once;
   static cudaError_t attr_err = cudaSuccess;
   std::call_once(once, [&] {
@@ -899,13 +931,13 @@ int64_t launch_batch(int64_t d, int64_t g) {
   }
 }
 
-template <int D>
+template <int D, bool SCORED>
 cudaError_t dispatch_group(int g, const DecParams& prm, int64_t upper, const LaunchCtx& ctx) {
   switch (g) {
-    case 1: return launch_decode_kernel<D, 1>(prm, upper, ctx);
-    case 2: return launch_decode_kernel<D, 2>(prm, upper, ctx);
-    case 4: return launch_decode_kernel<D, 4>(prm, upper, ctx);
-    case 8: return launch_decode_kernel<D, 8>(prm, upper, ctx);
+    case 1: return launch_decode_kernel<D, 1, SCORED>(prm, upper, ctx);
+    case 2: return launch_decode_kernel<D, 2, SCORED>(prm, upper, ctx);
+    case 4: return launch_decode_kernel<D, 4, SCORED>(prm, upper, ctx);
+    case 8: return launch_decode_kernel<D, 8, SCORED>(prm, upper, ctx);
     default: return cudaErrorInvalidValue;
   }
 }
@@ -973,7 +1005,14 @@ size_t decode_workspace_bytes(int64_t batch, int64_t hq, int64_t d, int64_t max_
   return carve_workspace(nullptr, batch, hq, d, splits_of(max_ctx, partition) * cap).bytes;
 }
 
+size_t decode_weights_workspace_bytes(int64_t batch, int64_t hq, int64_t hkv, int64_t d,
+                                      int64_t max_ctx, int64_t partition) {
+  return decode_workspace_bytes(batch, hq, d, max_ctx, partition) +
+         score_bytes(batch, hkv, hq / hkv, max_ctx);
+}
+
 cudaError_t launch_paged_decode(const DecodeArgs& a, bool partials_mode, const LaunchCtx& ctx) {
+  const bool scored = a.weights != nullptr;
   // Sub-split only while the units stay within one per resident warp.
   int64_t k = sub_split_cap(a.batch, a.hq, a.max_ctx, a.partition);
   const int64_t units = a.batch * a.hkv * splits_of(a.max_ctx, a.partition);
@@ -982,6 +1021,7 @@ cudaError_t launch_paged_decode(const DecodeArgs& a, bool partials_mode, const L
   const int64_t num_splits = splits_of(a.max_ctx, part);
   const int64_t rows = a.batch * a.hq;
   DecodeWorkspace w = carve_workspace(a.workspace, a.batch, a.hq, a.d, num_splits);
+  float* scores = reinterpret_cast<float*>(static_cast<uint8_t*>(a.workspace) + w.bytes);
   if (num_splits == 0 && !partials_mode) {
     return cudaMemsetAsync(a.out, 0, static_cast<size_t>(rows) * a.d * 2, ctx.stream);
   }
@@ -1016,13 +1056,27 @@ cudaError_t launch_paged_decode(const DecodeArgs& a, bool partials_mode, const L
       prm.partition = static_cast<int>(part);
       prm.num_blocks = static_cast<int>(a.num_blocks);
       prm.num_splits = static_cast<int>(num_splits);
-      prm.direct_out = partials_mode ? 0 : 1;
+      prm.direct_out = partials_mode || scored ? 0 : 1;
+      prm.max_ctx = static_cast<int>(a.max_ctx);
+      prm.scores = scored ? scores + static_cast<size_t>(b0) * a.hkv * a.max_ctx * g : nullptr;
       prm.scale_log2 = a.scale * kLog2e;
       const int64_t upper = nb * a.hkv * num_splits;
-      e = (a.d == 64) ? dispatch_group<64>(g, prm, upper, ctx)
-                      : dispatch_group<128>(g, prm, upper, ctx);
+      if (scored)
+        e = (a.d == 64) ? dispatch_group<64, true>(g, prm, upper, ctx)
+                        : dispatch_group<128, true>(g, prm, upper, ctx);
+      else
+        e = (a.d == 64) ? dispatch_group<64, false>(g, prm, upper, ctx)
+                        : dispatch_group<128, false>(g, prm, upper, ctx);
       if (e != cudaSuccess) return e;
     }
+  }
+  if (scored) {
+    cudaError_t e = launch_decode_merge({w.o_part, w.m_part, w.l_part, a.context_lens, a.batch, a.hq,
+                                         a.hkv, a.d, part, num_splits, false, a.out, false}, ctx);
+    if (e != cudaSuccess) return e;
+    return launch_add_weights({scores, w.m_part, w.l_part, a.block_tables, a.context_lens, a.weights,
+                               a.batch, a.hq, a.hkv, a.bs, a.num_blocks, a.max_blocks, a.max_ctx,
+                               part, num_splits}, ctx);
   }
   if (!partials_mode && num_splits <= 1) return cudaSuccess;
   MergeParams mp;
@@ -1039,10 +1093,34 @@ cudaError_t launch_paged_decode(const DecodeArgs& a, bool partials_mode, const L
   mp.partition = static_cast<int>(part);
   mp.num_parts = static_cast<int>(num_splits);
   mp.skip_single = partials_mode ? 0 : 1;
+  mp.out_bf16 = 0;
   mp.out16 = partials_mode ? nullptr : static_cast<__half*>(a.out);
   mp.out_o = a.o_final;
   mp.out_m = a.m_final;
   mp.out_l = a.l_final;
+  return launch_merge_impl(mp, static_cast<int>(a.d), ctx.stream);
+}
+
+cudaError_t launch_decode_merge(const DecodePartsArgs& a, const LaunchCtx& ctx) {
+  MergeParams mp;
+  mp.o = a.o;
+  mp.m = a.m;
+  mp.l = a.l;
+  mp.ctx = a.context_lens;
+  mp.rows = a.batch * a.hq;
+  mp.o_row_stride = a.parts * a.d;
+  mp.o_part_stride = a.d;
+  mp.ml_row_stride = a.parts;
+  mp.ml_part_stride = 1;
+  mp.hq = static_cast<int>(a.hq);
+  mp.partition = static_cast<int>(a.partition);
+  mp.num_parts = static_cast<int>(a.parts);
+  mp.skip_single = a.skip_single ? 1 : 0;
+  mp.out_bf16 = a.bf16 ? 1 : 0;
+  mp.out16 = static_cast<__half*>(a.out);
+  mp.out_o = nullptr;
+  mp.out_m = nullptr;
+  mp.out_l = nullptr;
   return launch_merge_impl(mp, static_cast<int>(a.d), ctx.stream);
 }
 
@@ -1063,6 +1141,7 @@ cudaError_t launch_merge(const float* o_parts, const float* m_parts, const float
   mp.partition = 1;
   mp.num_parts = static_cast<int>(num_parts);
   mp.skip_single = 0;
+  mp.out_bf16 = 0;
   mp.out16 = static_cast<__half*>(out);
   mp.out_o = nullptr;
   mp.out_m = nullptr;

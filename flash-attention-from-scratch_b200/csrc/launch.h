@@ -48,17 +48,107 @@ struct DecodeArgs {
   float scale;
   void* workspace;
   size_t workspace_bytes;
+  float* weights = nullptr;  // fp32 [num_blocks, hkv, bs]: attention weights are added (final mode)
 };
 
 // Workspace layout of the decode path.
 size_t decode_workspace_bytes(int64_t batch, int64_t hq, int64_t d, int64_t max_ctx,
                               int64_t partition);
 
+// The same with room for the scores behind it, for a call with weights.
+size_t decode_weights_workspace_bytes(int64_t batch, int64_t hq, int64_t hkv, int64_t d,
+                                      int64_t max_ctx, int64_t partition);
+
 cudaError_t launch_paged_decode(const DecodeArgs& a, bool partials_mode, const LaunchCtx& ctx);
 
 cudaError_t launch_merge(const float* o_parts, const float* m_parts, const float* l_parts,
                          int64_t num_parts, int64_t rows, int64_t d, int64_t o_part_stride,
                          int64_t ml_part_stride, void* out, const LaunchCtx& ctx);
+
+// The fp32 parts [batch * hq, parts] of a decode launch, merged into 16-bit rows;
+// sequence b has min(ceil(context_lens[b] / partition), parts) of them.
+struct DecodePartsArgs {
+  const float* o;
+  const float* m;
+  const float* l;
+  const int32_t* context_lens;
+  int64_t batch, hq, hkv, d, partition, parts;
+  bool skip_single;  // rows with exactly one part are already written
+  void* out;         // fp16 (or bf16) [batch, hq, d]
+  bool bf16;
+};
+cudaError_t launch_decode_merge(const DecodePartsArgs& a, const LaunchCtx& ctx);
+
+// Query heads a token's scores are stored for (the group, rounded up to a power
+// of two), and the bytes of fp32 scores [batch, hkv, max_ctx, score_heads].
+int64_t score_heads(int64_t group);
+size_t score_bytes(int64_t batch, int64_t hkv, int64_t group, int64_t max_ctx);
+
+// weights[page, h, off] += sum over the query heads of kv head h of
+// 2^(score - M) / L, with a row's M and L from its parts (csrc/evict.cu).
+struct AddWeightsArgs {
+  const float* scores;
+  const float* m;
+  const float* l;
+  const int32_t* block_tables;
+  const int32_t* context_lens;
+  float* weights;
+  int64_t batch, hq, hkv, bs, num_blocks, max_blocks, max_ctx, partition, parts;
+};
+cudaError_t launch_add_weights(const AddWeightsArgs& a, const LaunchCtx& ctx);
+
+// ------------------------------------------------------------ 4-bit paged cache
+
+struct Kv4CopyArgs {
+  void* k;              // fp16 or bf16 [tokens, hkv, d]: read (append) or written, dense (read)
+  void* v;
+  bool bf16;
+  int64_t token_stride[2], head_stride[2];  // of k and v, in elements (append)
+  void* k_cache;        // uint8 [num_blocks, hkv, bs, row bytes]
+  void* v_cache;
+  const int64_t* slots; // [tokens]
+  float* weights;       // append: [num_blocks, hkv, bs] to clear in the written slots, or null
+  int64_t tokens, hkv, d, bs, num_blocks;
+};
+cudaError_t launch_kv4_append(const Kv4CopyArgs& a, const LaunchCtx& ctx);
+cudaError_t launch_kv4_read(const Kv4CopyArgs& a, const LaunchCtx& ctx);
+
+struct Kv4DecodeArgs {
+  const void* q;        // fp16 or bf16 [batch, hq, d]
+  bool bf16;
+  const void* k_cache;  // uint8 [num_blocks, hkv, bs, row bytes]
+  const void* v_cache;
+  const int32_t* block_tables;
+  const int32_t* context_lens;
+  void* out;            // q's type [batch, hq, d]
+  float* weights;       // fp32 [num_blocks, hkv, bs] or null
+  int64_t batch, hq, hkv, d, bs, num_blocks, max_blocks, max_ctx, partition;
+  float scale;
+  void* workspace;
+  size_t workspace_bytes;
+};
+size_t kv4_decode_workspace_bytes(int64_t batch, int64_t hq, int64_t hkv, int64_t d, int64_t max_ctx,
+                                  int64_t partition, bool weights);
+cudaError_t launch_kv4_decode(const Kv4DecodeArgs& a, const LaunchCtx& ctx);
+
+// --------------------------------------------------------------------- eviction
+
+// Most cache arrays one eviction moves.
+constexpr int kMaxEvictArrays = 8;
+
+struct EvictArgs {
+  void* arrays[kMaxEvictArrays];  // [num_blocks, hkv, bs, row_bytes[i]]
+  int64_t row_bytes[kMaxEvictArrays];
+  int num_arrays;
+  float* weights;                 // [num_blocks, hkv, bs]
+  const int32_t* block_tables;    // [batch, max_blocks]
+  const int32_t* context_lens;    // [batch]
+  const int32_t* new_block_tables;  // [batch, new_max_blocks]
+  int32_t* new_lens;              // [batch]
+  int32_t* kept;                  // [batch, hkv, keep]
+  int64_t batch, hkv, bs, num_blocks, max_blocks, max_ctx, new_max_blocks, keep, recent, sinks;
+};
+cudaError_t launch_evict(const EvictArgs& a, const LaunchCtx& ctx);
 
 cudaError_t launch_selftest_wait(unsigned long long timeout_ns, const LaunchCtx& ctx);
 

@@ -222,6 +222,126 @@ int attn_paged_decode_noalloc(const void* q, const void* k_cache, const void* v_
                               int64_t max_blocks_per_seq, int64_t max_context_len, float scale,
                               int64_t partition, void* stream);
 
+/* ------------------------------------------------- attention weights, eviction */
+
+/*
+ * Bytes of workspace attn_paged_decode_weights needs: attn_paged_decode's, and
+ * fp32 scores of num_heads / num_kv_heads per (sequence, kv head, token).
+ */
+size_t attn_paged_decode_weights_workspace_bytes(int64_t batch, int64_t num_heads,
+                                                 int64_t num_kv_heads, int64_t head_dim,
+                                                 int64_t max_context_len, int64_t partition);
+
+/*
+ * attn_paged_decode that also adds each token's attention weight to the total of
+ * its cache slot: weights fp32 [num_blocks, num_kv_heads, block_size],
+ *   weights[page, h, offset] += sum over the query heads of kv head h of
+ *                               softmax(scale * q k^T)[token].
+ * Totals of other slots are left as they are. A page that stands in several
+ * sequences gets the adds of all of them (in no fixed order, so that such a
+ * total may differ in its last bits from call to call; with every page in one
+ * sequence the totals are the same each time). Lengths above max_context_len
+ * are cut to it. No counterpart in the reference.
+ */
+int attn_paged_decode_weights(const void* q, const void* k_cache, const void* v_cache,
+                              const int32_t* block_tables, const int32_t* context_lens, void* out,
+                              float* weights, int64_t batch, int64_t num_heads,
+                              int64_t num_kv_heads, int64_t head_dim, int64_t block_size,
+                              int64_t num_blocks, int64_t max_blocks_per_seq,
+                              int64_t max_context_len, float scale, int64_t partition,
+                              void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * Cut the caches of a batch to at most `keep` tokens per sequence. Per sequence
+ * and kv head the first `sinks` and the last `recent` tokens stay, and of the
+ * rest those with the largest totals in `weights` (ties to the lower index; NaN
+ * counts as the lowest); a sequence of `keep` tokens or fewer stays whole. The
+ * kept tokens, in their order, become tokens 0, 1, ... of the pages of
+ * new_block_tables [batch, new_max_blocks]: rows of `num_arrays` (1 to 8) cache
+ * arrays arrays[i], each [num_blocks, num_kv_heads, block_size, row_bytes[i]],
+ * and their totals in `weights`.
+ *   new_lens  int32 [batch]: min(length, keep)
+ *   kept      int32 [batch, num_kv_heads, keep]: the kept tokens' old indices,
+ *             ascending, then -1
+ * The pages of new_block_tables must not be pages that the sequences of the call
+ * read or write otherwise; a sequence that is not cut may give its old pages
+ * again, and is then not moved. Every other row of the arrays stays as it is, so
+ * old pages (which other sequences may share) are the caller's to free.
+ * sinks + recent <= keep. Lengths above max_context_len are cut to it. The
+ * selection walks a sequence's totals in one CTA per (sequence, kv head).
+ * No counterpart in the reference.
+ */
+int attn_paged_evict(void* const* arrays, const int64_t* row_bytes, int num_arrays, float* weights,
+                     const int32_t* block_tables, const int32_t* context_lens,
+                     const int32_t* new_block_tables, int32_t* new_lens, int32_t* kept,
+                     int64_t batch, int64_t num_kv_heads, int64_t block_size, int64_t num_blocks,
+                     int64_t max_blocks_per_seq, int64_t max_context_len, int64_t new_max_blocks,
+                     int64_t keep, int64_t recent, int64_t sinks, void* stream);
+
+/* ------------------------------------------------------------ 4-bit paged cache */
+
+/* Types of the 16-bit tensors of the 4-bit cache's entry points. */
+#define ATTN_FP16 0
+#define ATTN_BF16 1
+
+/*
+ * Bytes of one row of a 4-bit cache, K or V of one token of one kv head (80 at
+ * head_dim 128, 40 at 64; 0 for other head_dims). A cache is uint8
+ * [num_blocks, num_kv_heads, block_size, row bytes]. A row holds groups of 32
+ * values, value = low + scale * code with fp16 low and scale and codes 0..15:
+ * head_dim / 2 bytes of codes, then the scales, then the lows. With
+ * NG = head_dim / 32, 32-bit word t * NG + w of a K row holds dims
+ * 32 w + 8 t + e at bits 4 e (e < 8); 16-bit word g * NG + w of a V row holds
+ * columns 32 w + 4 g + j at bits 4 j (j < 4).
+ */
+int64_t attn_kv4_row_bytes(int64_t head_dim);
+
+/*
+ * Quantise new tokens into their slots: k, v [tokens, num_kv_heads, head_dim] of
+ * `dtype`, the last dim dense, token and head strides in elements (multiples of
+ * 8); slots int64 [tokens], slot = page * block_size + offset, a negative one
+ * meaning no token. Per group of 32: low = fp16(min), scale =
+ * fp16((max - low) / 15), code = (x - low) / scale rounded to nearest even and
+ * clamped to 0..15 (0 where the scale is 0). A group with a value outside
+ * fp16's finite range reads back as NaN. `weights`, if not null
+ * (fp32 [num_blocks, num_kv_heads, block_size]), is set to 0 in the slots. The
+ * slots of one call must differ. A slot past the cache is reported as
+ * ATTN_DEVICE_BAD_BLOCK and not written.
+ */
+int attn_kv4_append(const void* k, const void* v, int dtype, void* k_cache, void* v_cache,
+                    const int64_t* slots, float* weights, int64_t tokens, int64_t num_kv_heads,
+                    int64_t head_dim, int64_t k_token_stride, int64_t k_head_stride,
+                    int64_t v_token_stride, int64_t v_head_stride, int64_t block_size,
+                    int64_t num_blocks, void* stream);
+
+/*
+ * Read slots back: k, v [tokens, num_kv_heads, head_dim] of `dtype`, dense;
+ * value = low + scale * code, rounded once. A negative slot, or one past the
+ * cache (reported as ATTN_DEVICE_BAD_BLOCK), reads as zeros.
+ */
+int attn_kv4_read(const void* k_cache, const void* v_cache, const int64_t* slots, void* k, void* v,
+                  int dtype, int64_t tokens, int64_t num_kv_heads, int64_t head_dim,
+                  int64_t block_size, int64_t num_blocks, void* stream);
+
+/* Bytes of workspace attn_kv4_decode needs (with_weights: `weights` is given). */
+size_t attn_kv4_decode_workspace_bytes(int64_t batch, int64_t num_heads, int64_t num_kv_heads,
+                                       int64_t head_dim, int64_t max_context_len,
+                                       int64_t partition, int with_weights);
+
+/*
+ * Decode attention over a 4-bit cache: as attn_paged_decode, with q and out of
+ * `dtype`, num_heads / num_kv_heads any whole number from 1 to 8, and, where
+ * `weights` is not null, the totals of attn_paged_decode_weights. head_dim 64
+ * needs an even block_size (a page of one head is then a multiple of 16 bytes).
+ * Lengths above max_context_len are cut to it; an empty sequence gets zeros.
+ */
+int attn_kv4_decode(const void* q, int dtype, const void* k_cache, const void* v_cache,
+                    const int32_t* block_tables, const int32_t* context_lens, void* out,
+                    float* weights, int64_t batch, int64_t num_heads, int64_t num_kv_heads,
+                    int64_t head_dim, int64_t block_size, int64_t num_blocks,
+                    int64_t max_blocks_per_seq, int64_t max_context_len, float scale,
+                    int64_t partition, void* workspace, size_t workspace_bytes, void* stream);
+
 /* ------------------------------------------------------------ device status */
 
 /*
