@@ -2,7 +2,34 @@
 // (row layout: kv4.cuh), split over the context and merged like the fp16 decode
 // (decode.cu): scores in log2 units, a running maximum and sum, one fp32
 // (o, m, l) part per split.
+//
+// A token costs 160 bytes of K and V per kv head at head_dim 128 where fp16 takes
+// 512, so at the memory's rate an SM has about 7 cycles for a token: the kernel is
+// laid out to spend few instructions on it.
+//
+//   * Warps are independent pipelines over work units (sequence, kv head, split),
+//     as in decode.cu: bulk copies of whole page runs into a per-warp ring of
+//     32-token stages, signalled by mbarriers.
+//   * Both products run on the tensor cores (mma.sync m16n8k16) with the cached
+//     rows as the 16-row operand A and the query heads of the kv head as the 8
+//     columns of B, so up to 8 heads cost what one does:
+//         S^T [16 tokens x 8 heads] = K [16 x D] q^T
+//         O^T [16 columns x 8 heads] += V^T [16 x 16 tokens] P^T
+//   * Codes reach the tensor cores without arithmetic. A 4-bit code n in bits 0-3
+//     of an fp16 is the subnormal n 2^-24 (in bits 4-7: n 2^-20), which the tensor
+//     cores multiply exactly; so one AND makes two operands, and the row layout
+//     puts the codes that an operand register pairs 16 bits apart. q is halved four
+//     times for the codes in bits 4-7; of O the odd columns are divided by 16 at
+//     the end.
+//   * A group's scale stays outside the product over the codes: K has one fp32
+//     accumulator per group, combined as sum_w scale_w acc_w in fp32; V's scales
+//     multiply P (in fp16) before each group's columns. The lows are one product
+//     more: low . (sum of q over the group), with that sum as two fp16 terms (22
+//     bits), and P . low for V.
+//   * q of a head is scaled by the power of two that brings its largest value into
+//     [2^7, 2^8), so that fp16 holds every bit that matters of an fp16 or bf16 q.
 #include <algorithm>
+#include <mutex>
 
 #include "kv4.cuh"
 #include "launch.h"
@@ -10,7 +37,37 @@
 namespace fab {
 namespace {
 
-enum : unsigned int { kSiteKv4Block = 221 };
+enum : unsigned int { kSiteKv4Wait = 221, kSiteKv4Drain = 222, kSiteKv4Block = 223 };
+
+constexpr int kTok = 32;            // tokens per pipeline stage
+constexpr int kLaunchBatch = 2048;  // sequences per launch (their lengths live in shared memory)
+
+#ifndef FAB_KV4_W
+#define FAB_KV4_W 16
+#endif
+#ifndef FAB_KV4_S
+#define FAB_KV4_S 2
+#endif
+
+template <int D>
+struct Kv4Cfg {
+  using R = Kv4Row<D>;
+  static constexpr int W = FAB_KV4_W;  // warps per CTA, one CTA per SM
+  static constexpr int THREADS = W * 32;
+  static constexpr int NG = R::NG;
+  static constexpr int ROW = R::BYTES;
+  static constexpr int KV = kTok * ROW;  // K (or V) bytes of one stage
+  static constexpr int STAGE = 2 * KV;
+  static constexpr int STAGES = D == 64 ? 2 * FAB_KV4_S : FAB_KV4_S;
+  static constexpr int RING = STAGES * STAGE;
+  static constexpr int BAR_OFF = W * RING;
+  static constexpr int META_OFF = (BAR_OFF + W * STAGES * 8 + 15) / 16 * 16;
+  static constexpr int PREFIX_OFF = META_OFF + W * STAGES * 16;
+  static constexpr int CTX_OFF = PREFIX_OFF + (kLaunchBatch + 1) * 4;
+  static constexpr int SMEM = (CTX_OFF + kLaunchBatch * 4 + 15) / 16 * 16 + 16;  // + the abort flag
+  static_assert(STAGE % 16 == 0 && KV % 16 == 0 && BAR_OFF % 16 == 0, "bulk copy alignment");
+  static_assert(SMEM <= 227 * 1024, "shared memory per CTA");
+};
 
 struct Kv4DecParams {
   const void* q;          // [batch, hq, D] fp16 or bf16
@@ -18,184 +75,667 @@ struct Kv4DecParams {
   const uint8_t* vc;
   const int* bt;
   const int* ctx;
+  void* out;              // q's type [batch, hq, D]: rows of sequences with one split (direct_out)
   float* o_part;          // [batch * hq, num_splits, D]
   float* m_part;          // [batch * hq, num_splits]
   float* l_part;
-  float* scores;          // [batch, hkv, max_ctx, gp] log2-unit scores, or null
+  float* scores;          // SCORED: [batch, hkv, max_ctx, gp] log2-unit scores
+  unsigned int* counter;  // work counter, zero at launch
   DeviceStatus* status;
+  unsigned long long timeout_ns;
+  long long block_stride;  // bytes between physical blocks
   int batch, hq, hkv, group, gp, bs, max_blocks, num_blocks, partition, num_splits, max_ctx;
+  int direct_out;
   float scale_log2;
 };
 
-// One CTA per (split, kv head, sequence): its four warps take tokens in turn,
-// lane i holding dims i, i + 32, ... of every row.
-template <int D, typename T>
-__global__ void __launch_bounds__(128) kv4_decode_kernel(const Kv4DecParams p) {
-  using R = Kv4Row<D>;
-  constexpr int NG = R::NG;
-  const int split = blockIdx.x, kvh = blockIdx.y, b = blockIdx.z;
-  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-  const int ctx = min(max(p.ctx[b], 0), p.max_ctx);
-  const int t0 = split * p.partition, t1 = min(ctx, t0 + p.partition);
-  if (t0 >= ctx) return;
-  float q[8][NG], acc[8][NG], m[8], l[8];
-#pragma unroll
-  for (int g = 0; g < 8; ++g) {
-    m[g] = -INFINITY;
-    l[g] = 0.f;
-#pragma unroll
-    for (int w = 0; w < NG; ++w) {
-      acc[g][w] = 0.f;
-      q[g][w] = g < p.group ? to_f32(static_cast<const T*>(p.q)[(static_cast<size_t>(b) * p.hq +
-                                  kvh * p.group + g) * D + 32 * w + lane]) * p.scale_log2 : 0.f;
-    }
+// D (16x8, fp32) += A (16x16, fp16, rows) B (16x8, fp16, columns).
+__device__ __forceinline__ void mma_k16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2,
+                                        uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
+      "{%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// The same with A 16x8.
+__device__ __forceinline__ void mma_k8(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t b0) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k8.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5}, {%6}, "
+      "{%0, %1, %2, %3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(b0));
+}
+
+// Transpose of an 8x8 fp16 matrix whose row i lanes 4 i .. 4 i + 3 hold in pairs.
+__device__ __forceinline__ uint32_t transpose8(uint32_t a) {
+  uint32_t d;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
+  return d;
+}
+
+__device__ __forceinline__ uint32_t hmul2(uint32_t a, uint32_t b) {
+  const __half2 r = __hmul2(*reinterpret_cast<__half2*>(&a), *reinterpret_cast<__half2*>(&b));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+
+// N 32-bit words (1, 2 or 4) of shared memory in one load.
+template <int N>
+__device__ __forceinline__ void load_words(uint32_t (&r)[N], const uint8_t* p) {
+  if constexpr (N == 4) {
+    const uint4 v = *reinterpret_cast<const uint4*>(p);
+    r[0] = v.x; r[1] = v.y; r[2] = v.z; r[3] = v.w;
+  } else if constexpr (N == 2) {
+    const uint2 v = *reinterpret_cast<const uint2*>(p);
+    r[0] = v.x; r[1] = v.y;
+  } else {
+    r[0] = *reinterpret_cast<const uint32_t*>(p);
   }
-  for (int t = t0 + warp; t < t1; t += 4) {
-    int page = p.bt[static_cast<size_t>(b) * p.max_blocks + t / p.bs];
-    if (page < 0 || page >= p.num_blocks) {
-      if (lane == 0) report_status(p.status, 2u, kSiteKv4Block);
-      page = 0;
-    }
-    const size_t off =
-        ((static_cast<size_t>(page) * p.hkv + kvh) * p.bs + t % p.bs) * R::BYTES;
-    const uint8_t* kr = p.kc + off;
-    const uint8_t* vr = p.vc + off;
-    float kx[NG], vx[NG];
-#pragma unroll
-    for (int w = 0; w < NG; ++w) {
-      const uint32_t kw = reinterpret_cast<const uint32_t*>(kr)[(lane / 8) * NG + w];
-      const uint32_t vw = reinterpret_cast<const uint16_t*>(vr)[(lane / 4) * NG + w];
-      const __half* kp = reinterpret_cast<const __half*>(kr + R::CODES);
-      const __half* vp = reinterpret_cast<const __half*>(vr + R::CODES);
-      kx[w] = fmaf(__half2float(kp[w]), static_cast<float>((kw >> (4 * (lane % 8))) & 15u),
-                   __half2float(kp[NG + w]));
-      vx[w] = fmaf(__half2float(vp[w]), static_cast<float>((vw >> (4 * (lane % 4))) & 15u),
-                   __half2float(vp[NG + w]));
-    }
-#pragma unroll
-    for (int g = 0; g < 8; ++g) {
-      if (g >= p.group) break;
-      float s = 0.f;
-#pragma unroll
-      for (int w = 0; w < NG; ++w) s = fmaf(q[g][w], kx[w], s);
-      s = warp_sum(s);
-      if (p.scores != nullptr && lane == 0)
-        p.scores[((static_cast<size_t>(b) * p.hkv + kvh) * p.max_ctx + t) * p.gp + g] = s;
-      const float mn = fmaxf(m[g], s);
-      const float alpha = exp2f(m[g] - mn), e = exp2f(s - mn);
-      l[g] = l[g] * alpha + e;
-      m[g] = mn;
-#pragma unroll
-      for (int w = 0; w < NG; ++w) acc[g][w] = fmaf(e, vx[w], acc[g][w] * alpha);
-    }
-  }
-  __shared__ float so[4][8][D], sm[4][8], sl[4][8];
-#pragma unroll
-  for (int g = 0; g < 8; ++g) {
-#pragma unroll
-    for (int w = 0; w < NG; ++w) so[warp][g][32 * w + lane] = acc[g][w];
-    sm[warp][g] = m[g];
-    sl[warp][g] = l[g];
+}
+
+// 2^e as a float, -126 <= e <= 127.
+__device__ __forceinline__ float pow2i(int e) { return __int_as_float((e + 127) << 23); }
+
+template <int D, typename T, bool SCORED>
+__global__ void __launch_bounds__(Kv4Cfg<D>::THREADS, 1) kv4_decode_kernel(const Kv4DecParams p) {
+  using C = Kv4Cfg<D>;
+  constexpr int NG = C::NG, ROW = C::ROW, CODES = C::R::CODES;
+  extern __shared__ __align__(128) uint8_t smem[];
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+  const int g4 = lane >> 2, t4 = lane & 3;
+  uint8_t* ring = smem + warp * C::RING;
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::BAR_OFF) + warp * C::STAGES;
+  int4* meta = reinterpret_cast<int4*>(smem + C::META_OFF) + warp * C::STAGES;
+  int* prefix = reinterpret_cast<int*>(smem + C::PREFIX_OFF);
+  int* ctx_s = reinterpret_cast<int*>(smem + C::CTX_OFF);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + C::SMEM - 16);
+  // The merge that follows may be scheduled now; it waits for this launch's end
+  // before it reads the parts.
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+
+  // Lengths and the prefix sums of the splits per sequence: active (sequence,
+  // split) pairs are numbered densely, v in [0, prefix[batch]).
+  for (int b = threadIdx.x; b < p.batch; b += C::THREADS)
+    ctx_s[b] = min(max(p.ctx[b], 0), p.max_ctx);
+  if (threadIdx.x < C::W * C::STAGES)
+    mbar_init(reinterpret_cast<uint64_t*>(smem + C::BAR_OFF) + threadIdx.x, 1);
+  if (threadIdx.x == 0) {
+    *abort_flag = 0;
+    fence_mbar_init();
   }
   __syncthreads();
-  for (int g = warp; g < p.group; g += 4) {
-    const float mx = fmaxf(fmaxf(sm[0][g], sm[1][g]), fmaxf(sm[2][g], sm[3][g]));
-    float a[4], den = 0.f;
-    for (int i = 0; i < 4; ++i) {
-      a[i] = sm[i][g] == -INFINITY ? (sl[i][g] != sl[i][g] ? 1.f : 0.f) : exp2f(sm[i][g] - mx);
-      den += a[i] * sl[i][g];
+  if (warp == 0) {
+    const int per = (p.batch + 31) / 32;
+    const int b0 = lane * per;
+    int sum = 0;
+    for (int i = 0; i < per; ++i)
+      if (b0 + i < p.batch) sum += (ctx_s[b0 + i] + p.partition - 1) / p.partition;
+    int incl = sum;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += y;
     }
-    const size_t pr = (static_cast<size_t>(b) * p.hq + kvh * p.group + g) * p.num_splits + split;
-    for (int w = 0; w < NG; ++w) {
-      float num = 0.f;
-      for (int i = 0; i < 4; ++i) num += a[i] * so[i][g][32 * w + lane];
-      p.o_part[pr * D + 32 * w + lane] = num / den;
+    int run = incl - sum;
+    for (int i = 0; i < per; ++i) {
+      if (b0 + i < p.batch) {
+        prefix[b0 + i] = run;
+        run += (ctx_s[b0 + i] + p.partition - 1) / p.partition;
+      }
     }
+    if (lane == 31) prefix[p.batch] = incl;
+  }
+  __syncthreads();
+  // Without a merge pass, rows of empty sequences are written here (zeros).
+  if (p.direct_out && p.num_splits == 1 && blockIdx.x == 0) {
+    for (int b = warp; b < p.batch; b += C::W) {
+      if (ctx_s[b] != 0) continue;
+      uint32_t* dst = static_cast<uint32_t*>(p.out) + static_cast<size_t>(b) * p.hq * (D / 2);
+      for (int i = lane; i < p.hq * (D / 2); i += 32) dst[i] = 0u;
+    }
+  }
+  const int total_units = prefix[p.batch] * p.hkv;
+
+  // ---------------------------------------------------------- producer state
+  int pu = -1, pb = 0, pkvh = 0, psplit = 0, pstart = 0, pend = 0, pst = 0, pnst = 0;
+  // Block-table entries [bt_base, bt_base + 32) and the next 32, one per lane:
+  // the second window is on its way while the first is used.
+  int bt_base = 0, bt_cur = 0, bt_next = 0;
+  unsigned int nxt = 0;  // next unit id (valid in lane 0), fetched one unit ahead
+  unsigned int p_item = 0, c_item = 0;
+
+  auto table = [&](int pg) {
+    return pg < p.max_blocks ? p.bt[static_cast<size_t>(pb) * p.max_blocks + pg] : 0;
+  };
+
+  auto advance = [&]() {
+    const int u = static_cast<int>(__shfl_sync(0xffffffffu, nxt, 0));
+    if (u >= total_units) {
+      pu = -1;
+      return;
+    }
+    pu = u;
+    const int v = u / p.hkv;
+    pkvh = u - v * p.hkv;
+    int lo = 0, hi = p.batch - 1;  // last sequence whose first pair is <= v
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if (prefix[mid] <= v) lo = mid; else hi = mid - 1;
+    }
+    pb = lo;
+    psplit = v - prefix[lo];
+    pstart = psplit * p.partition;
+    pend = min(ctx_s[pb], pstart + p.partition);
+    pst = 0;
+    pnst = (pend - pstart + kTok - 1) / kTok;
+    bt_base = pstart / p.bs;
+    bt_cur = table(bt_base + lane);
+    bt_next = table(bt_base + 32 + lane);
+    if (lane == 0) nxt = C::W * gridDim.x + atomicAdd(p.counter, 1u);
+  };
+
+  // Issue the copies of the producer's next stage into its ring slot: a stage
+  // spans at most 32 pages, each lane copies one page's K and V rows.
+  auto produce = [&]() {
+    if (pu < 0) return;
+    const unsigned int slot = p_item % C::STAGES;
+    uint8_t* st = ring + slot * C::STAGE;
+    uint64_t* bar = full + slot;
+    const int t0 = pstart + pst * kTok;
+    int t1 = min(t0 + kTok, pend);
+    const int nt = t1 - t0;
+    // Copies are of whole 16 bytes: where a row is not (40 bytes), an odd last token
+    // brings the row after it along, which is in its page (the block size is even).
+    if constexpr (ROW % 16 != 0) t1 += t1 & 1;
     if (lane == 0) {
-      // A part whose scores are all NaN has no maximum, yet is not an empty one.
-      p.m_part[pr] = den != den ? fmaxf(mx, 0.f) : mx;
-      p.l_part[pr] = den;
+      mbar_arrive_expect_tx(bar, 2 * (t1 - t0) * ROW);
+      meta[slot] = make_int4(pb, pkvh, psplit,
+                             nt | ((pst == 0) ? 64 : 0) | ((pst == pnst - 1) ? 128 : 0));
     }
+    const int pg0 = t0 / p.bs, pages = (t1 - 1) / p.bs - pg0 + 1;
+    if (pg0 - bt_base >= 32) {
+      bt_base += 32;
+      bt_cur = bt_next;
+      bt_next = table(bt_base + 32 + lane);
+    }
+    const int rel = pg0 + lane - bt_base;  // below 64
+    const int cur = __shfl_sync(0xffffffffu, bt_cur, rel & 31);
+    const int next = __shfl_sync(0xffffffffu, bt_next, rel & 31);
+    __syncwarp();  // the expected bytes are set before any copy completes
+    if (lane < pages) {
+      int page = rel < 32 ? cur : next;
+      if (page < 0 || page >= p.num_blocks) {  // never read outside the cache
+        report_status(p.status, 2u /* ATTN_DEVICE_BAD_BLOCK */, kSiteKv4Block);
+        page = 0;
+      }
+      const int first = (pg0 + lane) * p.bs;
+      const int from = max(first, t0), to = min(first + p.bs, t1);
+      const long long src = page * p.block_stride +
+                            (static_cast<long long>(pkvh) * p.bs + (from - first)) * ROW;
+      const uint32_t bytes = static_cast<uint32_t>(to - from) * ROW;
+      uint8_t* dst = st + (from - t0) * ROW;
+      bulk_g2s(dst, p.kc + src, bytes, bar);
+      bulk_g2s(dst + C::KV, p.vc + src, bytes, bar);
+    }
+    ++p_item;
+    if (++pst == pnst) advance();
+    __syncwarp();
+  };
+
+  // ---------------------------------------------------------- consumer state
+  // Fragments (lane = 4 g4 + t4): B of S^T: head g4, dims 32 w + 8 t4 + e; D of
+  // S^T: tokens of rows g4 and g4 + 8, heads 2 t4 and 2 t4 + 1; D of O^T: of group
+  // w columns 32 w + 4 g4 + {0, 2} (acc[w][0]) and {1, 3} (acc[w][1], times 16),
+  // the same heads. Row r of a 16-token tile is token tau(r):
+  //     tau(2 i) = 2 i, tau(2 i + 1) = (2 i + 4) % 8 + 8, tau(r + 8) = tau(r) + 1,
+  // which makes the loads of 80-byte rows free of bank conflicts, K (8 lanes: two
+  // rows 4 or 12 apart) as well as V (16 lanes: four even or four odd rows).
+  uint32_t qf[NG][4];  // b0, b1 of the codes in bits 0-3, then of those in bits 4-7
+  uint32_t qs = 0;     // B of the lows' product: the groups' sums of q
+  float f[2];          // scale * log2(e) over q's power of two, per head
+  float m[2], l[2];    // running maximum; this lane's share of the sum, times 4
+  float acc[NG][2][4], z[4];
+  float* sc = nullptr;  // SCORED: the scores of the stage's first token
+  const int tok_k = (g4 & 1) ? ((g4 + 3) & 7) + 8 : g4;  // tau(g4)
+  const int tok_v = ((2 * t4 + 4) & 7) + 8;              // tau(2 t4 + 1)
+
+  auto load_q = [&](int b, int kvh) {
+    const bool real = g4 < p.group;
+    const T* src = static_cast<const T*>(p.q) +
+                   (static_cast<size_t>(b) * p.hq + kvh * p.group + g4) * D + 8 * t4;
+    uint4 raw[NG];
+#pragma unroll
+    for (int w = 0; w < NG; ++w)
+      raw[w] = real ? *reinterpret_cast<const uint4*>(src + 32 * w) : make_uint4(0u, 0u, 0u, 0u);
+    float big = 0.f;
+#pragma unroll
+    for (int w = 0; w < NG; ++w)
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        big = fmaxf(big, fabsf(to_f32(reinterpret_cast<const T*>(&raw[w])[e])));
+    big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 1));
+    big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
+    // k: big * 2^k in [2^7, 2^8); 0 for a zero or infinite q.
+    const int e8 = (__float_as_int(big) >> 23) & 255;
+    const int k = big == 0.f || e8 == 255 ? 0 : min(134 - e8, 126);
+    const float up = pow2i(k);
+    float sums[NG];
+#pragma unroll
+    for (int w = 0; w < NG; ++w) {
+      float x[8];
+      sums[w] = 0.f;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        x[e] = to_f32(reinterpret_cast<const T*>(&raw[w])[e]) * up;
+        sums[w] += x[e];
+      }
+      qf[w][0] = pack_half2(x[0], x[4]);
+      qf[w][1] = pack_half2(x[2], x[6]);
+      qf[w][2] = pack_half2(x[1] * 0.0625f, x[5] * 0.0625f);
+      qf[w][3] = pack_half2(x[3] * 0.0625f, x[7] * 0.0625f);
+      sums[w] += __shfl_xor_sync(0xffffffffu, sums[w], 1);
+      sums[w] += __shfl_xor_sync(0xffffffffu, sums[w], 2);
+    }
+    // k slots of the lows' product: the groups' sums rounded to fp16, then what
+    // that left over; slots past 2 NG are 0.
+    float s0 = sums[0], s1 = sums[1];
+    if (NG == 4 && (t4 & 1)) {
+      s0 = sums[NG - 2];
+      s1 = sums[NG - 1];
+    }
+    const float h0 = __half2float(__float2half_rn(s0)), h1 = __half2float(__float2half_rn(s1));
+    const bool rest = t4 >= NG / 2;
+    qs = rest ? pack_half2(s0 - h0, s1 - h1) : pack_half2(h0, h1);
+    if (NG == 2 && t4 >= 2) qs = 0u;
+    const float fh = p.scale_log2 * pow2i(-k);
+    f[0] = __shfl_sync(0xffffffffu, fh, 8 * t4);
+    f[1] = __shfl_sync(0xffffffffu, fh, 8 * t4 + 4);
+  };
+
+  auto consume = [&]() -> bool {
+    const unsigned int slot = c_item % C::STAGES;
+    const uint32_t parity = (c_item / C::STAGES) & 1u;
+    const int4 md = meta[slot];
+    const uint8_t* kst = ring + slot * C::STAGE;
+    uint8_t* vst = ring + slot * C::STAGE + C::KV;
+    const int nt = md.w & 63;
+    if (md.w & 64) {
+      load_q(md.x, md.y);
+      m[0] = m[1] = -INFINITY;
+      l[0] = l[1] = 0.f;
+#pragma unroll
+      for (int w = 0; w < NG; ++w)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[w][0][i] = acc[w][1][i] = 0.f;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) z[i] = 0.f;
+    }
+    if constexpr (SCORED) {
+      sc = (md.w & 64) ? p.scores + ((static_cast<size_t>(md.x) * p.hkv + md.y) * p.max_ctx +
+                                     static_cast<size_t>(md.z) * p.partition) * p.gp
+                       : sc + kTok * p.gp;
+    }
+    const bool ok = mbar_wait(full + slot, parity, abort_flag, p.status, kSiteKv4Wait,
+                              p.timeout_ns);
+    if (!__all_sync(0xffffffffu, ok)) return false;
+
+    // Scores of the stage's tokens: s[i][0..1] token 16 i + tok_k, s[i][2..3] the
+    // token after it.
+    float s[2][4];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const uint8_t* ra = kst + (16 * i + tok_k) * ROW;
+      const uint8_t* rb = ra + ROW;
+      uint32_t xa[NG], xb[NG];
+      load_words<NG>(xa, ra + 4 * NG * t4);
+      load_words<NG>(xb, rb + 4 * NG * t4);
+      uint32_t sa[NG / 2], sb[NG / 2];  // scales
+      load_words<NG / 2>(sa, ra + CODES);
+      load_words<NG / 2>(sb, rb + CODES);
+      const int low = CODES + 2 * NG + (NG == 4 ? 4 * (t4 & 1) : 0);
+      float lows[4] = {0.f, 0.f, 0.f, 0.f};
+      mma_k8(lows, *reinterpret_cast<const uint32_t*>(ra + low),
+             *reinterpret_cast<const uint32_t*>(rb + low), qs);
+      float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int w = 0; w < NG; ++w) {
+        float d[4] = {0.f, 0.f, 0.f, 0.f};
+        const uint32_t ya = xa[w] >> 8, yb = xb[w] >> 8;
+        mma_k16(d, xa[w] & 0x000F000Fu, xb[w] & 0x000F000Fu, ya & 0x000F000Fu, yb & 0x000F000Fu,
+                qf[w][0], qf[w][1]);
+        mma_k16(d, xa[w] & 0x00F000F0u, xb[w] & 0x00F000F0u, ya & 0x00F000F0u, yb & 0x00F000F0u,
+                qf[w][2], qf[w][3]);
+        const __half2 pa = *reinterpret_cast<const __half2*>(&sa[w / 2]);
+        const __half2 pb = *reinterpret_cast<const __half2*>(&sb[w / 2]);
+        const float fa = w % 2 == 0 ? __low2float(pa) : __high2float(pa);
+        const float fb = w % 2 == 0 ? __low2float(pb) : __high2float(pb);
+        sum[0] = fmaf(fa, d[0], sum[0]);
+        sum[1] = fmaf(fa, d[1], sum[1]);
+        sum[2] = fmaf(fb, d[2], sum[2]);
+        sum[3] = fmaf(fb, d[3], sum[3]);
+      }
+#pragma unroll
+      for (int c = 0; c < 4; ++c) s[i][c] = fmaf(sum[c], 0x1p24f, lows[c]) * f[c & 1];
+    }
+    if (nt < kTok) {
+      // Past the last token: no score; the ring's old bytes there must not reach
+      // the products as a NaN scale or low either.
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+          if (16 * i + tok_k + (c >> 1) >= nt) s[i][c] = -INFINITY;
+      if (lane >= nt) {
+        uint32_t* par = reinterpret_cast<uint32_t*>(vst + lane * ROW + CODES);
+#pragma unroll
+        for (int w = 0; w < NG; ++w) par[w] = 0u;
+      }
+      __syncwarp();
+    }
+    if constexpr (SCORED) {
+      if (2 * t4 < p.gp) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const int tok = 16 * i + tok_k + h;
+            if (tok < nt) {
+              if (p.gp == 1)
+                sc[tok] = s[i][2 * h];
+              else
+                *reinterpret_cast<float2*>(sc + tok * p.gp + 2 * t4) =
+                    make_float2(s[i][2 * h], s[i][2 * h + 1]);
+            }
+          }
+      }
+    }
+    // Online softmax: per head the maximum over the 8 lanes of its 32 scores. P is
+    // held times 4, which keeps small P * scale in fp16's normal range longer and
+    // cannot overflow (a scale is at most 8734).
+    float alpha[2], shift[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      float mx = fmaxf(fmaxf(s[0][h], s[0][h + 2]), fmaxf(s[1][h], s[1][h + 2]));
+      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+      mx = fmaxf(mx, m[h]);
+      alpha[h] = fast_exp2(m[h] - mx);
+      m[h] = mx;
+      shift[h] = mx - 2.f;
+    }
+    uint32_t pf[2][2];  // P^T as B fragments: tokens of rows 2 t4, 2 t4 + 1 (+ 8), head g4
+    float add[2] = {0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      float e[4];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        e[c] = fast_exp2(s[i][c] - shift[c & 1]);
+        add[c & 1] += e[c];
+      }
+      pf[i][0] = transpose8(pack_half2(e[0], e[1]));
+      pf[i][1] = transpose8(pack_half2(e[2], e[3]));
+    }
+    l[0] = fmaf(l[0], alpha[0], add[0]);
+    l[1] = fmaf(l[1], alpha[1], add[1]);
+    if (__any_sync(0xffffffffu, alpha[0] != 1.f || alpha[1] != 1.f)) {
+#pragma unroll
+      for (int w = 0; w < NG; ++w)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          acc[w][0][i] *= alpha[i & 1];
+          acc[w][1][i] *= alpha[i & 1];
+        }
+      z[0] *= alpha[0];
+      z[1] *= alpha[1];
+    }
+    // O^T += V^T P^T.
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const uint8_t* ra = vst + (16 * i + 2 * t4) * ROW;  // rows 2 t4 and (below, + ROW) 2 t4 + 8
+      const uint8_t* rb = vst + (16 * i + tok_v) * ROW;   // rows 2 t4 + 1 and 2 t4 + 9
+      uint32_t va[NG / 2], vb[NG / 2], vc[NG / 2], vd[NG / 2];
+      load_words<NG / 2>(va, ra + 2 * NG * g4);
+      load_words<NG / 2>(vb, rb + 2 * NG * g4);
+      load_words<NG / 2>(vc, ra + ROW + 2 * NG * g4);
+      load_words<NG / 2>(vd, rb + ROW + 2 * NG * g4);
+      uint32_t sa[NG / 2], sb[NG / 2], sc2[NG / 2], sd[NG / 2];
+      load_words<NG / 2>(sa, ra + CODES);
+      load_words<NG / 2>(sb, rb + CODES);
+      load_words<NG / 2>(sc2, ra + ROW + CODES);
+      load_words<NG / 2>(sd, rb + ROW + CODES);
+      // Lows of group g4 % NG (rows g4 >= NG repeat them and are not used).
+      const int low = CODES + 2 * NG + (NG == 4 ? 2 * (g4 & 2) : 0);
+      const uint32_t pick = (g4 & 1) ? 0x7632u : 0x5410u;
+      mma_k16(z,
+              __byte_perm(*reinterpret_cast<const uint32_t*>(ra + low),
+                          *reinterpret_cast<const uint32_t*>(rb + low), pick), 0u,
+              __byte_perm(*reinterpret_cast<const uint32_t*>(ra + ROW + low),
+                          *reinterpret_cast<const uint32_t*>(rb + ROW + low), pick), 0u,
+              pf[i][0], pf[i][1]);
+#pragma unroll
+      for (int w = 0; w < NG; ++w) {
+        const uint32_t half = w % 2 == 0 ? 0x5410u : 0x7632u;
+        const uint32_t b0 = hmul2(pf[i][0], __byte_perm(sa[w / 2], sb[w / 2], half));
+        const uint32_t b1 = hmul2(pf[i][1], __byte_perm(sc2[w / 2], sd[w / 2], half));
+        const uint32_t x = __byte_perm(va[w / 2], vb[w / 2], half);
+        const uint32_t y = __byte_perm(vc[w / 2], vd[w / 2], half);
+        const uint32_t x8 = x >> 8, y8 = y >> 8;
+        mma_k16(acc[w][0], x & 0x000F000Fu, x8 & 0x000F000Fu, y & 0x000F000Fu, y8 & 0x000F000Fu,
+                b0, b1);
+        mma_k16(acc[w][1], x & 0x00F000F0u, x8 & 0x00F000F0u, y & 0x00F000F0u, y8 & 0x00F000F0u,
+                b0, b1);
+      }
+    }
+    if (md.w & 128) {
+      const int ns = (ctx_s[md.x] + p.partition - 1) / p.partition;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+#pragma unroll
+        for (int o = 4; o < 32; o <<= 1) l[h] += __shfl_xor_sync(0xffffffffu, l[h], o);
+        const float inv = 1.f / l[h];
+        const int head = 2 * t4 + h;
+        const size_t row = static_cast<size_t>(md.x) * p.hq + md.y * p.group + head;
+        const size_t pr = row * p.num_splits + md.z;
+#pragma unroll
+        for (int w = 0; w < NG; ++w) {
+          const float low = __shfl_sync(0xffffffffu, z[h], 4 * w + t4);
+          float o[4];
+          o[0] = fmaf(acc[w][0][h], 0x1p24f, low) * inv;
+          o[1] = fmaf(acc[w][1][h], 0x1p20f, low) * inv;
+          o[2] = fmaf(acc[w][0][h + 2], 0x1p24f, low) * inv;
+          o[3] = fmaf(acc[w][1][h + 2], 0x1p20f, low) * inv;
+          if (head < p.group) {
+            const int col = 32 * w + 4 * g4;
+            if (p.direct_out && ns == 1)
+              *reinterpret_cast<uint2*>(static_cast<T*>(p.out) + row * D + col) =
+                  make_uint2(pack2<T>(o[0], o[1]), pack2<T>(o[2], o[3]));
+            else
+              *reinterpret_cast<float4*>(p.o_part + pr * D + col) =
+                  make_float4(o[0], o[1], o[2], o[3]);
+          }
+        }
+        if (head < p.group && g4 == 0 && !(p.direct_out && ns == 1)) {
+          // A part whose scores are all NaN has no maximum, yet is not an empty one.
+          p.m_part[pr] = l[h] != l[h] ? fmaxf(m[h], 0.f) : m[h];
+          p.l_part[pr] = 0.25f * l[h];
+        }
+      }
+    }
+    __syncwarp();
+    ++c_item;
+    return true;
+  };
+
+  // First unit: warp w of CTA c takes unit w * grid + c, so a launch with fewer
+  // units than warps spreads them over all SMs; later units come from the counter.
+  nxt = warp * gridDim.x + blockIdx.x;
+  advance();
+  for (int i = 0; i < C::STAGES; ++i) produce();
+  while (c_item < p_item) {
+    if (!consume()) break;
+    // The slot just read is refilled by the async proxy.
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    produce();
+  }
+  // Never exit with a copy in flight (only reached with copies pending after a timeout).
+  while (c_item < p_item) {
+    const unsigned int slot = c_item % C::STAGES;
+    mbar_wait(full + slot, (c_item / C::STAGES) & 1u, nullptr, p.status, kSiteKv4Drain,
+              p.timeout_ns);
+    ++c_item;
   }
 }
 
 size_t align256(size_t x) { return (x + 255) & ~static_cast<size_t>(255); }
 
 struct Workspace {
+  unsigned int* counters;
   float *o, *m, *l, *scores;
   size_t bytes;
 };
 
-Workspace carve(void* base, int64_t rows, int64_t d, int64_t splits, size_t score_bytes) {
+int64_t launches_of(int64_t batch) { return (batch + kLaunchBatch - 1) / kLaunchBatch; }
+
+Workspace carve(void* base, int64_t batch, int64_t hq, int64_t d, int64_t splits,
+                size_t score_bytes) {
   uint8_t* b = static_cast<uint8_t*>(base);
-  const size_t ob = align256(static_cast<size_t>(rows) * splits * d * 4);
-  const size_t ml = align256(static_cast<size_t>(rows) * splits * 4);
+  const size_t rows = static_cast<size_t>(batch) * hq;
+  const size_t cb = align256(static_cast<size_t>(launches_of(batch)) * 4);
+  const size_t ob = align256(rows * splits * d * 4);
+  const size_t ml = align256(rows * splits * 4);
   Workspace w;
-  w.o = reinterpret_cast<float*>(b);
-  w.m = reinterpret_cast<float*>(b + ob);
-  w.l = reinterpret_cast<float*>(b + ob + ml);
-  w.scores = reinterpret_cast<float*>(b + ob + 2 * ml);
-  w.bytes = ob + 2 * ml + align256(score_bytes);
+  w.counters = reinterpret_cast<unsigned int*>(b);
+  w.o = reinterpret_cast<float*>(b + cb);
+  w.m = reinterpret_cast<float*>(b + cb + ob);
+  w.l = reinterpret_cast<float*>(b + cb + ob + ml);
+  w.scores = reinterpret_cast<float*>(b + cb + ob + 2 * ml);
+  w.bytes = cb + ob + 2 * ml + align256(score_bytes);
   return w;
+}
+
+int64_t splits_of(int64_t max_ctx, int64_t partition) {
+  return (max_ctx + partition - 1) / partition;
+}
+
+// Sub-splits, as in decode.cu: a call with few units cuts each partition into 2 or
+// 4 (at least 64 tokens) that are merged like splits. The cap goes by sizes alone
+// (the workspace is made for it); the launch takes what its warps can use.
+int64_t sub_split_cap(int64_t batch, int64_t hq, int64_t max_ctx, int64_t partition) {
+  const int64_t rows = batch * hq * splits_of(max_ctx, partition);
+  for (int64_t k = 4; k > 1; k /= 2)
+    if (partition / k >= 64 && rows * k <= 8192) return k;
+  return 1;
+}
+
+template <int D, typename T, bool SCORED>
+cudaError_t launch_kernel(const Kv4DecParams& p, int64_t upper_units, const LaunchCtx& ctx) {
+  using C = Kv4Cfg<D>;
+  auto kern = kv4_decode_kernel<D, T, SCORED>;
+  // Per device: a function's attributes belong to the device that is current.
+  static std::mutex mu;
+  static bool done[64] = {};
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
+  {
+    std::lock_guard<std::mutex> lock(mu);
+    if (!done[dev]) {
+      e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
+      if (e != cudaSuccess) return e;
+      done[dev] = true;
+    }
+  }
+  // One CTA per SM, or one per unit when there are fewer units than SMs.
+  const int grid =
+      static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(ctx.sm_count, upper_units)));
+  kern<<<grid, C::THREADS, C::SMEM, ctx.stream>>>(p);
+  return cudaGetLastError();
+}
+
+template <int D, typename T>
+cudaError_t dispatch(const Kv4DecParams& p, int64_t units, const LaunchCtx& ctx) {
+  return p.scores != nullptr ? launch_kernel<D, T, true>(p, units, ctx)
+                             : launch_kernel<D, T, false>(p, units, ctx);
 }
 
 }  // namespace
 
 size_t kv4_decode_workspace_bytes(int64_t batch, int64_t hq, int64_t hkv, int64_t d, int64_t max_ctx,
                                   int64_t partition, bool weights) {
-  const int64_t splits = (max_ctx + partition - 1) / partition;
-  return carve(nullptr, batch * hq, d, splits,
+  const int64_t cap = sub_split_cap(batch, hq, max_ctx, partition);
+  return carve(nullptr, batch, hq, d, splits_of(max_ctx, partition / cap),
                weights ? score_bytes(batch, hkv, hq / hkv, max_ctx) : 0).bytes;
 }
 
 cudaError_t launch_kv4_decode(const Kv4DecodeArgs& a, const LaunchCtx& ctx) {
-  const int64_t splits = (a.max_ctx + a.partition - 1) / a.partition;
+  const int64_t warps =
+      static_cast<int64_t>(a.d == 64 ? Kv4Cfg<64>::W : Kv4Cfg<128>::W) * ctx.sm_count;
+  int64_t k = sub_split_cap(a.batch, a.hq, a.max_ctx, a.partition);
+  while (k > 1 && a.batch * a.hkv * splits_of(a.max_ctx, a.partition) * k > warps) k /= 2;
+  const int64_t part = a.partition / k;
+  const int64_t splits = splits_of(a.max_ctx, part);
   const int64_t group = a.hq / a.hkv;
+  const bool scored = a.weights != nullptr;
   if (splits == 0)
     return cudaMemsetAsync(a.out, 0, static_cast<size_t>(a.batch) * a.hq * a.d * 2, ctx.stream);
-  Workspace w = carve(a.workspace, a.batch * a.hq, a.d, splits,
-                      a.weights != nullptr ? score_bytes(a.batch, a.hkv, group, a.max_ctx) : 0);
-  Kv4DecParams p;
-  p.q = a.q;
-  p.kc = static_cast<const uint8_t*>(a.k_cache);
-  p.vc = static_cast<const uint8_t*>(a.v_cache);
-  p.bt = a.block_tables;
-  p.ctx = a.context_lens;
-  p.o_part = w.o;
-  p.m_part = w.m;
-  p.l_part = w.l;
-  p.scores = a.weights != nullptr ? w.scores : nullptr;
-  p.status = ctx.status;
-  p.batch = static_cast<int>(a.batch);
-  p.hq = static_cast<int>(a.hq);
-  p.hkv = static_cast<int>(a.hkv);
-  p.group = static_cast<int>(group);
-  p.gp = static_cast<int>(score_heads(group));
-  p.bs = static_cast<int>(a.bs);
-  p.max_blocks = static_cast<int>(a.max_blocks);
-  p.num_blocks = static_cast<int>(a.num_blocks);
-  p.partition = static_cast<int>(a.partition);
-  p.num_splits = static_cast<int>(splits);
-  p.max_ctx = static_cast<int>(a.max_ctx);
-  p.scale_log2 = a.scale * kLog2e;
-  const dim3 grid(static_cast<unsigned>(splits), static_cast<unsigned>(a.hkv),
-                  static_cast<unsigned>(a.batch));
-  if (a.d == 64) {
-    if (a.bf16) kv4_decode_kernel<64, __nv_bfloat16><<<grid, 128, 0, ctx.stream>>>(p);
-    else kv4_decode_kernel<64, __half><<<grid, 128, 0, ctx.stream>>>(p);
-  } else {
-    if (a.bf16) kv4_decode_kernel<128, __nv_bfloat16><<<grid, 128, 0, ctx.stream>>>(p);
-    else kv4_decode_kernel<128, __half><<<grid, 128, 0, ctx.stream>>>(p);
-  }
-  cudaError_t e = cudaGetLastError();
+  Workspace w = carve(a.workspace, a.batch, a.hq, a.d, splits,
+                      scored ? score_bytes(a.batch, a.hkv, group, a.max_ctx) : 0);
+  const int64_t launches = launches_of(a.batch);
+  cudaError_t e = cudaMemsetAsync(w.counters, 0, static_cast<size_t>(launches) * 4, ctx.stream);
   if (e != cudaSuccess) return e;
-  DecodePartsArgs f{w.o, w.m, w.l, a.context_lens, a.batch, a.hq, a.hkv, a.d, a.partition, splits,
-                    false, a.out, a.bf16};
-  e = launch_decode_merge(f, ctx);
-  if (e != cudaSuccess || a.weights == nullptr) return e;
+  for (int64_t i = 0; i < launches; ++i) {
+    const int64_t b0 = i * kLaunchBatch, nb = std::min<int64_t>(kLaunchBatch, a.batch - b0);
+    const int64_t row_bytes = a.d / 2 + a.d / 8, row0 = b0 * a.hq;
+    Kv4DecParams p;
+    p.q = static_cast<const uint8_t*>(a.q) + row0 * a.d * 2;
+    p.kc = static_cast<const uint8_t*>(a.k_cache);
+    p.vc = static_cast<const uint8_t*>(a.v_cache);
+    p.bt = a.block_tables + b0 * a.max_blocks;
+    p.ctx = a.context_lens + b0;
+    p.out = static_cast<uint8_t*>(a.out) + row0 * a.d * 2;
+    p.o_part = w.o + row0 * splits * a.d;
+    p.m_part = w.m + row0 * splits;
+    p.l_part = w.l + row0 * splits;
+    p.gp = static_cast<int>(score_heads(group));
+    p.scores = scored ? w.scores + static_cast<size_t>(b0) * a.hkv * a.max_ctx * p.gp : nullptr;
+    p.counter = w.counters + i;
+    p.status = ctx.status;
+    p.timeout_ns = ctx.timeout_ns;
+    p.block_stride = a.hkv * a.bs * row_bytes;
+    p.batch = static_cast<int>(nb);
+    p.hq = static_cast<int>(a.hq);
+    p.hkv = static_cast<int>(a.hkv);
+    p.group = static_cast<int>(group);
+    p.bs = static_cast<int>(a.bs);
+    p.max_blocks = static_cast<int>(a.max_blocks);
+    p.num_blocks = static_cast<int>(a.num_blocks);
+    p.partition = static_cast<int>(part);
+    p.num_splits = static_cast<int>(splits);
+    p.max_ctx = static_cast<int>(a.max_ctx);
+    p.direct_out = scored ? 0 : 1;
+    p.scale_log2 = a.scale * kLog2e;
+    const int64_t units = nb * a.hkv * splits;
+    if (a.d == 64)
+      e = a.bf16 ? dispatch<64, __nv_bfloat16>(p, units, ctx) : dispatch<64, __half>(p, units, ctx);
+    else
+      e = a.bf16 ? dispatch<128, __nv_bfloat16>(p, units, ctx)
+                 : dispatch<128, __half>(p, units, ctx);
+    if (e != cudaSuccess) return e;
+  }
+  if (splits > 1 || scored) {
+    e = launch_decode_merge({w.o, w.m, w.l, a.context_lens, a.batch, a.hq, a.hkv, a.d, part, splits,
+                             !scored, a.out, a.bf16}, ctx);
+    if (e != cudaSuccess) return e;
+  }
+  if (!scored) return cudaSuccess;
   return launch_add_weights({w.scores, w.m, w.l, a.block_tables, a.context_lens, a.weights, a.batch,
-                             a.hq, a.hkv, a.bs, a.num_blocks, a.max_blocks, a.max_ctx, a.partition,
-                             splits}, ctx);
+                             a.hq, a.hkv, a.bs, a.num_blocks, a.max_blocks, a.max_ctx, part, splits},
+                            ctx);
 }
 
 }  // namespace fab
