@@ -57,9 +57,9 @@ SIGNATURES = {
     "attn_kv4_append": (_int, [_vp, _vp, _int, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64,
                                _i64, _i64, _i64, _i64, _vp]),
     "attn_kv4_read": (_int, [_vp, _vp, _vp, _vp, _vp, _int, _i64, _i64, _i64, _i64, _i64, _vp]),
-    "attn_kv4_decode_workspace_bytes": (_size, [_i64, _i64, _i64, _i64, _i64, _i64, _int]),
+    "attn_kv4_decode_workspace_bytes": (_size, [_i64, _i64, _i64, _i64, _i64, _int]),
     "attn_kv4_decode": (_int, [_vp, _int, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64,
-                               _i64, _i64, _i64, _i64, _f32, _i64, _vp, _size, _vp]),
+                               _i64, _i64, _i64, _i64, _f32, _vp, _size, _vp]),
     "attn_device_status": (_int, [_u32p, _u32p]),
     "attn_selftest_wait_timeout": (_int, [ctypes.c_uint64, _vp]),
     "attn_selftest_exp2": (_int, [_vp, _vp, _vp, _vp, _i64, _vp]),
@@ -302,19 +302,19 @@ class Extension:
                 head_dim, kc.shape[2], kc.shape[0], _stream(kc.device)))
         return k, v
 
-    def kv4_decode(self, q, kc, vc, bt, ctx, max_ctx, weights, scale, partition):
+    def kv4_decode(self, q, kc, vc, bt, ctx, max_ctx, weights, scale):
         out = torch.empty_like(q)
         B, H, Hkv, D, bs, nblk, maxb = self._decode_sizes(q, kc, bt)
         with _on(q.device):
             stream = _stream(q.device)
             ws = _call_workspace(
-                self.lib.attn_kv4_decode_workspace_bytes(B, H, Hkv, D, max_ctx, partition,
+                self.lib.attn_kv4_decode_workspace_bytes(B, H, Hkv, D, max_ctx,
                                                          int(weights is not None)),
                 q.device, stream)
             _check(self.lib.attn_kv4_decode(
                 _ptr(q), _DTYPES[q.dtype], _ptr(kc), _ptr(vc), _ptr(bt), _ptr(ctx), _ptr(out),
-                _ptr(weights), B, H, Hkv, D, bs, nblk, maxb, max_ctx, scale, partition, _ptr(ws),
-                ws.numel(), stream))
+                _ptr(weights), B, H, Hkv, D, bs, nblk, maxb, max_ctx, scale, _ptr(ws), ws.numel(),
+                stream))
         return out
 
     def paged_evict(self, caches, row_bytes, weights, bt, ctx, max_ctx, new_bt, keep, recent,

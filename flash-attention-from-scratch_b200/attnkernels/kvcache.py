@@ -32,7 +32,7 @@ import math
 
 import torch
 
-from . import CHUNK, decode_partition, load_extension, _check_decode, _decode_args
+from . import load_extension, _check_decode, _decode_args
 
 _FLOATS = (torch.float16, torch.bfloat16)
 
@@ -148,7 +148,7 @@ def paged_read_kv4(k_cache, v_cache, slots, dtype=torch.float16):
 
 
 def paged_decode_kv4(q, k_cache, v_cache, block_tables, context_lens, max_context_len,
-                     scale=None, partition_size=None, weights=None):
+                     scale=None, weights=None):
     """Decode attention over a 4-bit paged cache: paged_decode with its arguments, but
 
     q:            [B, H, D] (or [B, H, 1, D]) fp16 or bf16; H / H_kv any whole number from 1 to 8
@@ -157,6 +157,7 @@ def paged_decode_kv4(q, k_cache, v_cache, block_tables, context_lens, max_contex
     context_lens: 0 gives a row of zeros; lengths above max_context_len are cut to it
     weights:      optional fp32 [num_blocks, H_kv, block_size]: each token's softmax weight,
                   summed over the query heads of its kv head, is added to its slot's total
+    There is no partition size: the context is split over the GPU's warps in equal runs.
     Returns q's shape and type.
     """
     if q.dtype not in _FLOATS:
@@ -181,17 +182,12 @@ def paged_decode_kv4(q, k_cache, v_cache, block_tables, context_lens, max_contex
     if q3.shape[0] == 0 or max_context_len == 0:
         return torch.zeros_like(q)
     scale = 1.0 / math.sqrt(q3.shape[-1]) if scale is None else scale
-    if partition_size is None:
-        partition_size = decode_partition(q3.shape[0], k_cache.shape[1], max_context_len,
-                                          q.device.index, num_heads=q3.shape[1],
-                                          head_dim=q3.shape[2])
-    partition_size = -(-int(partition_size) // CHUNK) * CHUNK
     q3 = q3.contiguous()
     if q3.data_ptr() % 16:
         q3 = q3.clone()
     return load_extension().kv4_decode(
         q3, k_cache, v_cache, _index32(block_tables, q.device), _index32(context_lens, q.device),
-        int(max_context_len), weights, float(scale), partition_size).reshape(q.shape)
+        int(max_context_len), weights, float(scale)).reshape(q.shape)
 
 
 def paged_decode_weights(q, k_cache, v_cache, block_tables, context_lens, max_context_len, weights,

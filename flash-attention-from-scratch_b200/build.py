@@ -28,7 +28,7 @@ CSRC = PKG / "csrc"
 BUILD = PKG / "_build"
 LIB = PKG / "attnkernels" / "libattn_b200.so"
 SOURCES = ["api.cu", "prefill_tc.cu", "prefill_simt.cu", "decode.cu", "exchange.cu",
-           "kv4.cu", "kv4_decode.cu", "evict.cu"]
+           "kv4.cu", "kv4_decode.cu", "evict.cu", "finish.cu"]
 HEADERS = ["common.cuh", "kv4.cuh", "launch.h"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 

@@ -597,12 +597,11 @@ int attn_kv4_read(const void* k_cache, const void* v_cache, const int64_t* slots
 
 size_t attn_kv4_decode_workspace_bytes(int64_t batch, int64_t num_heads, int64_t num_kv_heads,
                                        int64_t head_dim, int64_t max_context_len,
-                                       int64_t partition, int with_weights) {
-  if (batch <= 0 || num_heads <= 0 || num_kv_heads <= 0 || head_dim <= 0 || partition <= 0 ||
-      max_context_len < 0)
+                                       int with_weights) {
+  if (batch <= 0 || num_heads <= 0 || num_kv_heads <= 0 || head_dim <= 0 || max_context_len < 0)
     return 0;
   return kv4_decode_workspace_bytes(batch, num_heads, num_kv_heads, head_dim, max_context_len,
-                                    partition, with_weights != 0);
+                                    with_weights != 0);
 }
 
 int attn_kv4_decode(const void* q, int dtype, const void* k_cache, const void* v_cache,
@@ -610,7 +609,7 @@ int attn_kv4_decode(const void* q, int dtype, const void* k_cache, const void* v
                     float* weights, int64_t batch, int64_t num_heads, int64_t num_kv_heads,
                     int64_t head_dim, int64_t block_size, int64_t num_blocks,
                     int64_t max_blocks_per_seq, int64_t max_context_len, float scale,
-                    int64_t partition, void* workspace, size_t workspace_bytes, void* stream) {
+                    void* workspace, size_t workspace_bytes, void* stream) {
   const char* name = "paged_decode_kv4";
   int rc = check_kv4(name, dtype, head_dim, k_cache, v_cache);
   if (rc == ATTN_OK && weights != nullptr) rc = check_weights(name, weights);
@@ -626,11 +625,12 @@ int attn_kv4_decode(const void* q, int dtype, const void* k_cache, const void* v
     return fail(ATTN_ERR_INVALID, "%s: num_heads must be a multiple of num_kv_heads", name);
   if (num_heads / num_kv_heads > 8)
     return fail(ATTN_ERR_UNSUPPORTED, "%s: num_heads / num_kv_heads must be 1 to 8", name);
-  if (partition <= 0 || partition % 256 != 0 || partition > 0x40000000LL)
-    return fail(ATTN_ERR_INVALID, "%s: partition size must be a positive multiple of 256", name);
   if (head_dim == 64 && block_size % 2 != 0)
     return fail(ATTN_ERR_UNSUPPORTED, "%s: head_dim 64 needs an even block_size", name);
-  if (max_context_len > 0x40000000LL || max_blocks_per_seq > 0x7fffffffLL ||
+  // Tokens of a launch (up to 2048 sequences) over 32: counted in 31 bits.
+  if ((batch < 2048 ? batch : 2048) * ((max_context_len + 31) / 32) > 0x7fffffffLL)
+    return fail(ATTN_ERR_UNSUPPORTED, "%s: 2^36 tokens of context or more in 2048 sequences", name);
+  if (num_kv_heads > 0x20000 || max_context_len > 0x40000000LL || max_blocks_per_seq > 0x7fffffffLL ||
       block_size > 0x10000 || num_blocks > 0x7fffffffLL || batch > 0x7fffffffLL ||
       num_heads > 0x7fffffffLL || batch * num_heads > 0x7fffffffLL)
     return fail(ATTN_ERR_UNSUPPORTED,
@@ -642,7 +642,7 @@ int attn_kv4_decode(const void* q, int dtype, const void* k_cache, const void* v
     return fail(ATTN_ERR_INVALID, "%s: empty cache with a non-empty context", name);
   if (batch == 0) return ATTN_OK;
   const size_t need = kv4_decode_workspace_bytes(batch, num_heads, num_kv_heads, head_dim,
-                                                 max_context_len, partition, weights != nullptr);
+                                                 max_context_len, weights != nullptr);
   if (workspace == nullptr || workspace_bytes < need ||
       (reinterpret_cast<uintptr_t>(workspace) & 255u))
     return fail(ATTN_ERR_WORKSPACE, "%s: workspace of %zu bytes (256-byte aligned) needed", name,
@@ -652,7 +652,7 @@ int attn_kv4_decode(const void* q, int dtype, const void* k_cache, const void* v
   if (rc != ATTN_OK) return rc;
   Kv4DecodeArgs a{q, dtype == ATTN_BF16, k_cache, v_cache, block_tables, context_lens, out, weights,
                   batch, num_heads, num_kv_heads, head_dim, block_size, num_blocks,
-                  max_blocks_per_seq, max_context_len, partition, scale, workspace,
+                  max_blocks_per_seq, max_context_len, scale, workspace,
                   workspace_bytes};
   cudaError_t e = launch_kv4_decode(a, ctx);
   if (e != cudaSuccess) return cuda_fail(e, "paged_decode_kv4 launch");

@@ -37,7 +37,7 @@
 #include <algorithm>
 #include <mutex>
 
-#include "kv4.cuh"
+#include "common.cuh"
 #include "launch.h"
 
 namespace fab {
@@ -693,7 +693,6 @@ struct MergeParams {
   long long o_row_stride, o_part_stride, ml_row_stride, ml_part_stride;
   int hq, partition, num_parts;
   int skip_single;  // rows with exactly one part were written by the decode kernel
-  int out_bf16;     // out16 holds bf16 instead
   __half* out16;    // fp16 [rows, D], or else the merged partial state:
   float* out_o;     // fp32 [rows, D]
   float* out_m;     // fp32 [rows]
@@ -829,12 +828,7 @@ __global__ void __launch_bounds__(256) merge_partials_kernel(const MergeParams p
   const float inv = den > 0.f ? 1.f / den : 0.f;
   if (p.out16 != nullptr) {
     __half* dst = p.out16 + row * D + lane * DV;
-    if (p.out_bf16) {
-#pragma unroll
-      for (int j = 0; j < DV; j += 2)
-        reinterpret_cast<uint32_t*>(dst)[j / 2] =
-            pack2<__nv_bfloat16>(num[j] * inv, num[j + 1] * inv);
-    } else if constexpr (DV == 4) {
+    if constexpr (DV == 4) {
       *reinterpret_cast<uint2*>(dst) =
           make_uint2(pack_half2(num[0] * inv, num[1] * inv), pack_half2(num[2] * inv, num[3] * inv));
     } else {
@@ -1071,12 +1065,29 @@ cudaError_t launch_paged_decode(const DecodeArgs& a, bool partials_mode, const L
     }
   }
   if (scored) {
-    cudaError_t e = launch_decode_merge({w.o_part, w.m_part, w.l_part, a.context_lens, a.batch, a.hq,
-                                         a.hkv, a.d, part, num_splits, false, a.out, false}, ctx);
-    if (e != cudaSuccess) return e;
-    return launch_add_weights({scores, w.m_part, w.l_part, a.block_tables, a.context_lens, a.weights,
-                               a.batch, a.hq, a.hkv, a.bs, a.num_blocks, a.max_blocks, a.max_ctx,
-                               part, num_splits}, ctx);
+    FinishArgs f;
+    f.o = w.o_part;
+    f.m = w.m_part;
+    f.l = w.l_part;
+    f.context_lens = a.context_lens;
+    f.first = nullptr;
+    f.workers = 0;
+    f.partition = part;
+    f.parts = num_splits;
+    f.scores = scores;
+    f.weights = a.weights;
+    f.block_tables = a.block_tables;
+    f.out = a.out;
+    f.bf16 = false;
+    f.batch = a.batch;
+    f.hq = a.hq;
+    f.hkv = a.hkv;
+    f.d = a.d;
+    f.bs = a.bs;
+    f.num_blocks = a.num_blocks;
+    f.max_blocks = a.max_blocks;
+    f.max_ctx = a.max_ctx;
+    return launch_finish(f, ctx);
   }
   if (!partials_mode && num_splits <= 1) return cudaSuccess;
   MergeParams mp;
@@ -1093,34 +1104,10 @@ cudaError_t launch_paged_decode(const DecodeArgs& a, bool partials_mode, const L
   mp.partition = static_cast<int>(part);
   mp.num_parts = static_cast<int>(num_splits);
   mp.skip_single = partials_mode ? 0 : 1;
-  mp.out_bf16 = 0;
   mp.out16 = partials_mode ? nullptr : static_cast<__half*>(a.out);
   mp.out_o = a.o_final;
   mp.out_m = a.m_final;
   mp.out_l = a.l_final;
-  return launch_merge_impl(mp, static_cast<int>(a.d), ctx.stream);
-}
-
-cudaError_t launch_decode_merge(const DecodePartsArgs& a, const LaunchCtx& ctx) {
-  MergeParams mp;
-  mp.o = a.o;
-  mp.m = a.m;
-  mp.l = a.l;
-  mp.ctx = a.context_lens;
-  mp.rows = a.batch * a.hq;
-  mp.o_row_stride = a.parts * a.d;
-  mp.o_part_stride = a.d;
-  mp.ml_row_stride = a.parts;
-  mp.ml_part_stride = 1;
-  mp.hq = static_cast<int>(a.hq);
-  mp.partition = static_cast<int>(a.partition);
-  mp.num_parts = static_cast<int>(a.parts);
-  mp.skip_single = a.skip_single ? 1 : 0;
-  mp.out_bf16 = a.bf16 ? 1 : 0;
-  mp.out16 = static_cast<__half*>(a.out);
-  mp.out_o = nullptr;
-  mp.out_m = nullptr;
-  mp.out_l = nullptr;
   return launch_merge_impl(mp, static_cast<int>(a.d), ctx.stream);
 }
 
@@ -1141,7 +1128,6 @@ cudaError_t launch_merge(const float* o_parts, const float* m_parts, const float
   mp.partition = 1;
   mp.num_parts = static_cast<int>(num_parts);
   mp.skip_single = 0;
-  mp.out_bf16 = 0;
   mp.out16 = static_cast<__half*>(out);
   mp.out_o = nullptr;
   mp.out_m = nullptr;

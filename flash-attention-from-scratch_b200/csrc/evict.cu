@@ -1,12 +1,4 @@
-// Accumulated attention weights of cached tokens, and the eviction that goes by
-// them.
-//
-// add_weights: the decode kernels leave every token's score s (log2 units) and
-// the (m, l) parts of every query row. With M = max_s m_s and
-// L = sum_s l_s 2^(m_s - M) of a row, its weight on the token is 2^(s - M) / L;
-// the token's total grows by the sum over the query heads of its kv head.
-//
-// evict: per (sequence, kv head) the tokens to keep (the first `sinks`, the last
+// Eviction of cached tokens by their accumulated attention weights: per (sequence, kv head) the tokens to keep (the first `sinks`, the last
 // `recent`, the largest totals of the rest, ties to the lower index), then their
 // rows moved, in order, into the sequence's new pages.
 #include <algorithm>
@@ -17,57 +9,7 @@
 namespace fab {
 namespace {
 
-enum : unsigned int { kSiteSelectBlock = 231, kSiteMoveBlock = 232, kSiteWeightBlock = 233 };
-
-struct AddWeightsParams {
-  const float* scores;  // [batch, hkv, max_ctx, gp]
-  const float* m;       // [batch * hq, parts]
-  const float* l;
-  const int* bt;
-  const int* ctx;
-  float* weights;       // [num_blocks, hkv, bs]
-  DeviceStatus* status;
-  int hq, hkv, group, gp, bs, num_blocks, max_blocks, max_ctx, partition, parts;
-};
-
-constexpr int kAddTokens = 1024;  // tokens per CTA
-
-__global__ void __launch_bounds__(256) add_weights_kernel(const AddWeightsParams p) {
-  const int kvh = blockIdx.x % p.hkv, b = blockIdx.x / p.hkv;
-  const int ctx = min(max(p.ctx[b], 0), p.max_ctx);
-  if (static_cast<long long>(blockIdx.y) * kAddTokens >= ctx) return;
-  __shared__ float mx[8], inv[8];
-  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-  const int parts = min((ctx + p.partition - 1) / p.partition, p.parts);
-  if (warp < p.group) {
-    const size_t row = (static_cast<size_t>(b) * p.hq + kvh * p.group + warp) * p.parts;
-    float big = -INFINITY;
-    for (int s = lane; s < parts; s += 32) big = fmaxf(big, p.m[row + s]);
-    big = warp_max(big);
-    float sum = 0.f;
-    for (int s = lane; s < parts; s += 32) sum += p.l[row + s] * exp2f(p.m[row + s] - big);
-    sum = warp_sum(sum);
-    if (lane == 0) {
-      mx[warp] = big;
-      inv[warp] = 1.f / sum;
-    }
-  }
-  __syncthreads();
-  for (long long t0 = static_cast<long long>(blockIdx.y) * kAddTokens; t0 < ctx;
-       t0 += static_cast<long long>(gridDim.y) * kAddTokens)
-  for (int t = t0 + threadIdx.x; t < min(static_cast<long long>(ctx), t0 + kAddTokens); t += 256) {
-    const float* s = p.scores + ((static_cast<size_t>(b) * p.hkv + kvh) * p.max_ctx + t) * p.gp;
-    float w = 0.f;
-    for (int g = 0; g < p.group; ++g) w += exp2f(s[g] - mx[g]) * inv[g];
-    const int page = p.bt[static_cast<size_t>(b) * p.max_blocks + t / p.bs];
-    if (page < 0 || page >= p.num_blocks) {
-      report_status(p.status, 2u, kSiteWeightBlock);
-      continue;
-    }
-    // A page can stand in several sequences (a shared prefix): their adds all count.
-    atomicAdd(p.weights + (static_cast<size_t>(page) * p.hkv + kvh) * p.bs + t % p.bs, w);
-  }
-}
+enum : unsigned int { kSiteSelectBlock = 231, kSiteMoveBlock = 232 };
 
 // ------------------------------------------------------------------- select
 
@@ -252,40 +194,6 @@ unsigned grid_y(int64_t n, int64_t per) {
 }
 
 }  // namespace
-
-int64_t score_heads(int64_t group) {
-  int64_t gp = 1;
-  while (gp < group) gp *= 2;
-  return gp;
-}
-
-size_t score_bytes(int64_t batch, int64_t hkv, int64_t group, int64_t max_ctx) {
-  return static_cast<size_t>(batch) * hkv * max_ctx * score_heads(group) * 4;
-}
-
-cudaError_t launch_add_weights(const AddWeightsArgs& a, const LaunchCtx& ctx) {
-  AddWeightsParams p;
-  p.scores = a.scores;
-  p.m = a.m;
-  p.l = a.l;
-  p.bt = a.block_tables;
-  p.ctx = a.context_lens;
-  p.weights = a.weights;
-  p.status = ctx.status;
-  p.hq = static_cast<int>(a.hq);
-  p.hkv = static_cast<int>(a.hkv);
-  p.group = static_cast<int>(a.hq / a.hkv);
-  p.gp = static_cast<int>(score_heads(p.group));
-  p.bs = static_cast<int>(a.bs);
-  p.num_blocks = static_cast<int>(a.num_blocks);
-  p.max_blocks = static_cast<int>(a.max_blocks);
-  p.max_ctx = static_cast<int>(a.max_ctx);
-  p.partition = static_cast<int>(a.partition);
-  p.parts = static_cast<int>(a.parts);
-  const dim3 grid(static_cast<unsigned>(a.batch * a.hkv), grid_y(a.max_ctx, kAddTokens));
-  add_weights_kernel<<<grid, 256, 0, ctx.stream>>>(p);
-  return cudaGetLastError();
-}
 
 cudaError_t launch_evict(const EvictArgs& a, const LaunchCtx& ctx) {
   SelectParams s;

@@ -1,0 +1,308 @@
+// The end of a split decode launch, in one kernel: the fp32 (o, m, l) parts of a
+// row are merged,
+//     M = max_s m_s,  L = sum_s l_s 2^(m_s - M),  o = sum_s l_s 2^(m_s - M) o_s / L,
+// and, where the decode left every token's score s (log2 units), the token's
+// attention weight 2^(s - M) / L, summed over the query heads of its kv head, is
+// added to its slot's total. One kernel, because a short call is bound by its
+// launches: the CTAs that add weights find M and L from the parts themselves
+// instead of waiting for a merge.
+#include <algorithm>
+
+#include "kv4.cuh"
+#include "launch.h"
+
+namespace fab {
+namespace {
+
+enum : unsigned int { kSiteWeightBlock = 241 };
+
+struct FinishParams {
+  const float* o;
+  const float* m;
+  const float* l;
+  const int* ctx;
+  const int* first;
+  const float* scores;
+  float* weights;
+  const int* bt;
+  void* out;
+  DeviceStatus* status;
+  long long workers;
+  int partition, parts;
+  int batch, hq, hkv, group, gp, bs, num_blocks, max_blocks, max_ctx;
+  int merge_blocks;  // CTAs [0, merge_blocks) merge, the others add weights
+  int add_chunks;    // CTAs per (sequence, kv head) that add
+};
+
+// The parts of one (sequence, kv head) pair: part s of query head g is at
+// base + s * stride + g * head. Set before the decode launch has ended: false.
+struct Parts {
+  long long base, stride, head;
+  int count;
+};
+
+__device__ __forceinline__ Parts parts_of(const FinishParams& p, int b, int kvh, int ctx) {
+  Parts r;
+  if (p.first == nullptr) {
+    r.count = min((ctx + p.partition - 1) / p.partition, p.parts);
+    r.base = (static_cast<long long>(b) * p.hq + kvh * p.group) * p.parts;
+    r.stride = 1;
+    r.head = p.parts;
+    return r;
+  }
+  const unsigned long long total = static_cast<unsigned long long>(p.first[p.batch]) * p.hkv;
+  const int n = p.first[b + 1] - p.first[b];
+  if (n == 0) return {0, 0, 0, 0};
+  const unsigned long long s0 =
+      static_cast<unsigned long long>(p.first[b]) * p.hkv + static_cast<unsigned long long>(kvh) * n;
+  // Worker i has the stages [i total / workers, (i + 1) total / workers).
+  const unsigned long long workers = min(static_cast<unsigned long long>(p.workers), total);
+  const long long i0 = static_cast<long long>(((s0 + 1) * workers - 1) / total);
+  const long long i1 = static_cast<long long>(((s0 + n) * workers - 1) / total);
+  r.count = static_cast<int>(i1 - i0 + 1);
+  r.base = (i0 + static_cast<long long>(b) * p.hkv + kvh) * p.group;
+  r.stride = p.group;
+  r.head = 1;
+  return r;
+}
+
+// WPR warps per row (1 or 8) merge: lane owns D / 32 columns; each warp folds
+// chunks of 8 parts into a running (max, sum, numerator), and the warps of a row
+// combine in shared memory.
+template <int D, int WPR, typename T>
+__device__ void merge_row(const FinishParams& p, long long row, bool live, const Parts& r, int g) {
+  constexpr int DV = D / 32;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, sub = warp % WPR;
+  float mw = -INFINITY, den = 0.f, num[DV];
+#pragma unroll
+  for (int j = 0; j < DV; ++j) num[j] = 0.f;
+  if (live) {
+    const long long at = r.base + g * r.head;
+    const int per = (r.count + WPR - 1) / WPR;
+    const int begin = min(r.count, sub * per), end = min(r.count, begin + per);
+    for (int s0 = begin; s0 < end; s0 += 8) {
+      const int cnt = min(8, end - s0);
+      // Lane u holds m and l of part s0 + u % 8.
+      const bool have = (lane & 7) < cnt;
+      const long long su = at + (s0 + (lane & 7)) * r.stride;
+      const float mu = have ? p.m[su] : -INFINITY;
+      const float lu = have ? p.l[su] : 0.f;
+      float v[8][DV];
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {
+        const float* src = p.o + (at + (s0 + u) * r.stride) * D + lane * DV;
+        if (u < cnt) {
+          if constexpr (DV == 4) {
+            const float4 x = *reinterpret_cast<const float4*>(src);
+            v[u][0] = x.x; v[u][1] = x.y; v[u][2] = x.z; v[u][3] = x.w;
+          } else {
+            const float2 x = *reinterpret_cast<const float2*>(src);
+            v[u][0] = x.x; v[u][1] = x.y;
+          }
+        } else {
+#pragma unroll
+          for (int j = 0; j < DV; ++j) v[u][j] = 0.f;
+        }
+      }
+      float mn = mu;
+#pragma unroll
+      for (int o = 1; o < 8; o <<= 1) mn = fmaxf(mn, __shfl_xor_sync(0xffffffffu, mn, o));
+      mn = fmaxf(mw, mn);
+      const float alpha = mw == -INFINITY ? 0.f : fast_exp2(mw - mn);
+      const float wu = have ? lu * fast_exp2(mu - mn) : 0.f;
+      float ws = wu;
+#pragma unroll
+      for (int o = 1; o < 8; o <<= 1) ws += __shfl_xor_sync(0xffffffffu, ws, o);
+      den = den * alpha + ws;
+#pragma unroll
+      for (int j = 0; j < DV; ++j) num[j] *= alpha;
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {
+        const float w = __shfl_sync(0xffffffffu, wu, u);
+#pragma unroll
+        for (int j = 0; j < DV; ++j) num[j] = fmaf(w, v[u][j], num[j]);
+      }
+      mw = mn;
+    }
+  }
+  if constexpr (WPR > 1) {
+    __shared__ float red[8][D + 2];
+#pragma unroll
+    for (int j = 0; j < DV; ++j) red[warp][lane * DV + j] = num[j];
+    if (lane == 0) {
+      red[warp][D] = den;
+      red[warp][D + 1] = mw;
+    }
+    __syncthreads();
+    if (!live || sub != 0) return;
+    float big = mw;
+    for (int w = 1; w < WPR; ++w) big = fmaxf(big, red[w][D + 1]);
+    den = 0.f;
+#pragma unroll
+    for (int j = 0; j < DV; ++j) num[j] = 0.f;
+    for (int w = 0; w < WPR; ++w) {
+      const float mx = red[w][D + 1];
+      if (mx == -INFINITY) continue;  // a warp without parts
+      const float a = fast_exp2(mx - big);
+      den = fmaf(a, red[w][D], den);
+#pragma unroll
+      for (int j = 0; j < DV; ++j) num[j] = fmaf(a, red[w][lane * DV + j], num[j]);
+    }
+  }
+  if (!live) return;
+  // An empty sequence has no part: zeros.
+  const float inv = r.count == 0 ? 0.f : 1.f / den;
+  uint32_t* dst = reinterpret_cast<uint32_t*>(static_cast<T*>(p.out) + row * D + lane * DV);
+#pragma unroll
+  for (int j = 0; j < DV; j += 2) dst[j / 2] = pack2<T>(num[j] * inv, num[j + 1] * inv);
+}
+
+constexpr int kAddTokens = 1024;  // tokens a CTA adds at a time
+
+// Launched as a programmatic dependent of the decode: it waits for that launch's
+// end before it reads what the decode wrote.
+template <int D, int WPR, typename T>
+__global__ void __launch_bounds__(256) finish_kernel(const FinishParams p) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  if (static_cast<int>(blockIdx.x) < p.merge_blocks) {
+    const long long row = static_cast<long long>(blockIdx.x) * (8 / WPR) + warp / WPR;
+    bool live = row < static_cast<long long>(p.batch) * p.hq;
+    Parts r = {0, 0, 0, 0};
+    int g = 0;
+    if (live) {
+      const int b = static_cast<int>(row / p.hq), head = static_cast<int>(row - static_cast<long long>(b) * p.hq);
+      const int kvh = head / p.group;
+      g = head - kvh * p.group;
+      r = parts_of(p, b, kvh, min(max(p.ctx[b], 0), p.max_ctx));
+      if (p.first != nullptr && r.count == 1) live = false;  // written by the decode
+    }
+    merge_row<D, WPR, T>(p, row, live, r, g);
+    return;
+  }
+  const int at = blockIdx.x - p.merge_blocks;
+  const int pair = at / p.add_chunks, chunk = at - pair * p.add_chunks;
+  const int b = pair / p.hkv, kvh = pair - b * p.hkv;
+  const int ctx = min(max(p.ctx[b], 0), p.max_ctx);
+  if (static_cast<long long>(chunk) * kAddTokens >= ctx) return;
+  const Parts r = parts_of(p, b, kvh, ctx);
+  __shared__ float mx[8], inv[8];
+  if (warp < p.group) {
+    const long long base = r.base + warp * r.head;
+    float big = -INFINITY;
+    for (int s = lane; s < r.count; s += 32) big = fmaxf(big, p.m[base + s * r.stride]);
+    big = warp_max(big);
+    float sum = 0.f;
+    for (int s = lane; s < r.count; s += 32)
+      sum += p.l[base + s * r.stride] * exp2f(p.m[base + s * r.stride] - big);
+    sum = warp_sum(sum);
+    if (lane == 0) {
+      mx[warp] = big;
+      inv[warp] = 1.f / sum;
+    }
+  }
+  __syncthreads();
+  const int* bt = p.bt + static_cast<size_t>(b) * p.max_blocks;
+  const float* sc = p.scores + static_cast<size_t>(pair) * p.max_ctx * p.gp;
+  for (long long t0 = static_cast<long long>(chunk) * kAddTokens; t0 < ctx;
+       t0 += static_cast<long long>(p.add_chunks) * kAddTokens) {
+    const int end = static_cast<int>(min(static_cast<long long>(ctx), t0 + kAddTokens));
+    for (int t = static_cast<int>(t0) + threadIdx.x; t < end; t += 256) {
+      const float* s = sc + static_cast<size_t>(t) * p.gp;
+      float w = 0.f;
+      for (int g = 0; g < p.group; ++g) w += exp2f(s[g] - mx[g]) * inv[g];
+      const int page = bt[t / p.bs];
+      if (page < 0 || page >= p.num_blocks) {
+        report_status(p.status, 2u /* ATTN_DEVICE_BAD_BLOCK */, kSiteWeightBlock);
+        continue;
+      }
+      // A page can stand in several sequences (a shared prefix): their adds all count.
+      atomicAdd(p.weights + (static_cast<size_t>(page) * p.hkv + kvh) * p.bs + t % p.bs, w);
+    }
+  }
+}
+
+template <int D, int WPR, typename T>
+cudaError_t launch(const FinishParams& p, unsigned grid, cudaStream_t stream) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(256);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, finish_kernel<D, WPR, T>, p);
+}
+
+template <int D, int WPR>
+cudaError_t by_type(const FinishParams& p, unsigned grid, bool bf16, cudaStream_t stream) {
+  return bf16 ? launch<D, WPR, __nv_bfloat16>(p, grid, stream)
+              : launch<D, WPR, __half>(p, grid, stream);
+}
+
+}  // namespace
+
+int64_t score_heads(int64_t group) {
+  int64_t gp = 1;
+  while (gp < group) gp *= 2;
+  return gp;
+}
+
+size_t score_bytes(int64_t batch, int64_t hkv, int64_t group, int64_t max_ctx) {
+  return static_cast<size_t>(batch) * hkv * max_ctx * score_heads(group) * 4;
+}
+
+cudaError_t launch_finish(const FinishArgs& a, const LaunchCtx& ctx) {
+  FinishParams p;
+  p.o = a.o;
+  p.m = a.m;
+  p.l = a.l;
+  p.ctx = a.context_lens;
+  p.first = a.first;
+  p.scores = a.scores;
+  p.weights = a.weights;
+  p.bt = a.block_tables;
+  p.out = a.out;
+  p.status = ctx.status;
+  p.workers = a.workers;
+  p.partition = static_cast<int>(a.partition);
+  p.parts = static_cast<int>(a.parts);
+  p.batch = static_cast<int>(a.batch);
+  p.hq = static_cast<int>(a.hq);
+  p.hkv = static_cast<int>(a.hkv);
+  p.group = static_cast<int>(a.hq / a.hkv);
+  p.gp = static_cast<int>(score_heads(p.group));
+  p.bs = static_cast<int>(a.bs);
+  p.num_blocks = static_cast<int>(a.num_blocks);
+  p.max_blocks = static_cast<int>(a.max_blocks);
+  p.max_ctx = static_cast<int>(a.max_ctx);
+  const int64_t rows = a.batch * a.hq;
+  // Eight warps per row where a row can have 32 parts or more (four per warp).
+  const int64_t per_row = a.first == nullptr
+                              ? a.parts
+                              : std::min((a.max_ctx + a.partition - 1) / a.partition,
+                                         a.workers / (a.batch * a.hkv) + 1);
+  const bool wide = per_row >= 32;
+  const int64_t merge = wide ? rows : (rows + 7) / 8;
+  // CTAs that add: one per 1024 tokens of a pair, fewer (each then walks on) where
+  // that would be more than a launch's grid holds.
+  const int64_t pairs = a.batch * a.hkv;
+  int64_t chunks = 0;
+  if (a.scores != nullptr) {
+    chunks = std::max<int64_t>(1, (a.max_ctx + kAddTokens - 1) / kAddTokens);
+    chunks = std::min(chunks, std::max<int64_t>(1, (int64_t(1) << 30) / pairs));
+  }
+  if (merge + pairs * chunks > 0x7fffffffLL) return cudaErrorInvalidConfiguration;
+  p.merge_blocks = static_cast<int>(merge);
+  p.add_chunks = static_cast<int>(chunks);
+  const unsigned grid = static_cast<unsigned>(merge + pairs * chunks);
+  if (a.d == 64)
+    return wide ? by_type<64, 8>(p, grid, a.bf16, ctx.stream)
+                : by_type<64, 1>(p, grid, a.bf16, ctx.stream);
+  return wide ? by_type<128, 8>(p, grid, a.bf16, ctx.stream)
+              : by_type<128, 1>(p, grid, a.bf16, ctx.stream);
+}
+
+}  // namespace fab

@@ -1,15 +1,20 @@
 // Decode attention of one query token per sequence over the 4-bit paged cache
-// (row layout: kv4.cuh), split over the context and merged like the fp16 decode
-// (decode.cu): scores in log2 units, a running maximum and sum, one fp32
-// (o, m, l) part per split.
+// (row layout: kv4.cuh): scores in log2 units, a running maximum and sum, and
+// fp32 (o, m, l) parts that the finish kernel (finish.cu) merges.
 //
 // A token costs 160 bytes of K and V per kv head at head_dim 128 where fp16 takes
 // 512, so at the memory's rate an SM has about 7 cycles for a token: the kernel is
 // laid out to spend few instructions on it.
 //
-//   * Warps are independent pipelines over work units (sequence, kv head, split),
-//     as in decode.cu: bulk copies of whole page runs into a per-warp ring of
-//     32-token stages, signalled by mbarriers.
+//   * Warps are independent pipelines: bulk copies of whole page runs into a
+//     per-warp ring of 32-token stages, signalled by mbarriers.
+//   * The stages of all (sequence, kv head) rows, in that order, are dealt out to
+//     the resident warps in equal runs: warp i of n (at most S of them) takes stages
+//     [i S / n, (i + 1) S / n) of S. Every warp has the same work whatever the
+//     lengths are, without a work counter. A row that lies in one warp's run is
+//     written at once; of the others each warp leaves a part, in slot i + row,
+//     which no two (warp, row) pairs share, since along the runs one of the two
+//     grows at each step: n + rows slots are enough for any lengths.
 //   * Both products run on the tensor cores (mma.sync m16n8k16) with the cached
 //     rows as the 16-row operand A and the query heads of the kv head as the 8
 //     columns of B, so up to 8 heads cost what one does:
@@ -41,6 +46,10 @@ enum : unsigned int { kSiteKv4Wait = 221, kSiteKv4Drain = 222, kSiteKv4Block = 2
 
 constexpr int kTok = 32;            // tokens per pipeline stage
 constexpr int kLaunchBatch = 2048;  // sequences per launch (their lengths live in shared memory)
+
+// Flags of a stage beside its tokens (at most 32): the first and the last of its
+// row for this warp, and, with the last, the row lies wholly in this warp's run.
+enum : int { kTokens = 63, kFirst = 64, kLast = 128, kWhole = 256 };
 
 #ifndef FAB_KV4_W
 #define FAB_KV4_W 16
@@ -75,43 +84,52 @@ struct Kv4DecParams {
   const uint8_t* vc;
   const int* bt;
   const int* ctx;
-  void* out;              // q's type [batch, hq, D]: rows of sequences with one split (direct_out)
-  float* o_part;          // [batch * hq, num_splits, D]
-  float* m_part;          // [batch * hq, num_splits]
+  void* out;              // q's type [batch, hq, D]: rows that one warp has whole
+  float* o_part;          // [slots, group, D]
+  float* m_part;          // [slots, group]
   float* l_part;
+  int* first;             // [batch + 1]: stages of one head before each sequence
   float* scores;          // SCORED: [batch, hkv, max_ctx, gp] log2-unit scores
-  unsigned int* counter;  // work counter, zero at launch
   DeviceStatus* status;
   unsigned long long timeout_ns;
   long long block_stride;  // bytes between physical blocks
-  int batch, hq, hkv, group, gp, bs, max_blocks, num_blocks, partition, num_splits, max_ctx;
-  int direct_out;
+  int batch, hq, hkv, group, gp, bs, max_blocks, num_blocks, max_ctx;
+  // n / bs = umulhi(n, bs_mul) >> bs_shift for n < 2^31; bs_mul is 0 for bs = 1.
+  uint32_t bs_mul, bs_shift;
   float scale_log2;
 };
 
 // D (16x8, fp32) += A (16x16, fp16, rows) B (16x8, fp16, columns).
 __device__ __forceinline__ void mma_k16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2,
                                         uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm volatile(
+  asm(
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
       "{%8, %9}, {%0, %1, %2, %3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// The same with A 16x8.
-__device__ __forceinline__ void mma_k8(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t b0) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k8.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5}, {%6}, "
-      "{%0, %1, %2, %3};"
-      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-      : "r"(a0), "r"(a1), "r"(b0));
+// D = A B.
+__device__ __forceinline__ void mma_k16_new(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2,
+                                            uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
+      "{%8, %9}, {%10, %10, %10, %10};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+}
+
+// D = A B with A 16x8.
+__device__ __forceinline__ void mma_k8_new(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t b0) {
+  asm("mma.sync.aligned.m16n8k8.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5}, {%6}, "
+      "{%7, %7, %7, %7};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a0), "r"(a1), "r"(b0), "f"(0.f));
 }
 
 // Transpose of an 8x8 fp16 matrix whose row i lanes 4 i .. 4 i + 3 hold in pairs.
 __device__ __forceinline__ uint32_t transpose8(uint32_t a) {
   uint32_t d;
-  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
   return d;
 }
 
@@ -155,8 +173,8 @@ __global__ void __launch_bounds__(Kv4Cfg<D>::THREADS, 1) kv4_decode_kernel(const
   // before it reads the parts.
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
-  // Lengths and the prefix sums of the splits per sequence: active (sequence,
-  // split) pairs are numbered densely, v in [0, prefix[batch]).
+  // Lengths and the stages of one head before each sequence, which the finish
+  // kernel goes by too.
   for (int b = threadIdx.x; b < p.batch; b += C::THREADS)
     ctx_s[b] = min(max(p.ctx[b], 0), p.max_ctx);
   if (threadIdx.x < C::W * C::STAGES)
@@ -171,7 +189,7 @@ __global__ void __launch_bounds__(Kv4Cfg<D>::THREADS, 1) kv4_decode_kernel(const
     const int b0 = lane * per;
     int sum = 0;
     for (int i = 0; i < per; ++i)
-      if (b0 + i < p.batch) sum += (ctx_s[b0 + i] + p.partition - 1) / p.partition;
+      if (b0 + i < p.batch) sum += (ctx_s[b0 + i] + kTok - 1) / kTok;
     int incl = sum;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -182,79 +200,89 @@ __global__ void __launch_bounds__(Kv4Cfg<D>::THREADS, 1) kv4_decode_kernel(const
     for (int i = 0; i < per; ++i) {
       if (b0 + i < p.batch) {
         prefix[b0 + i] = run;
-        run += (ctx_s[b0 + i] + p.partition - 1) / p.partition;
+        run += (ctx_s[b0 + i] + kTok - 1) / kTok;
       }
     }
     if (lane == 31) prefix[p.batch] = incl;
   }
   __syncthreads();
-  // Without a merge pass, rows of empty sequences are written here (zeros).
-  if (p.direct_out && p.num_splits == 1 && blockIdx.x == 0) {
-    for (int b = warp; b < p.batch; b += C::W) {
-      if (ctx_s[b] != 0) continue;
-      uint32_t* dst = static_cast<uint32_t*>(p.out) + static_cast<size_t>(b) * p.hq * (D / 2);
-      for (int i = lane; i < p.hq * (D / 2); i += 32) dst[i] = 0u;
-    }
+  if (blockIdx.x == 0) {
+    for (int b = threadIdx.x; b <= p.batch; b += C::THREADS) p.first[b] = prefix[b];
   }
-  const int total_units = prefix[p.batch] * p.hkv;
+
+  // This warp's run of stages. Warps next to each other in number are on different
+  // SMs, so that a small call spreads over all of them.
+  const unsigned int worker = warp * gridDim.x + blockIdx.x;
+  const unsigned long long total = static_cast<unsigned long long>(prefix[p.batch]) * p.hkv;
+  // No more workers than stages: a worker between two others always has a part.
+  const unsigned long long workers =
+      min(static_cast<unsigned long long>(C::W * gridDim.x), total);
+  unsigned long long run0 = 0;
+  long long left = 0;
+  if (worker < workers) {
+    run0 = total * worker / workers;
+    left = static_cast<long long>(total * (worker + 1) / workers - run0);
+  }
 
   // ---------------------------------------------------------- producer state
-  int pu = -1, pb = 0, pkvh = 0, psplit = 0, pstart = 0, pend = 0, pst = 0, pnst = 0;
+  int pb = 0, pkvh = 0, pst = 0, pnst = 0;  // the next stage: sequence, kv head, stage of that row
+  bool pfirst = true, pwhole = true;        // it is this warp's first of the row; from the row's first
   // Block-table entries [bt_base, bt_base + 32) and the next 32, one per lane:
   // the second window is on its way while the first is used.
   int bt_base = 0, bt_cur = 0, bt_next = 0;
-  unsigned int nxt = 0;  // next unit id (valid in lane 0), fetched one unit ahead
   unsigned int p_item = 0, c_item = 0;
 
+  auto page_of = [&](int t) {
+    return p.bs_mul == 0
+               ? t
+               : static_cast<int>(__umulhi(static_cast<uint32_t>(t), p.bs_mul) >> p.bs_shift);
+  };
   auto table = [&](int pg) {
     return pg < p.max_blocks ? p.bt[static_cast<size_t>(pb) * p.max_blocks + pg] : 0;
   };
-
-  auto advance = [&]() {
-    const int u = static_cast<int>(__shfl_sync(0xffffffffu, nxt, 0));
-    if (u >= total_units) {
-      pu = -1;
-      return;
-    }
-    pu = u;
-    const int v = u / p.hkv;
-    pkvh = u - v * p.hkv;
-    int lo = 0, hi = p.batch - 1;  // last sequence whose first pair is <= v
-    while (lo < hi) {
-      const int mid = (lo + hi + 1) >> 1;
-      if (prefix[mid] <= v) lo = mid; else hi = mid - 1;
-    }
-    pb = lo;
-    psplit = v - prefix[lo];
-    pstart = psplit * p.partition;
-    pend = min(ctx_s[pb], pstart + p.partition);
-    pst = 0;
-    pnst = (pend - pstart + kTok - 1) / kTok;
-    bt_base = pstart / p.bs;
+  auto open_row = [&]() {
+    pfirst = true;
+    pwhole = pst == 0;
+    bt_base = page_of(pst * kTok);
     bt_cur = table(bt_base + lane);
     bt_next = table(bt_base + 32 + lane);
-    if (lane == 0) nxt = C::W * gridDim.x + atomicAdd(p.counter, 1u);
   };
+
+  if (left > 0) {
+    int lo = 0, hi = p.batch - 1;  // last sequence whose first stage is <= run0
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if (static_cast<unsigned long long>(prefix[mid]) * p.hkv <= run0) lo = mid; else hi = mid - 1;
+    }
+    pb = lo;
+    pnst = prefix[lo + 1] - prefix[lo];
+    const unsigned long long in_seq = run0 - static_cast<unsigned long long>(prefix[lo]) * p.hkv;
+    pkvh = static_cast<int>(in_seq / pnst);
+    pst = static_cast<int>(in_seq - static_cast<unsigned long long>(pkvh) * pnst);
+    open_row();
+  }
 
   // Issue the copies of the producer's next stage into its ring slot: a stage
   // spans at most 32 pages, each lane copies one page's K and V rows.
   auto produce = [&]() {
-    if (pu < 0) return;
+    if (left == 0) return;
     const unsigned int slot = p_item % C::STAGES;
     uint8_t* st = ring + slot * C::STAGE;
     uint64_t* bar = full + slot;
-    const int t0 = pstart + pst * kTok;
-    int t1 = min(t0 + kTok, pend);
+    const int t0 = pst * kTok;
+    int t1 = min(t0 + kTok, ctx_s[pb]);
     const int nt = t1 - t0;
     // Copies are of whole 16 bytes: where a row is not (40 bytes), an odd last token
     // brings the row after it along, which is in its page (the block size is even).
     if constexpr (ROW % 16 != 0) t1 += t1 & 1;
+    const bool row_end = pst + 1 == pnst;
     if (lane == 0) {
       mbar_arrive_expect_tx(bar, 2 * (t1 - t0) * ROW);
-      meta[slot] = make_int4(pb, pkvh, psplit,
-                             nt | ((pst == 0) ? 64 : 0) | ((pst == pnst - 1) ? 128 : 0));
+      meta[slot] = make_int4(pb, pkvh, t0,
+                             nt | (pfirst ? kFirst : 0) | (row_end || left == 1 ? kLast : 0) |
+                                 (row_end && pwhole ? kWhole : 0));
     }
-    const int pg0 = t0 / p.bs, pages = (t1 - 1) / p.bs - pg0 + 1;
+    const int pg0 = page_of(t0), pages = page_of(t1 - 1) - pg0 + 1;
     if (pg0 - bt_base >= 32) {
       bt_base += 32;
       bt_cur = bt_next;
@@ -280,7 +308,18 @@ __global__ void __launch_bounds__(Kv4Cfg<D>::THREADS, 1) kv4_decode_kernel(const
       bulk_g2s(dst + C::KV, p.vc + src, bytes, bar);
     }
     ++p_item;
-    if (++pst == pnst) advance();
+    --left;
+    pfirst = false;
+    ++pst;
+    if (row_end && left > 0) {
+      pst = 0;
+      if (++pkvh == p.hkv) {
+        pkvh = 0;
+        do ++pb; while (prefix[pb + 1] == prefix[pb]);  // left > 0: one with stages follows
+        pnst = prefix[pb + 1] - prefix[pb];
+      }
+      open_row();
+    }
     __syncwarp();
   };
 
@@ -360,8 +399,8 @@ __global__ void __launch_bounds__(Kv4Cfg<D>::THREADS, 1) kv4_decode_kernel(const
     const int4 md = meta[slot];
     const uint8_t* kst = ring + slot * C::STAGE;
     uint8_t* vst = ring + slot * C::STAGE + C::KV;
-    const int nt = md.w & 63;
-    if (md.w & 64) {
+    const int nt = md.w & kTokens;
+    if (md.w & kFirst) {
       load_q(md.x, md.y);
       m[0] = m[1] = -INFINITY;
       l[0] = l[1] = 0.f;
@@ -372,11 +411,8 @@ __global__ void __launch_bounds__(Kv4Cfg<D>::THREADS, 1) kv4_decode_kernel(const
 #pragma unroll
       for (int i = 0; i < 4; ++i) z[i] = 0.f;
     }
-    if constexpr (SCORED) {
-      sc = (md.w & 64) ? p.scores + ((static_cast<size_t>(md.x) * p.hkv + md.y) * p.max_ctx +
-                                     static_cast<size_t>(md.z) * p.partition) * p.gp
-                       : sc + kTok * p.gp;
-    }
+    if constexpr (SCORED)
+      sc = p.scores + ((static_cast<size_t>(md.x) * p.hkv + md.y) * p.max_ctx + md.z) * p.gp;
     const bool ok = mbar_wait(full + slot, parity, abort_flag, p.status, kSiteKv4Wait,
                               p.timeout_ns);
     if (!__all_sync(0xffffffffu, ok)) return false;
@@ -395,15 +431,15 @@ __global__ void __launch_bounds__(Kv4Cfg<D>::THREADS, 1) kv4_decode_kernel(const
       load_words<NG / 2>(sa, ra + CODES);
       load_words<NG / 2>(sb, rb + CODES);
       const int low = CODES + 2 * NG + (NG == 4 ? 4 * (t4 & 1) : 0);
-      float lows[4] = {0.f, 0.f, 0.f, 0.f};
-      mma_k8(lows, *reinterpret_cast<const uint32_t*>(ra + low),
+      float lows[4];
+      mma_k8_new(lows, *reinterpret_cast<const uint32_t*>(ra + low),
              *reinterpret_cast<const uint32_t*>(rb + low), qs);
       float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int w = 0; w < NG; ++w) {
-        float d[4] = {0.f, 0.f, 0.f, 0.f};
+        float d[4];
         const uint32_t ya = xa[w] >> 8, yb = xb[w] >> 8;
-        mma_k16(d, xa[w] & 0x000F000Fu, xb[w] & 0x000F000Fu, ya & 0x000F000Fu, yb & 0x000F000Fu,
+        mma_k16_new(d, xa[w] & 0x000F000Fu, xb[w] & 0x000F000Fu, ya & 0x000F000Fu, yb & 0x000F000Fu,
                 qf[w][0], qf[w][1]);
         mma_k16(d, xa[w] & 0x00F000F0u, xb[w] & 0x00F000F0u, ya & 0x00F000F0u, yb & 0x00F000F0u,
                 qf[w][2], qf[w][3]);
@@ -530,16 +566,16 @@ __global__ void __launch_bounds__(Kv4Cfg<D>::THREADS, 1) kv4_decode_kernel(const
                 b0, b1);
       }
     }
-    if (md.w & 128) {
-      const int ns = (ctx_s[md.x] + p.partition - 1) / p.partition;
+    if (md.w & kLast) {
+      const int pair = md.x * p.hkv + md.y;
+      const size_t slot0 = (static_cast<size_t>(worker) + pair) * p.group;
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
 #pragma unroll
         for (int o = 4; o < 32; o <<= 1) l[h] += __shfl_xor_sync(0xffffffffu, l[h], o);
         const float inv = 1.f / l[h];
         const int head = 2 * t4 + h;
-        const size_t row = static_cast<size_t>(md.x) * p.hq + md.y * p.group + head;
-        const size_t pr = row * p.num_splits + md.z;
+        const size_t row = static_cast<size_t>(pair) * p.group + head, pr = slot0 + head;
 #pragma unroll
         for (int w = 0; w < NG; ++w) {
           const float low = __shfl_sync(0xffffffffu, z[h], 4 * w + t4);
@@ -550,7 +586,7 @@ __global__ void __launch_bounds__(Kv4Cfg<D>::THREADS, 1) kv4_decode_kernel(const
           o[3] = fmaf(acc[w][1][h + 2], 0x1p20f, low) * inv;
           if (head < p.group) {
             const int col = 32 * w + 4 * g4;
-            if (p.direct_out && ns == 1)
+            if (md.w & kWhole)
               *reinterpret_cast<uint2*>(static_cast<T*>(p.out) + row * D + col) =
                   make_uint2(pack2<T>(o[0], o[1]), pack2<T>(o[2], o[3]));
             else
@@ -558,7 +594,7 @@ __global__ void __launch_bounds__(Kv4Cfg<D>::THREADS, 1) kv4_decode_kernel(const
                   make_float4(o[0], o[1], o[2], o[3]);
           }
         }
-        if (head < p.group && g4 == 0 && !(p.direct_out && ns == 1)) {
+        if (head < p.group && g4 == 0 && (SCORED || !(md.w & kWhole))) {
           // A part whose scores are all NaN has no maximum, yet is not an empty one.
           p.m_part[pr] = l[h] != l[h] ? fmaxf(m[h], 0.f) : m[h];
           p.l_part[pr] = 0.25f * l[h];
@@ -570,10 +606,6 @@ __global__ void __launch_bounds__(Kv4Cfg<D>::THREADS, 1) kv4_decode_kernel(const
     return true;
   };
 
-  // First unit: warp w of CTA c takes unit w * grid + c, so a launch with fewer
-  // units than warps spreads them over all SMs; later units come from the counter.
-  nxt = warp * gridDim.x + blockIdx.x;
-  advance();
   for (int i = 0; i < C::STAGES; ++i) produce();
   while (c_item < p_item) {
     if (!consume()) break;
@@ -592,47 +624,37 @@ __global__ void __launch_bounds__(Kv4Cfg<D>::THREADS, 1) kv4_decode_kernel(const
 
 size_t align256(size_t x) { return (x + 255) & ~static_cast<size_t>(255); }
 
+// Workspace of one launch (launches of one call follow each other in the stream
+// and use the same): parts of every resident warp and every (sequence, kv head).
 struct Workspace {
-  unsigned int* counters;
+  int* first;
   float *o, *m, *l, *scores;
   size_t bytes;
 };
 
-int64_t launches_of(int64_t batch) { return (batch + kLaunchBatch - 1) / kLaunchBatch; }
+// Resident warps the workspace has room for: of 160 SMs, more than a B200 has, so
+// that its size goes by the call's sizes alone.
+constexpr int64_t kMaxWorkers = 160 * std::max(Kv4Cfg<64>::W, Kv4Cfg<128>::W);
 
-Workspace carve(void* base, int64_t batch, int64_t hq, int64_t d, int64_t splits,
-                size_t score_bytes) {
+Workspace carve(void* base, int64_t batch, int64_t hq, int64_t hkv, int64_t d, size_t score_bytes) {
   uint8_t* b = static_cast<uint8_t*>(base);
-  const size_t rows = static_cast<size_t>(batch) * hq;
-  const size_t cb = align256(static_cast<size_t>(launches_of(batch)) * 4);
-  const size_t ob = align256(rows * splits * d * 4);
-  const size_t ml = align256(rows * splits * 4);
+  const int64_t nb = std::min<int64_t>(batch, kLaunchBatch);
+  const size_t rows = static_cast<size_t>(kMaxWorkers + nb * hkv) * (hq / hkv);
+  const size_t fb = align256(static_cast<size_t>(nb + 1) * 4);
+  const size_t ob = align256(rows * d * 4);
+  const size_t ml = align256(rows * 4);
   Workspace w;
-  w.counters = reinterpret_cast<unsigned int*>(b);
-  w.o = reinterpret_cast<float*>(b + cb);
-  w.m = reinterpret_cast<float*>(b + cb + ob);
-  w.l = reinterpret_cast<float*>(b + cb + ob + ml);
-  w.scores = reinterpret_cast<float*>(b + cb + ob + 2 * ml);
-  w.bytes = cb + ob + 2 * ml + align256(score_bytes);
+  w.first = reinterpret_cast<int*>(b);
+  w.o = reinterpret_cast<float*>(b + fb);
+  w.m = reinterpret_cast<float*>(b + fb + ob);
+  w.l = reinterpret_cast<float*>(b + fb + ob + ml);
+  w.scores = reinterpret_cast<float*>(b + fb + ob + 2 * ml);
+  w.bytes = fb + ob + 2 * ml + align256(score_bytes);
   return w;
 }
 
-int64_t splits_of(int64_t max_ctx, int64_t partition) {
-  return (max_ctx + partition - 1) / partition;
-}
-
-// Sub-splits, as in decode.cu: a call with few units cuts each partition into 2 or
-// 4 (at least 64 tokens) that are merged like splits. The cap goes by sizes alone
-// (the workspace is made for it); the launch takes what its warps can use.
-int64_t sub_split_cap(int64_t batch, int64_t hq, int64_t max_ctx, int64_t partition) {
-  const int64_t rows = batch * hq * splits_of(max_ctx, partition);
-  for (int64_t k = 4; k > 1; k /= 2)
-    if (partition / k >= 64 && rows * k <= 8192) return k;
-  return 1;
-}
-
 template <int D, typename T, bool SCORED>
-cudaError_t launch_kernel(const Kv4DecParams& p, int64_t upper_units, const LaunchCtx& ctx) {
+cudaError_t launch_kernel(const Kv4DecParams& p, int grid, const LaunchCtx& ctx) {
   using C = Kv4Cfg<D>;
   auto kern = kv4_decode_kernel<D, T, SCORED>;
   // Per device: a function's attributes belong to the device that is current.
@@ -650,46 +672,40 @@ cudaError_t launch_kernel(const Kv4DecParams& p, int64_t upper_units, const Laun
       done[dev] = true;
     }
   }
-  // One CTA per SM, or one per unit when there are fewer units than SMs.
-  const int grid =
-      static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(ctx.sm_count, upper_units)));
   kern<<<grid, C::THREADS, C::SMEM, ctx.stream>>>(p);
   return cudaGetLastError();
 }
 
 template <int D, typename T>
-cudaError_t dispatch(const Kv4DecParams& p, int64_t units, const LaunchCtx& ctx) {
-  return p.scores != nullptr ? launch_kernel<D, T, true>(p, units, ctx)
-                             : launch_kernel<D, T, false>(p, units, ctx);
+cudaError_t dispatch(const Kv4DecParams& p, int grid, const LaunchCtx& ctx) {
+  return p.scores != nullptr ? launch_kernel<D, T, true>(p, grid, ctx)
+                             : launch_kernel<D, T, false>(p, grid, ctx);
 }
 
 }  // namespace
 
 size_t kv4_decode_workspace_bytes(int64_t batch, int64_t hq, int64_t hkv, int64_t d, int64_t max_ctx,
-                                  int64_t partition, bool weights) {
-  const int64_t cap = sub_split_cap(batch, hq, max_ctx, partition);
-  return carve(nullptr, batch, hq, d, splits_of(max_ctx, partition / cap),
-               weights ? score_bytes(batch, hkv, hq / hkv, max_ctx) : 0).bytes;
+                                  bool weights) {
+  const int64_t nb = std::min<int64_t>(batch, kLaunchBatch);
+  return carve(nullptr, batch, hq, hkv, d,
+               weights ? score_bytes(nb, hkv, hq / hkv, max_ctx) : 0).bytes;
 }
 
 cudaError_t launch_kv4_decode(const Kv4DecodeArgs& a, const LaunchCtx& ctx) {
-  const int64_t warps =
-      static_cast<int64_t>(a.d == 64 ? Kv4Cfg<64>::W : Kv4Cfg<128>::W) * ctx.sm_count;
-  int64_t k = sub_split_cap(a.batch, a.hq, a.max_ctx, a.partition);
-  while (k > 1 && a.batch * a.hkv * splits_of(a.max_ctx, a.partition) * k > warps) k /= 2;
-  const int64_t part = a.partition / k;
-  const int64_t splits = splits_of(a.max_ctx, part);
   const int64_t group = a.hq / a.hkv;
   const bool scored = a.weights != nullptr;
-  if (splits == 0)
+  if (a.max_ctx == 0)
     return cudaMemsetAsync(a.out, 0, static_cast<size_t>(a.batch) * a.hq * a.d * 2, ctx.stream);
-  Workspace w = carve(a.workspace, a.batch, a.hq, a.d, splits,
-                      scored ? score_bytes(a.batch, a.hkv, group, a.max_ctx) : 0);
-  const int64_t launches = launches_of(a.batch);
-  cudaError_t e = cudaMemsetAsync(w.counters, 0, static_cast<size_t>(launches) * 4, ctx.stream);
-  if (e != cudaSuccess) return e;
-  for (int64_t i = 0; i < launches; ++i) {
-    const int64_t b0 = i * kLaunchBatch, nb = std::min<int64_t>(kLaunchBatch, a.batch - b0);
+  Workspace w = carve(a.workspace, a.batch, a.hq, a.hkv, a.d, 0);
+  // n / bs by a product: with 2^s >= bs > 2^(s - 1), s >= 1, m = ceil(2^(31 + s) / bs)
+  // is below 2^32, and m bs - 2^(31 + s) < 2^s makes n m >> (31 + s) exact for n < 2^31.
+  int shift = 1;
+  while ((int64_t(1) << shift) < a.bs) ++shift;
+  const uint64_t mul =
+      a.bs == 1 ? 0 : ((uint64_t(1) << (31 + shift)) + a.bs - 1) / static_cast<uint64_t>(a.bs);
+  const int64_t warps = a.d == 64 ? Kv4Cfg<64>::W : Kv4Cfg<128>::W;
+  for (int64_t b0 = 0; b0 < a.batch; b0 += kLaunchBatch) {
+    const int64_t nb = std::min<int64_t>(kLaunchBatch, a.batch - b0);
     const int64_t row_bytes = a.d / 2 + a.d / 8, row0 = b0 * a.hq;
     Kv4DecParams p;
     p.q = static_cast<const uint8_t*>(a.q) + row0 * a.d * 2;
@@ -698,12 +714,12 @@ cudaError_t launch_kv4_decode(const Kv4DecodeArgs& a, const LaunchCtx& ctx) {
     p.bt = a.block_tables + b0 * a.max_blocks;
     p.ctx = a.context_lens + b0;
     p.out = static_cast<uint8_t*>(a.out) + row0 * a.d * 2;
-    p.o_part = w.o + row0 * splits * a.d;
-    p.m_part = w.m + row0 * splits;
-    p.l_part = w.l + row0 * splits;
+    p.o_part = w.o;
+    p.m_part = w.m;
+    p.l_part = w.l;
+    p.first = w.first;
     p.gp = static_cast<int>(score_heads(group));
-    p.scores = scored ? w.scores + static_cast<size_t>(b0) * a.hkv * a.max_ctx * p.gp : nullptr;
-    p.counter = w.counters + i;
+    p.scores = scored ? w.scores : nullptr;
     p.status = ctx.status;
     p.timeout_ns = ctx.timeout_ns;
     p.block_stride = a.hkv * a.bs * row_bytes;
@@ -714,28 +730,46 @@ cudaError_t launch_kv4_decode(const Kv4DecodeArgs& a, const LaunchCtx& ctx) {
     p.bs = static_cast<int>(a.bs);
     p.max_blocks = static_cast<int>(a.max_blocks);
     p.num_blocks = static_cast<int>(a.num_blocks);
-    p.partition = static_cast<int>(part);
-    p.num_splits = static_cast<int>(splits);
     p.max_ctx = static_cast<int>(a.max_ctx);
-    p.direct_out = scored ? 0 : 1;
+    p.bs_mul = static_cast<uint32_t>(mul);
+    p.bs_shift = static_cast<uint32_t>(shift) - 1;
     p.scale_log2 = a.scale * kLog2e;
-    const int64_t units = nb * a.hkv * splits;
+    // One CTA per SM, or one per stage when there cannot be that many.
+    const int64_t stages = nb * a.hkv * ((a.max_ctx + kTok - 1) / kTok);
+    const int grid = static_cast<int>(
+        std::min<int64_t>(std::min<int64_t>(ctx.sm_count, kMaxWorkers / warps), stages));
+    cudaError_t e;
     if (a.d == 64)
-      e = a.bf16 ? dispatch<64, __nv_bfloat16>(p, units, ctx) : dispatch<64, __half>(p, units, ctx);
+      e = a.bf16 ? dispatch<64, __nv_bfloat16>(p, grid, ctx) : dispatch<64, __half>(p, grid, ctx);
     else
-      e = a.bf16 ? dispatch<128, __nv_bfloat16>(p, units, ctx)
-                 : dispatch<128, __half>(p, units, ctx);
+      e = a.bf16 ? dispatch<128, __nv_bfloat16>(p, grid, ctx) : dispatch<128, __half>(p, grid, ctx);
+    if (e != cudaSuccess) return e;
+    FinishArgs f;
+    f.o = w.o;
+    f.m = w.m;
+    f.l = w.l;
+    f.context_lens = p.ctx;
+    f.first = w.first;
+    f.workers = static_cast<int64_t>(grid) * warps;
+    f.partition = kTok;
+    f.parts = 0;
+    f.scores = p.scores;
+    f.weights = a.weights;
+    f.block_tables = p.bt;
+    f.out = p.out;
+    f.bf16 = a.bf16;
+    f.batch = nb;
+    f.hq = a.hq;
+    f.hkv = a.hkv;
+    f.d = a.d;
+    f.bs = a.bs;
+    f.num_blocks = a.num_blocks;
+    f.max_blocks = a.max_blocks;
+    f.max_ctx = a.max_ctx;
+    e = launch_finish(f, ctx);
     if (e != cudaSuccess) return e;
   }
-  if (splits > 1 || scored) {
-    e = launch_decode_merge({w.o, w.m, w.l, a.context_lens, a.batch, a.hq, a.hkv, a.d, part, splits,
-                             !scored, a.out, a.bf16}, ctx);
-    if (e != cudaSuccess) return e;
-  }
-  if (!scored) return cudaSuccess;
-  return launch_add_weights({w.scores, w.m, w.l, a.block_tables, a.context_lens, a.weights, a.batch,
-                             a.hq, a.hkv, a.bs, a.num_blocks, a.max_blocks, a.max_ctx, part, splits},
-                            ctx);
+  return cudaSuccess;
 }
 
 }  // namespace fab

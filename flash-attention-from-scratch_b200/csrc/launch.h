@@ -65,37 +65,33 @@ cudaError_t launch_merge(const float* o_parts, const float* m_parts, const float
                          int64_t num_parts, int64_t rows, int64_t d, int64_t o_part_stride,
                          int64_t ml_part_stride, void* out, const LaunchCtx& ctx);
 
-// The fp32 parts [batch * hq, parts] of a decode launch, merged into 16-bit rows;
-// sequence b has min(ceil(context_lens[b] / partition), parts) of them.
-struct DecodePartsArgs {
-  const float* o;
-  const float* m;
-  const float* l;
-  const int32_t* context_lens;
-  int64_t batch, hq, hkv, d, partition, parts;
-  bool skip_single;  // rows with exactly one part are already written
-  void* out;         // fp16 (or bf16) [batch, hq, d]
-  bool bf16;
-};
-cudaError_t launch_decode_merge(const DecodePartsArgs& a, const LaunchCtx& ctx);
-
 // Query heads a token's scores are stored for (the group, rounded up to a power
 // of two), and the bytes of fp32 scores [batch, hkv, max_ctx, score_heads].
 int64_t score_heads(int64_t group);
 size_t score_bytes(int64_t batch, int64_t hkv, int64_t group, int64_t max_ctx);
 
-// weights[page, h, off] += sum over the query heads of kv head h of
-// 2^(score - M) / L, with a row's M and L from its parts (csrc/evict.cu).
-struct AddWeightsArgs {
-  const float* scores;
+// The end of a decode launch in one kernel (csrc/finish.cu): fp32 parts merged
+// into 16-bit rows, and, with scores, the attention weights added to the totals.
+struct FinishArgs {
+  const float* o;             // parts
   const float* m;
   const float* l;
-  const int32_t* block_tables;
   const int32_t* context_lens;
-  float* weights;
-  int64_t batch, hq, hkv, bs, num_blocks, max_blocks, max_ctx, partition, parts;
+  // Where the parts are. first == null: of (sequence, query head) row r the parts
+  // r * parts + s, s < ceil(length / partition). Else: equal runs of `workers` (or one
+  // per stage, if that is fewer) over the stages of `partition` tokens, the part of
+  // worker i and (sequence, kv head) pair j in slot i + j ([slots, group]); a pair in
+  // one run has its rows written.
+  const int32_t* first;       // [batch + 1] stages of one head before each sequence
+  int64_t workers, partition, parts;
+  const float* scores;        // [batch, hkv, max_ctx, score_heads] or null
+  float* weights;             // [num_blocks, hkv, bs]
+  const int32_t* block_tables;
+  void* out;                  // fp16 (or bf16) [batch, hq, d]
+  bool bf16;
+  int64_t batch, hq, hkv, d, bs, num_blocks, max_blocks, max_ctx;
 };
-cudaError_t launch_add_weights(const AddWeightsArgs& a, const LaunchCtx& ctx);
+cudaError_t launch_finish(const FinishArgs& a, const LaunchCtx& ctx);
 
 // ------------------------------------------------------------ 4-bit paged cache
 
@@ -122,13 +118,13 @@ struct Kv4DecodeArgs {
   const int32_t* context_lens;
   void* out;            // q's type [batch, hq, d]
   float* weights;       // fp32 [num_blocks, hkv, bs] or null
-  int64_t batch, hq, hkv, d, bs, num_blocks, max_blocks, max_ctx, partition;
+  int64_t batch, hq, hkv, d, bs, num_blocks, max_blocks, max_ctx;
   float scale;
   void* workspace;
   size_t workspace_bytes;
 };
 size_t kv4_decode_workspace_bytes(int64_t batch, int64_t hq, int64_t hkv, int64_t d, int64_t max_ctx,
-                                  int64_t partition, bool weights);
+                                  bool weights);
 cudaError_t launch_kv4_decode(const Kv4DecodeArgs& a, const LaunchCtx& ctx);
 
 // --------------------------------------------------------------------- eviction

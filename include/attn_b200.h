@@ -326,7 +326,7 @@ int attn_kv4_read(const void* k_cache, const void* v_cache, const int64_t* slots
 /* Bytes of workspace attn_kv4_decode needs (with_weights: `weights` is given). */
 size_t attn_kv4_decode_workspace_bytes(int64_t batch, int64_t num_heads, int64_t num_kv_heads,
                                        int64_t head_dim, int64_t max_context_len,
-                                       int64_t partition, int with_weights);
+                                       int with_weights);
 
 /*
  * Decode attention over a 4-bit cache: as attn_paged_decode, with q and out of
@@ -334,13 +334,16 @@ size_t attn_kv4_decode_workspace_bytes(int64_t batch, int64_t num_heads, int64_t
  * `weights` is not null, the totals of attn_paged_decode_weights. head_dim 64
  * needs an even block_size (a page of one head is then a multiple of 16 bytes).
  * Lengths above max_context_len are cut to it; an empty sequence gets zeros.
+ * The context is split over the GPU's resident warps in equal runs, whatever the
+ * lengths, so there is no partition to choose; the outputs of one sequence differ
+ * by rounding with the sequences beside it.
  */
 int attn_kv4_decode(const void* q, int dtype, const void* k_cache, const void* v_cache,
                     const int32_t* block_tables, const int32_t* context_lens, void* out,
                     float* weights, int64_t batch, int64_t num_heads, int64_t num_kv_heads,
                     int64_t head_dim, int64_t block_size, int64_t num_blocks,
                     int64_t max_blocks_per_seq, int64_t max_context_len, float scale,
-                    int64_t partition, void* workspace, size_t workspace_bytes, void* stream);
+                    void* workspace, size_t workspace_bytes, void* stream);
 
 /* ------------------------------------------------------------ device status */
 

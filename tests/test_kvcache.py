@@ -54,7 +54,7 @@ def cache4(lens, hkv, d, bs, seed=0, spread=1.0):
     return caches[0], caches[1], bt
 
 
-def check_decode4(lens, hq, hkv, d, bs, dtype=torch.float16, partition=None, seed=0, spread=1.0,
+def check_decode4(lens, hq, hkv, d, bs, dtype=torch.float16, seed=0, spread=1.0,
                   weights=True, max_ctx=None, scale=None):
     kc, vc, bt = cache4(lens, hkv, d, bs, seed, spread)
     g = hq // hkv
@@ -64,7 +64,7 @@ def check_decode4(lens, hq, hkv, d, bs, dtype=torch.float16, partition=None, see
     lens_t = torch.tensor(lens, dtype=torch.int32)
     out = ak.paged_decode_kv4(q.cuda(), kc.cuda(), vc.cuda(), bt.cuda(), lens_t.cuda(),
                               max(lens) if max_ctx is None else max_ctx, scale=scale,
-                              partition_size=partition, weights=w)
+                              weights=w)
     assert out.shape == q.shape and out.dtype == dtype
     out = out.cpu().double()
     sc = scale if scale is not None else d ** -0.5
@@ -242,26 +242,28 @@ EDGES = [1, 15, 16, 17, 31, 32, 33, 0, 63, 64, 65, 255, 256, 257]
 @pytest.mark.parametrize("d", [64, 128])
 @pytest.mark.parametrize("group", [1, 2, 3, 4, 5, 7, 8])
 def test_decode4_lengths(d, group):
-    check_decode4(EDGES, 2 * group, 2, d, 16, partition=256, seed=group)
+    check_decode4(EDGES, 2 * group, 2, d, 16, seed=group)
 
 
 @pytest.mark.parametrize("d", [64, 128])
 @pytest.mark.parametrize("bs", [2, 6, 8, 24, 32, 64, 128])
 def test_decode4_block_sizes(d, bs):
-    check_decode4([300, 1, 50, 17], 8, 2, d, bs, partition=256, seed=bs)
+    check_decode4([300, 1, 50, 17], 8, 2, d, bs, seed=bs)
 
 
 @pytest.mark.parametrize("bs", [1, 3, 5])
 def test_decode4_odd_block_sizes(bs):
-    check_decode4([300, 1, 50, 17], 8, 2, 128, bs, partition=256, seed=bs)
+    check_decode4([300, 1, 50, 17], 8, 2, 128, bs, seed=bs)
 
 
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
-@pytest.mark.parametrize("partition", [None, 256, 512, 1 << 20])
+@pytest.mark.parametrize("lens", [[1100, 257, 700, 64], [3] * 40 + [900] + [0] * 20 + [33] * 9,
+                                  [31] * 700])
 @pytest.mark.parametrize("weights", [False, True])
-def test_decode4_partitions(dtype, partition, weights):
-    check_decode4([1100, 257, 700, 64], 16, 4, 128, 16, dtype=dtype, partition=partition,
-                  weights=weights)
+def test_decode4_runs(dtype, lens, weights):
+    """Rows cut into one-stage runs, long rows among short and empty ones, and runs of several
+    rows (2800 stages over the GPU's warps)."""
+    check_decode4(lens, 16, 4, 128, 16, dtype=dtype, weights=weights)
 
 
 @pytest.mark.parametrize("d", [64, 128])
@@ -607,7 +609,7 @@ def test_on_another_stream_and_in_graphs():
     w16 = [torch.zeros(kc.shape[:3], device="cuda") for _ in range(3)]
 
     def calls(i):
-        return (ak.paged_decode_kv4(qs[i], kc, vc, bt, lt, 700, partition_size=256, weights=w4[i]),
+        return (ak.paged_decode_kv4(qs[i], kc, vc, bt, lt, 700, weights=w4[i]),
                 ak.paged_decode_weights(qs[i], f16[0], f16[1], bt, lt, 700, w16[i],
                                         partition_size=256))
 

@@ -107,17 +107,16 @@ def test_evict_refusals():
 
 def decode4(lib, **kw):
     a = dict(q=P, dtype=0, batch=2, hq=8, hkv=8, d=128, bs=16, nblk=10, maxb=5, max_ctx=80,
-             partition=256, ws=P, ws_bytes=1 << 30, weights=None)
+             ws=P, ws_bytes=1 << 30, weights=None)
     a.update(kw)
     return lib.attn_kv4_decode(a["q"], a["dtype"], P, P, P, P, P, a["weights"], a["batch"], a["hq"],
                                a["hkv"], a["d"], a["bs"], a["nblk"], a["maxb"], a["max_ctx"], 0.1,
-                               a["partition"], a["ws"], a["ws_bytes"], None)
+                               a["ws"], a["ws_bytes"], None)
 
 
 def test_abi_decode_refusals(lib):
     assert decode4(lib, hq=6, hkv=4) == 1 and "multiple of num_kv_heads" in err(lib)
     assert decode4(lib, hq=72, hkv=8) == 2 and "1 to 8" in err(lib)
-    assert decode4(lib, partition=100) == 1 and "multiple of 256" in err(lib)
     assert decode4(lib, d=96) == 2 and "head_dim" in err(lib)
     assert decode4(lib, dtype=2) == 2 and "dtype" in err(lib)
     assert decode4(lib, d=64, bs=15) == 2 and "even block_size" in err(lib)
