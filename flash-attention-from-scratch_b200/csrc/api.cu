@@ -635,6 +635,8 @@ int attn_kv4_decode(const void* q, int dtype, const void* k_cache, const void* v
       num_heads > 0x7fffffffLL || batch * num_heads > 0x7fffffffLL)
     return fail(ATTN_ERR_UNSUPPORTED,
                 "%s: sizes must fit in 31 bits (max_context_len <= 2^30, block_size <= 65536)", name);
+  if (num_kv_heads * block_size * attn_kv4_row_bytes(head_dim) > 0x7fffffffLL)
+    return fail(ATTN_ERR_UNSUPPORTED, "%s: a page of all kv heads must be below 2 GiB", name);
   if (max_context_len > max_blocks_per_seq * block_size)
     return fail(ATTN_ERR_INVALID, "%s: max_context_len needs more than max_blocks_per_seq blocks",
                 name);

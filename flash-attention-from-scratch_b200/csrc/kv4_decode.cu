@@ -92,10 +92,8 @@ struct Kv4DecParams {
   float* scores;          // SCORED: [batch, hkv, max_ctx, gp] log2-unit scores
   DeviceStatus* status;
   unsigned long long timeout_ns;
-  long long block_stride;  // bytes between physical blocks
+  unsigned int block_stride;  // bytes between physical blocks
   int batch, hq, hkv, group, gp, bs, max_blocks, num_blocks, max_ctx;
-  // n / bs = umulhi(n, bs_mul) >> bs_shift for n < 2^31; bs_mul is 0 for bs = 1.
-  uint32_t bs_mul, bs_shift;
   float scale_log2;
 };
 
@@ -160,7 +158,9 @@ __global__ void __launch_bounds__(Kv4Cfg<D>::THREADS, 1) kv4_decode_kernel(const
   using C = Kv4Cfg<D>;
   constexpr int NG = C::NG, ROW = C::ROW, CODES = C::R::CODES;
   extern __shared__ __align__(128) uint8_t smem[];
-  const int warp = threadIdx.x >> 5;
+  // By a shuffle, which tells the compiler that it is the same in all lanes: the
+  // producer's state then stays in uniform registers, which bulk copies are issued from.
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);
   const int lane = threadIdx.x & 31;
   const int g4 = lane >> 2, t4 = lane & 3;
   uint8_t* ring = smem + warp * C::RING;
@@ -226,26 +226,28 @@ __global__ void __launch_bounds__(Kv4Cfg<D>::THREADS, 1) kv4_decode_kernel(const
 
   // ---------------------------------------------------------- producer state
   int pb = 0, pkvh = 0, pst = 0, pnst = 0;  // the next stage: sequence, kv head, stage of that row
+  int ppg = 0, poff = 0;                    // page of the row and token in it where it begins
   bool pfirst = true, pwhole = true;        // it is this warp's first of the row; from the row's first
   // Block-table entries [bt_base, bt_base + 32) and the next 32, one per lane:
   // the second window is on its way while the first is used.
   int bt_base = 0, bt_cur = 0, bt_next = 0;
-  unsigned int p_item = 0, c_item = 0;
+  const uint8_t *pk = nullptr, *pv = nullptr;  // the row's kv head in page 0
+  unsigned int p_slot = 0, c_slot = 0, c_parity = 0, ahead = 0;
+  const bool leader = elect_one();
 
-  auto page_of = [&](int t) {
-    return p.bs_mul == 0
-               ? t
-               : static_cast<int>(__umulhi(static_cast<uint32_t>(t), p.bs_mul) >> p.bs_shift);
-  };
   auto table = [&](int pg) {
     return pg < p.max_blocks ? p.bt[static_cast<size_t>(pb) * p.max_blocks + pg] : 0;
   };
   auto open_row = [&]() {
     pfirst = true;
     pwhole = pst == 0;
-    bt_base = page_of(pst * kTok);
+    ppg = pst * kTok / p.bs;
+    poff = pst * kTok - ppg * p.bs;
+    bt_base = ppg;
     bt_cur = table(bt_base + lane);
     bt_next = table(bt_base + 32 + lane);
+    pk = p.kc + static_cast<long long>(pkvh) * p.bs * ROW;
+    pv = p.vc + static_cast<long long>(pkvh) * p.bs * ROW;
   };
 
   if (left > 0) {
@@ -262,52 +264,56 @@ __global__ void __launch_bounds__(Kv4Cfg<D>::THREADS, 1) kv4_decode_kernel(const
     open_row();
   }
 
-  // Issue the copies of the producer's next stage into its ring slot: a stage
-  // spans at most 32 pages, each lane copies one page's K and V rows.
+  // Issue the copies of the producer's next stage into its ring slot, page by page
+  // from one elected lane, with operands that are the same in all lanes. (With a
+  // page per lane the compiler puts a loop over the lanes around each copy.)
   auto produce = [&]() {
     if (left == 0) return;
-    const unsigned int slot = p_item % C::STAGES;
-    uint8_t* st = ring + slot * C::STAGE;
-    uint64_t* bar = full + slot;
+    uint8_t* dst = ring + p_slot * C::STAGE;
+    uint64_t* bar = full + p_slot;
     const int t0 = pst * kTok;
-    int t1 = min(t0 + kTok, ctx_s[pb]);
-    const int nt = t1 - t0;
+    const int nt = min(kTok, ctx_s[pb] - t0);
     // Copies are of whole 16 bytes: where a row is not (40 bytes), an odd last token
     // brings the row after it along, which is in its page (the block size is even).
-    if constexpr (ROW % 16 != 0) t1 += t1 & 1;
+    int todo = ROW % 16 != 0 ? nt + (nt & 1) : nt;
     const bool row_end = pst + 1 == pnst;
-    if (lane == 0) {
-      mbar_arrive_expect_tx(bar, 2 * (t1 - t0) * ROW);
-      meta[slot] = make_int4(pb, pkvh, t0,
-                             nt | (pfirst ? kFirst : 0) | (row_end || left == 1 ? kLast : 0) |
-                                 (row_end && pwhole ? kWhole : 0));
+    if (leader) {
+      mbar_arrive_expect_tx(bar, 2 * todo * ROW);
+      meta[p_slot] = make_int4(pb, pkvh, t0,
+                               nt | (pfirst ? kFirst : 0) | (row_end || left == 1 ? kLast : 0) |
+                                   (row_end && pwhole ? kWhole : 0));
     }
-    const int pg0 = page_of(t0), pages = page_of(t1 - 1) - pg0 + 1;
-    if (pg0 - bt_base >= 32) {
+    if (ppg - bt_base >= 32) {
       bt_base += 32;
       bt_cur = bt_next;
       bt_next = table(bt_base + 32 + lane);
     }
-    const int rel = pg0 + lane - bt_base;  // below 64
-    const int cur = __shfl_sync(0xffffffffu, bt_cur, rel & 31);
-    const int next = __shfl_sync(0xffffffffu, bt_next, rel & 31);
-    __syncwarp();  // the expected bytes are set before any copy completes
-    if (lane < pages) {
-      int page = rel < 32 ? cur : next;
-      if (page < 0 || page >= p.num_blocks) {  // never read outside the cache
-        report_status(p.status, 2u /* ATTN_DEVICE_BAD_BLOCK */, kSiteKv4Block);
+    do {
+      const int rel = ppg - bt_base;  // below 64
+      int page = __shfl_sync(0xffffffffu, rel < 32 ? bt_cur : bt_next, rel & 31);
+      if (static_cast<unsigned int>(page) >= static_cast<unsigned int>(p.num_blocks)) {
+        // Never read outside the cache.
+        if (leader) report_status(p.status, 2u /* ATTN_DEVICE_BAD_BLOCK */, kSiteKv4Block);
         page = 0;
       }
-      const int first = (pg0 + lane) * p.bs;
-      const int from = max(first, t0), to = min(first + p.bs, t1);
-      const long long src = page * p.block_stride +
-                            (static_cast<long long>(pkvh) * p.bs + (from - first)) * ROW;
-      const uint32_t bytes = static_cast<uint32_t>(to - from) * ROW;
-      uint8_t* dst = st + (from - t0) * ROW;
-      bulk_g2s(dst, p.kc + src, bytes, bar);
-      bulk_g2s(dst + C::KV, p.vc + src, bytes, bar);
-    }
-    ++p_item;
+      const int rows = min(p.bs - poff, todo);
+      const unsigned long long src =
+          static_cast<unsigned long long>(static_cast<unsigned int>(page)) * p.block_stride +
+          static_cast<unsigned int>(poff * ROW);
+      if (leader) {
+        bulk_g2s(dst, pk + src, rows * ROW, bar);
+        bulk_g2s(dst + C::KV, pv + src, rows * ROW, bar);
+      }
+      dst += rows * ROW;
+      todo -= rows;
+      poff += rows;
+      if (poff == p.bs) {
+        poff = 0;
+        ++ppg;
+      }
+    } while (todo > 0);
+    p_slot = p_slot + 1 == C::STAGES ? 0 : p_slot + 1;
+    ++ahead;
     --left;
     pfirst = false;
     ++pst;
@@ -332,7 +338,7 @@ __global__ void __launch_bounds__(Kv4Cfg<D>::THREADS, 1) kv4_decode_kernel(const
   // which makes the loads of 80-byte rows free of bank conflicts, K (8 lanes: two
   // rows 4 or 12 apart) as well as V (16 lanes: four even or four odd rows).
   uint32_t qf[NG][4];  // b0, b1 of the codes in bits 0-3, then of those in bits 4-7
-  uint32_t qs = 0;     // B of the lows' product: the groups' sums of q
+  uint32_t qs[2];      // B of the lows' product: the groups' sums of q
   float f[2];          // scale * log2(e) over q's power of two, per head
   float m[2], l[2];    // running maximum; this lane's share of the sum, times 4
   float acc[NG][2][4], z[4];
@@ -377,28 +383,27 @@ __global__ void __launch_bounds__(Kv4Cfg<D>::THREADS, 1) kv4_decode_kernel(const
       sums[w] += __shfl_xor_sync(0xffffffffu, sums[w], 1);
       sums[w] += __shfl_xor_sync(0xffffffffu, sums[w], 2);
     }
-    // k slots of the lows' product: the groups' sums rounded to fp16, then what
-    // that left over; slots past 2 NG are 0.
-    float s0 = sums[0], s1 = sums[1];
-    if (NG == 4 && (t4 & 1)) {
-      s0 = sums[NG - 2];
-      s1 = sums[NG - 1];
+    // The lows' product: its A has the lows of groups 0, 1 in every pair of k slots
+    // below 8 and those of groups 2, 3 in every pair above; its B has the groups'
+    // sums of q, rounded to fp16, in the first pair (lane t4 = 0), what that left over
+    // in the second, and zeros in the others.
+#pragma unroll
+    for (int i = 0; i < NG / 2; ++i) {
+      const float h0 = __half2float(__float2half_rn(sums[2 * i]));
+      const float h1 = __half2float(__float2half_rn(sums[2 * i + 1]));
+      qs[i] = t4 == 0   ? pack_half2(h0, h1)
+              : t4 == 1 ? pack_half2(sums[2 * i] - h0, sums[2 * i + 1] - h1)
+                        : 0u;
     }
-    const float h0 = __half2float(__float2half_rn(s0)), h1 = __half2float(__float2half_rn(s1));
-    const bool rest = t4 >= NG / 2;
-    qs = rest ? pack_half2(s0 - h0, s1 - h1) : pack_half2(h0, h1);
-    if (NG == 2 && t4 >= 2) qs = 0u;
     const float fh = p.scale_log2 * pow2i(-k);
     f[0] = __shfl_sync(0xffffffffu, fh, 8 * t4);
     f[1] = __shfl_sync(0xffffffffu, fh, 8 * t4 + 4);
   };
 
   auto consume = [&]() -> bool {
-    const unsigned int slot = c_item % C::STAGES;
-    const uint32_t parity = (c_item / C::STAGES) & 1u;
-    const int4 md = meta[slot];
-    const uint8_t* kst = ring + slot * C::STAGE;
-    uint8_t* vst = ring + slot * C::STAGE + C::KV;
+    const int4 md = meta[c_slot];
+    const uint8_t* kst = ring + c_slot * C::STAGE;
+    uint8_t* vst = ring + c_slot * C::STAGE + C::KV;
     const int nt = md.w & kTokens;
     if (md.w & kFirst) {
       load_q(md.x, md.y);
@@ -413,7 +418,7 @@ __global__ void __launch_bounds__(Kv4Cfg<D>::THREADS, 1) kv4_decode_kernel(const
     }
     if constexpr (SCORED)
       sc = p.scores + ((static_cast<size_t>(md.x) * p.hkv + md.y) * p.max_ctx + md.z) * p.gp;
-    const bool ok = mbar_wait(full + slot, parity, abort_flag, p.status, kSiteKv4Wait,
+    const bool ok = mbar_wait(full + c_slot, c_parity, abort_flag, p.status, kSiteKv4Wait,
                               p.timeout_ns);
     if (!__all_sync(0xffffffffu, ok)) return false;
 
@@ -427,13 +432,14 @@ __global__ void __launch_bounds__(Kv4Cfg<D>::THREADS, 1) kv4_decode_kernel(const
       uint32_t xa[NG], xb[NG];
       load_words<NG>(xa, ra + 4 * NG * t4);
       load_words<NG>(xb, rb + 4 * NG * t4);
-      uint32_t sa[NG / 2], sb[NG / 2];  // scales
-      load_words<NG / 2>(sa, ra + CODES);
-      load_words<NG / 2>(sb, rb + CODES);
-      const int low = CODES + 2 * NG + (NG == 4 ? 4 * (t4 & 1) : 0);
+      uint32_t sa[NG], sb[NG];  // scales, then lows
+      load_words<NG>(sa, ra + CODES);
+      load_words<NG>(sb, rb + CODES);
       float lows[4];
-      mma_k8_new(lows, *reinterpret_cast<const uint32_t*>(ra + low),
-             *reinterpret_cast<const uint32_t*>(rb + low), qs);
+      if constexpr (NG == 4)
+        mma_k16_new(lows, sa[2], sb[2], sa[3], sb[3], qs[0], qs[1]);
+      else
+        mma_k8_new(lows, sa[1], sb[1], qs[0]);
       float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int w = 0; w < NG; ++w) {
@@ -452,8 +458,11 @@ __global__ void __launch_bounds__(Kv4Cfg<D>::THREADS, 1) kv4_decode_kernel(const
         sum[2] = fmaf(fb, d[2], sum[2]);
         sum[3] = fmaf(fb, d[3], sum[3]);
       }
+      const uint64_t f2 = f2_pack(f[0], f[1]), up = f2_pack(0x1p24f, 0x1p24f);
 #pragma unroll
-      for (int c = 0; c < 4; ++c) s[i][c] = fmaf(sum[c], 0x1p24f, lows[c]) * f[c & 1];
+      for (int c = 0; c < 4; c += 2)
+        f2_unpack(f2_mul(f2_fma(f2_pack(sum[c], sum[c + 1]), up, f2_pack(lows[c], lows[c + 1])), f2),
+                  s[i][c], s[i][c + 1]);
     }
     if (nt < kTok) {
       // Past the last token: no score; the ring's old bytes there must not reach
@@ -490,7 +499,7 @@ __global__ void __launch_bounds__(Kv4Cfg<D>::THREADS, 1) kv4_decode_kernel(const
     // Online softmax: per head the maximum over the 8 lanes of its 32 scores. P is
     // held times 4, which keeps small P * scale in fp16's normal range longer and
     // cannot overflow (a scale is at most 8734).
-    float alpha[2], shift[2];
+    float alpha[2], shift[2];  // shift: 2 - m
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       float mx = fmaxf(fmaxf(s[0][h], s[0][h + 2]), fmaxf(s[1][h], s[1][h + 2]));
@@ -500,23 +509,27 @@ __global__ void __launch_bounds__(Kv4Cfg<D>::THREADS, 1) kv4_decode_kernel(const
       mx = fmaxf(mx, m[h]);
       alpha[h] = fast_exp2(m[h] - mx);
       m[h] = mx;
-      shift[h] = mx - 2.f;
+      shift[h] = 2.f - mx;
     }
     uint32_t pf[2][2];  // P^T as B fragments: tokens of rows 2 t4, 2 t4 + 1 (+ 8), head g4
-    float add[2] = {0.f, 0.f};
+    uint64_t add = f2_pack(0.f, 0.f);
+    const uint64_t sh = f2_pack(shift[0], shift[1]);
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      float e[4];
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        e[c] = fast_exp2(s[i][c] - shift[c & 1]);
-        add[c & 1] += e[c];
+      for (int c = 0; c < 2; ++c) {
+        float e0, e1;
+        f2_unpack(f2_add(f2_pack(s[i][2 * c], s[i][2 * c + 1]), sh), e0, e1);
+        e0 = fast_exp2(e0);
+        e1 = fast_exp2(e1);
+        add = f2_add(add, f2_pack(e0, e1));
+        pf[i][c] = transpose8(pack_half2(e0, e1));
       }
-      pf[i][0] = transpose8(pack_half2(e[0], e[1]));
-      pf[i][1] = transpose8(pack_half2(e[2], e[3]));
     }
-    l[0] = fmaf(l[0], alpha[0], add[0]);
-    l[1] = fmaf(l[1], alpha[1], add[1]);
+    float add0, add1;
+    f2_unpack(add, add0, add1);
+    l[0] = fmaf(l[0], alpha[0], add0);
+    l[1] = fmaf(l[1], alpha[1], add1);
     if (__any_sync(0xffffffffu, alpha[0] != 1.f || alpha[1] != 1.f)) {
 #pragma unroll
       for (int w = 0; w < NG; ++w)
@@ -525,8 +538,8 @@ __global__ void __launch_bounds__(Kv4Cfg<D>::THREADS, 1) kv4_decode_kernel(const
           acc[w][0][i] *= alpha[i & 1];
           acc[w][1][i] *= alpha[i & 1];
         }
-      z[0] *= alpha[0];
-      z[1] *= alpha[1];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) z[i] *= alpha[i & 1];
     }
     // O^T += V^T P^T.
 #pragma unroll
@@ -538,19 +551,17 @@ __global__ void __launch_bounds__(Kv4Cfg<D>::THREADS, 1) kv4_decode_kernel(const
       load_words<NG / 2>(vb, rb + 2 * NG * g4);
       load_words<NG / 2>(vc, ra + ROW + 2 * NG * g4);
       load_words<NG / 2>(vd, rb + ROW + 2 * NG * g4);
-      uint32_t sa[NG / 2], sb[NG / 2], sc2[NG / 2], sd[NG / 2];
-      load_words<NG / 2>(sa, ra + CODES);
-      load_words<NG / 2>(sb, rb + CODES);
-      load_words<NG / 2>(sc2, ra + ROW + CODES);
-      load_words<NG / 2>(sd, rb + ROW + CODES);
-      // Lows of group g4 % NG (rows g4 >= NG repeat them and are not used).
-      const int low = CODES + 2 * NG + (NG == 4 ? 2 * (g4 & 2) : 0);
+      uint32_t sa[NG], sb[NG], sc2[NG], sd[NG];  // scales, then lows
+      load_words<NG>(sa, ra + CODES);
+      load_words<NG>(sb, rb + CODES);
+      load_words<NG>(sc2, ra + ROW + CODES);
+      load_words<NG>(sd, rb + ROW + CODES);
+      // P . low: row g4 has the lows of group g4 % 2, row g4 + 8 those of group
+      // 2 + g4 % 2.
       const uint32_t pick = (g4 & 1) ? 0x7632u : 0x5410u;
-      mma_k16(z,
-              __byte_perm(*reinterpret_cast<const uint32_t*>(ra + low),
-                          *reinterpret_cast<const uint32_t*>(rb + low), pick), 0u,
-              __byte_perm(*reinterpret_cast<const uint32_t*>(ra + ROW + low),
-                          *reinterpret_cast<const uint32_t*>(rb + ROW + low), pick), 0u,
+      constexpr int L = NG / 2;
+      mma_k16(z, __byte_perm(sa[L], sb[L], pick), __byte_perm(sa[NG - 1], sb[NG - 1], pick),
+              __byte_perm(sc2[L], sd[L], pick), __byte_perm(sc2[NG - 1], sd[NG - 1], pick),
               pf[i][0], pf[i][1]);
 #pragma unroll
       for (int w = 0; w < NG; ++w) {
@@ -578,7 +589,7 @@ __global__ void __launch_bounds__(Kv4Cfg<D>::THREADS, 1) kv4_decode_kernel(const
         const size_t row = static_cast<size_t>(pair) * p.group + head, pr = slot0 + head;
 #pragma unroll
         for (int w = 0; w < NG; ++w) {
-          const float low = __shfl_sync(0xffffffffu, z[h], 4 * w + t4);
+          const float low = __shfl_sync(0xffffffffu, z[h + 2 * (w / 2)], 4 * (w % 2) + t4);
           float o[4];
           o[0] = fmaf(acc[w][0][h], 0x1p24f, low) * inv;
           o[1] = fmaf(acc[w][1][h], 0x1p20f, low) * inv;
@@ -602,23 +613,28 @@ __global__ void __launch_bounds__(Kv4Cfg<D>::THREADS, 1) kv4_decode_kernel(const
       }
     }
     __syncwarp();
-    ++c_item;
+    --ahead;
+    if (++c_slot == C::STAGES) {
+      c_slot = 0;
+      c_parity ^= 1u;
+    }
     return true;
   };
 
   for (int i = 0; i < C::STAGES; ++i) produce();
-  while (c_item < p_item) {
+  while (ahead > 0) {
     if (!consume()) break;
     // The slot just read is refilled by the async proxy.
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     produce();
   }
   // Never exit with a copy in flight (only reached with copies pending after a timeout).
-  while (c_item < p_item) {
-    const unsigned int slot = c_item % C::STAGES;
-    mbar_wait(full + slot, (c_item / C::STAGES) & 1u, nullptr, p.status, kSiteKv4Drain,
-              p.timeout_ns);
-    ++c_item;
+  for (; ahead > 0; --ahead) {
+    mbar_wait(full + c_slot, c_parity, nullptr, p.status, kSiteKv4Drain, p.timeout_ns);
+    if (++c_slot == C::STAGES) {
+      c_slot = 0;
+      c_parity ^= 1u;
+    }
   }
 }
 
@@ -697,12 +713,6 @@ cudaError_t launch_kv4_decode(const Kv4DecodeArgs& a, const LaunchCtx& ctx) {
   if (a.max_ctx == 0)
     return cudaMemsetAsync(a.out, 0, static_cast<size_t>(a.batch) * a.hq * a.d * 2, ctx.stream);
   Workspace w = carve(a.workspace, a.batch, a.hq, a.hkv, a.d, 0);
-  // n / bs by a product: with 2^s >= bs > 2^(s - 1), s >= 1, m = ceil(2^(31 + s) / bs)
-  // is below 2^32, and m bs - 2^(31 + s) < 2^s makes n m >> (31 + s) exact for n < 2^31.
-  int shift = 1;
-  while ((int64_t(1) << shift) < a.bs) ++shift;
-  const uint64_t mul =
-      a.bs == 1 ? 0 : ((uint64_t(1) << (31 + shift)) + a.bs - 1) / static_cast<uint64_t>(a.bs);
   const int64_t warps = a.d == 64 ? Kv4Cfg<64>::W : Kv4Cfg<128>::W;
   for (int64_t b0 = 0; b0 < a.batch; b0 += kLaunchBatch) {
     const int64_t nb = std::min<int64_t>(kLaunchBatch, a.batch - b0);
@@ -722,7 +732,7 @@ cudaError_t launch_kv4_decode(const Kv4DecodeArgs& a, const LaunchCtx& ctx) {
     p.scores = scored ? w.scores : nullptr;
     p.status = ctx.status;
     p.timeout_ns = ctx.timeout_ns;
-    p.block_stride = a.hkv * a.bs * row_bytes;
+    p.block_stride = static_cast<unsigned int>(a.hkv * a.bs * row_bytes);
     p.batch = static_cast<int>(nb);
     p.hq = static_cast<int>(a.hq);
     p.hkv = static_cast<int>(a.hkv);
@@ -731,8 +741,6 @@ cudaError_t launch_kv4_decode(const Kv4DecodeArgs& a, const LaunchCtx& ctx) {
     p.max_blocks = static_cast<int>(a.max_blocks);
     p.num_blocks = static_cast<int>(a.num_blocks);
     p.max_ctx = static_cast<int>(a.max_ctx);
-    p.bs_mul = static_cast<uint32_t>(mul);
-    p.bs_shift = static_cast<uint32_t>(shift) - 1;
     p.scale_log2 = a.scale * kLog2e;
     // One CTA per SM, or one per stage when there cannot be that many.
     const int64_t stages = nb * a.hkv * ((a.max_ctx + kTok - 1) / kTok);
