@@ -20,6 +20,25 @@
 
 namespace fab {
 
+// n / d for n < 2^31 by a product: with 2^s >= d > 2^(s - 1), s >= 1, the factor
+// m = ceil(2^(31 + s) / d) is below 2^32, and m d - 2^(31 + s) < 2^s makes
+// n m >> (31 + s) exact. d = 1: factor 0 stands for it.
+struct FastDiv {
+  uint32_t factor, shift;
+  FastDiv() = default;
+  explicit FastDiv(int64_t d) {
+    shift = 1;
+    while ((int64_t(1) << shift) < d) ++shift;
+    factor = d == 1 ? 0u
+                    : static_cast<uint32_t>(((uint64_t(1) << (31 + shift)) + d - 1) /
+                                            static_cast<uint64_t>(d));
+    --shift;
+  }
+  __device__ __forceinline__ uint32_t quotient(uint32_t n) const {
+    return factor == 0u ? n : __umulhi(n, factor) >> shift;
+  }
+};
+
 template <int D>
 struct Kv4Row {
   static constexpr int NG = D / 32;
