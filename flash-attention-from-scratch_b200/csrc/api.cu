@@ -500,11 +500,11 @@ int attn_paged_evict(void* const* arrays, const int64_t* row_bytes, int num_arra
   if (keep < 0 || recent < 0 || sinks < 0 || recent > keep || sinks > keep - recent)
     return fail(ATTN_ERR_INVALID, "%s: sinks and recent must be >= 0 and add up to keep at most",
                 name);
-  if (max_context_len > 0x7fffffffLL || max_blocks_per_seq > 0x7fffffffLL ||
+  if (max_context_len > 0x40000000LL || max_blocks_per_seq > 0x7fffffffLL ||
       new_max_blocks > 0x7fffffffLL || block_size > 0x10000 || num_blocks > 0x7fffffffLL ||
       keep > 0x7fffffffLL || num_kv_heads > 0x7fffffffLL || batch > 0x7fffffffLL ||
       batch * num_kv_heads > 0x7fffffffLL)
-    return fail(ATTN_ERR_UNSUPPORTED, "%s: sizes must fit in 31 bits (block_size <= 65536)", name);
+    return fail(ATTN_ERR_UNSUPPORTED, "%s: sizes must fit in 31 bits (max_context_len <= 2^30, block_size <= 65536)", name);
   if (max_context_len > max_blocks_per_seq * block_size)
     return fail(ATTN_ERR_INVALID, "%s: max_context_len needs more than max_blocks_per_seq blocks",
                 name);

@@ -32,6 +32,7 @@ struct FinishParams {
   int batch, hq, hkv, group, gp, bs, num_blocks, max_blocks, max_ctx;
   int merge_blocks;  // CTAs [0, merge_blocks) merge, the others add weights
   int add_chunks;    // CTAs per (sequence, kv head) that add
+  FastDiv by_bs;
 };
 
 // The parts of one (sequence, kv head) pair: part s of query head g is at
@@ -159,6 +160,95 @@ __device__ void merge_row(const FinishParams& p, long long row, bool live, const
 
 constexpr int kAddTokens = 1024;  // tokens a CTA adds at a time
 
+// The totals of up to kAddTokens tokens of one (sequence, kv head), GP scores a
+// token. A CTA's scores are on their way while it finds M and L of its query heads.
+template <int GP>
+__device__ void add_weights(const FinishParams& p) {
+  constexpr int U = kAddTokens / 256;  // tokens per thread
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int at = blockIdx.x - p.merge_blocks;
+  const int pair = at / p.add_chunks, chunk = at - pair * p.add_chunks;
+  const int b = pair / p.hkv, kvh = pair - b * p.hkv;
+  const int ctx = min(max(p.ctx[b], 0), p.max_ctx);
+  const long long stride = static_cast<long long>(p.add_chunks) * kAddTokens;
+  long long t0 = static_cast<long long>(chunk) * kAddTokens;
+  if (t0 >= ctx) return;
+  __shared__ float mx[8], inv[8];
+  const int* bt = p.bt + static_cast<size_t>(b) * p.max_blocks;
+  const float* sc = p.scores + static_cast<size_t>(pair) * p.max_ctx * GP;
+  float s[U][GP];
+  int page[U];
+  auto load = [&]() {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const long long t = t0 + u * 256 + threadIdx.x;
+      page[u] = -1;
+      if (t >= ctx) continue;
+      const float* src = sc + t * GP;
+      if constexpr (GP == 1) {
+        s[u][0] = *src;
+      } else if constexpr (GP == 2) {
+        const float2 x = *reinterpret_cast<const float2*>(src);
+        s[u][0] = x.x; s[u][1] = x.y;
+      } else {
+#pragma unroll
+        for (int i = 0; i < GP; i += 4) {
+          const float4 x = *reinterpret_cast<const float4*>(src + i);
+          s[u][i] = x.x; s[u][i + 1] = x.y; s[u][i + 2] = x.z; s[u][i + 3] = x.w;
+        }
+      }
+      page[u] = bt[p.by_bs.quotient(static_cast<uint32_t>(t))];
+    }
+  };
+  load();
+  const Parts r = parts_of(p, b, kvh, ctx);
+  if (warp < p.group) {
+    const long long base = r.base + warp * r.head;
+    float big = -INFINITY, sum = 0.f;
+    for (int i = lane; i < r.count; i += 32) {
+      const float m = p.m[base + i * r.stride], l = p.l[base + i * r.stride];
+      const float mn = fmaxf(big, m);
+      sum = (big == -INFINITY ? 0.f : sum * exp2f(big - mn)) + l * exp2f(m - mn);
+      big = mn;
+    }
+    const float all = warp_max(big);
+    sum = warp_sum(big == -INFINITY ? 0.f : sum * exp2f(big - all));
+    if (lane == 0) {
+      mx[warp] = all;
+      inv[warp] = 1.f / sum;
+    }
+  }
+  __syncthreads();
+  float mh[GP], ih[GP];
+#pragma unroll
+  for (int g = 0; g < GP; ++g) {
+    // Heads past the group (GP is a power of two) weigh nothing.
+    mh[g] = g < p.group ? mx[g] : 0.f;
+    ih[g] = g < p.group ? inv[g] : 0.f;
+  }
+  for (;;) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const long long t = t0 + u * 256 + threadIdx.x;
+      if (t >= ctx) continue;
+      float w = 0.f;
+#pragma unroll
+      for (int g = 0; g < GP; ++g)
+        if (g < p.group) w = fmaf(fast_exp2(s[u][g] - mh[g]), ih[g], w);
+      if (static_cast<unsigned>(page[u]) >= static_cast<unsigned>(p.num_blocks)) {
+        report_status(p.status, 2u /* ATTN_DEVICE_BAD_BLOCK */, kSiteWeightBlock);
+        continue;
+      }
+      const uint32_t n = static_cast<uint32_t>(t), off = n - p.by_bs.quotient(n) * p.bs;
+      // A page can stand in several sequences (a shared prefix): their adds all count.
+      atomicAdd(p.weights + (static_cast<size_t>(page[u]) * p.hkv + kvh) * p.bs + off, w);
+    }
+    t0 += stride;
+    if (t0 >= ctx) break;
+    load();
+  }
+}
+
 // Launched as a programmatic dependent of the decode: it waits for that launch's
 // end before it reads what the decode wrote.
 template <int D, int WPR, typename T>
@@ -180,45 +270,11 @@ __global__ void __launch_bounds__(256) finish_kernel(const FinishParams p) {
     merge_row<D, WPR, T>(p, row, live, r, g);
     return;
   }
-  const int at = blockIdx.x - p.merge_blocks;
-  const int pair = at / p.add_chunks, chunk = at - pair * p.add_chunks;
-  const int b = pair / p.hkv, kvh = pair - b * p.hkv;
-  const int ctx = min(max(p.ctx[b], 0), p.max_ctx);
-  if (static_cast<long long>(chunk) * kAddTokens >= ctx) return;
-  const Parts r = parts_of(p, b, kvh, ctx);
-  __shared__ float mx[8], inv[8];
-  if (warp < p.group) {
-    const long long base = r.base + warp * r.head;
-    float big = -INFINITY;
-    for (int s = lane; s < r.count; s += 32) big = fmaxf(big, p.m[base + s * r.stride]);
-    big = warp_max(big);
-    float sum = 0.f;
-    for (int s = lane; s < r.count; s += 32)
-      sum += p.l[base + s * r.stride] * exp2f(p.m[base + s * r.stride] - big);
-    sum = warp_sum(sum);
-    if (lane == 0) {
-      mx[warp] = big;
-      inv[warp] = 1.f / sum;
-    }
-  }
-  __syncthreads();
-  const int* bt = p.bt + static_cast<size_t>(b) * p.max_blocks;
-  const float* sc = p.scores + static_cast<size_t>(pair) * p.max_ctx * p.gp;
-  for (long long t0 = static_cast<long long>(chunk) * kAddTokens; t0 < ctx;
-       t0 += static_cast<long long>(p.add_chunks) * kAddTokens) {
-    const int end = static_cast<int>(min(static_cast<long long>(ctx), t0 + kAddTokens));
-    for (int t = static_cast<int>(t0) + threadIdx.x; t < end; t += 256) {
-      const float* s = sc + static_cast<size_t>(t) * p.gp;
-      float w = 0.f;
-      for (int g = 0; g < p.group; ++g) w += exp2f(s[g] - mx[g]) * inv[g];
-      const int page = bt[t / p.bs];
-      if (page < 0 || page >= p.num_blocks) {
-        report_status(p.status, 2u /* ATTN_DEVICE_BAD_BLOCK */, kSiteWeightBlock);
-        continue;
-      }
-      // A page can stand in several sequences (a shared prefix): their adds all count.
-      atomicAdd(p.weights + (static_cast<size_t>(page) * p.hkv + kvh) * p.bs + t % p.bs, w);
-    }
+  switch (p.gp) {
+    case 1: add_weights<1>(p); break;
+    case 2: add_weights<2>(p); break;
+    case 4: add_weights<4>(p); break;
+    default: add_weights<8>(p); break;
   }
 }
 
@@ -275,6 +331,7 @@ cudaError_t launch_finish(const FinishArgs& a, const LaunchCtx& ctx) {
   p.group = static_cast<int>(a.hq / a.hkv);
   p.gp = static_cast<int>(score_heads(p.group));
   p.bs = static_cast<int>(a.bs);
+  p.by_bs = FastDiv(a.bs);
   p.num_blocks = static_cast<int>(a.num_blocks);
   p.max_blocks = static_cast<int>(a.max_blocks);
   p.max_ctx = static_cast<int>(a.max_ctx);
