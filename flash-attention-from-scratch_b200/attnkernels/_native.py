@@ -15,6 +15,7 @@ from __future__ import annotations
 
 import contextlib
 import ctypes
+import functools
 import threading
 from pathlib import Path
 
@@ -109,15 +110,17 @@ def _ptr(t: torch.Tensor | None):
     return None if t is None else t.data_ptr()
 
 
-_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+def _raw_stream(idx: int):
+    """The current CUDA stream of device `idx` as an integer handle."""
+    return torch.cuda.current_stream(idx).cuda_stream
+
+
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", _raw_stream)
 
 
 def _stream(device: torch.device):
     """The current CUDA stream of `device` as an integer handle."""
-    idx = device.index if device.index is not None else torch.cuda.current_device()
-    if _raw_stream is not None:
-        return _raw_stream(idx)
-    return torch.cuda.current_stream(idx).cuda_stream
+    return _raw_stream(device.index if device.index is not None else torch.cuda.current_device())
 
 
 def _on(device: torch.device):
@@ -127,6 +130,14 @@ def _on(device: torch.device):
     if torch.cuda.current_device() == idx:
         return contextlib.nullcontext()
     return torch.cuda.device(idx)
+
+
+_SAME_DEVICE = contextlib.nullcontext()
+
+
+def _on_index(idx: int):
+    """_on for a device index."""
+    return _SAME_DEVICE if torch.cuda.current_device() == idx else torch.cuda.device(idx)
 
 
 def _workspace(nbytes: int, device: torch.device) -> torch.Tensor:
@@ -171,6 +182,12 @@ def _call_workspace(nbytes: int, device: torch.device, stream: int) -> torch.Ten
     if torch.cuda.is_current_stream_capturing():
         return _workspace(nbytes, device)
     return _decode_ws.get(nbytes, device, stream)
+
+
+@functools.lru_cache(maxsize=4096)
+def _workspace_bytes(query: str, *sizes) -> int:
+    """A workspace query of the library, which goes by its arguments alone."""
+    return getattr(library(), query)(*sizes)
 
 
 _DTYPES = {torch.float16: 0, torch.bfloat16: 1}  # ATTN_FP16, ATTN_BF16
@@ -270,67 +287,70 @@ class Extension:
                 int(head_dim), int(slot_stride), _ptr(out), _stream(out.device)))
         return out
 
-    def paged_decode_weights(self, q, kc, vc, bt, ctx, max_ctx, weights, scale, partition):
+    # The calls below are short on the GPU, so they keep the host side short: sizes
+    # come from the caller, which has checked them, and `dev` is the tensors' device
+    # index.
+    def paged_decode_weights(self, dev, q, kc, vc, bt, ctx, weights, sizes, max_ctx, scale,
+                             partition):
         out = torch.empty_like(q)
-        B, H, Hkv, D, bs, nblk, maxb = self._decode_sizes(q, kc, bt)
-        with _on(q.device):
-            stream = _stream(q.device)
-            ws = _call_workspace(
-                self.lib.attn_paged_decode_weights_workspace_bytes(B, H, Hkv, D, max_ctx,
-                                                                   partition), q.device, stream)
-            _check(self.lib.attn_paged_decode_weights(
-                _ptr(q), _ptr(kc), _ptr(vc), _ptr(bt), _ptr(ctx), _ptr(out), _ptr(weights), B, H,
-                Hkv, D, bs, nblk, maxb, max_ctx, scale, partition, _ptr(ws), ws.numel(), stream))
+        lib = self.lib
+        B, H, Hkv, D = sizes[:4]
+        with _on_index(dev):
+            stream = _raw_stream(dev)
+            ws = _call_workspace(_workspace_bytes("attn_paged_decode_weights_workspace_bytes", B, H,
+                                                  Hkv, D, max_ctx, partition), q.device, stream)
+            _check(lib.attn_paged_decode_weights(
+                q.data_ptr(), kc.data_ptr(), vc.data_ptr(), bt.data_ptr(), ctx.data_ptr(),
+                out.data_ptr(), weights.data_ptr(), *sizes, max_ctx, scale, partition,
+                ws.data_ptr(), ws.numel(), stream))
         return out
 
     # ------------------------------------------------- 4-bit cache, eviction
-    def kv4_append(self, k, v, kc, vc, slots, weights):
-        T, Hkv, D = k.shape
-        with _on(k.device):
+    def kv4_append(self, dev, k, v, kc, vc, slots, weights, sizes):
+        T, Hkv, D, bs, nblk = sizes
+        ks, vs = k.stride(), v.stride()
+        with _on_index(dev):
             _check(self.lib.attn_kv4_append(
-                _ptr(k), _ptr(v), _DTYPES[k.dtype], _ptr(kc), _ptr(vc), _ptr(slots),
-                _ptr(weights), T, Hkv, D, k.stride(0), k.stride(1), v.stride(0), v.stride(1),
-                kc.shape[2], kc.shape[0], _stream(k.device)))
+                k.data_ptr(), v.data_ptr(), _DTYPES[k.dtype], kc.data_ptr(), vc.data_ptr(),
+                slots.data_ptr(), None if weights is None else weights.data_ptr(), T, Hkv, D,
+                ks[0], ks[1], vs[0], vs[1], bs, nblk, _raw_stream(dev)))
 
-    def kv4_read(self, kc, vc, slots, head_dim, dtype):
-        T = slots.shape[0]
-        k, v = (torch.empty(T, kc.shape[1], head_dim, dtype=dtype, device=kc.device)
-                for _ in range(2))
-        with _on(kc.device):
+    def kv4_read(self, dev, kc, vc, slots, dtype, sizes):
+        T, Hkv, D, bs, nblk = sizes
+        k = kc.new_empty((T, Hkv, D), dtype=dtype)
+        v = torch.empty_like(k)
+        with _on_index(dev):
             _check(self.lib.attn_kv4_read(
-                _ptr(kc), _ptr(vc), _ptr(slots), _ptr(k), _ptr(v), _DTYPES[dtype], T, kc.shape[1],
-                head_dim, kc.shape[2], kc.shape[0], _stream(kc.device)))
+                kc.data_ptr(), vc.data_ptr(), slots.data_ptr(), k.data_ptr(), v.data_ptr(),
+                _DTYPES[dtype], T, Hkv, D, bs, nblk, _raw_stream(dev)))
         return k, v
 
-    def kv4_decode(self, q, kc, vc, bt, ctx, max_ctx, weights, scale):
+    def kv4_decode(self, dev, q, kc, vc, bt, ctx, weights, sizes, max_ctx, scale):
         out = torch.empty_like(q)
-        B, H, Hkv, D, bs, nblk, maxb = self._decode_sizes(q, kc, bt)
-        with _on(q.device):
-            stream = _stream(q.device)
-            ws = _call_workspace(
-                self.lib.attn_kv4_decode_workspace_bytes(B, H, Hkv, D, max_ctx,
-                                                         int(weights is not None)),
-                q.device, stream)
+        B, H, Hkv, D = sizes[:4]
+        with _on_index(dev):
+            stream = _raw_stream(dev)
+            ws = _call_workspace(_workspace_bytes("attn_kv4_decode_workspace_bytes", B, H, Hkv, D,
+                                                  max_ctx, 0 if weights is None else 1),
+                                 q.device, stream)
             _check(self.lib.attn_kv4_decode(
-                _ptr(q), _DTYPES[q.dtype], _ptr(kc), _ptr(vc), _ptr(bt), _ptr(ctx), _ptr(out),
-                _ptr(weights), B, H, Hkv, D, bs, nblk, maxb, max_ctx, scale, _ptr(ws), ws.numel(),
-                stream))
+                q.data_ptr(), _DTYPES[q.dtype], kc.data_ptr(), vc.data_ptr(), bt.data_ptr(),
+                ctx.data_ptr(), out.data_ptr(), None if weights is None else weights.data_ptr(),
+                *sizes, max_ctx, scale, ws.data_ptr(), ws.numel(), stream))
         return out
 
-    def paged_evict(self, caches, row_bytes, weights, bt, ctx, max_ctx, new_bt, keep, recent,
-                    sinks):
-        nblk, Hkv, bs = weights.shape
-        B = bt.shape[0]
-        i32 = dict(dtype=torch.int32, device=weights.device)
-        new_lens = torch.empty(B, **i32)
-        kept = torch.empty(B, Hkv, keep, **i32)
+    def paged_evict(self, dev, caches, row_bytes, weights, bt, ctx, new_bt, sizes, max_ctx, keep,
+                    recent, sinks):
+        B, Hkv, bs, nblk, maxb, new_maxb = sizes
+        new_lens = torch.empty(B, dtype=torch.int32, device=weights.device)
+        kept = torch.empty((B, Hkv, keep), dtype=torch.int32, device=weights.device)
         n = len(caches)
-        with _on(weights.device):
+        with _on_index(dev):
             _check(self.lib.attn_paged_evict(
                 (_vp * n)(*(c.data_ptr() for c in caches)), (_i64 * n)(*row_bytes), n,
-                _ptr(weights), _ptr(bt), _ptr(ctx), _ptr(new_bt), _ptr(new_lens), _ptr(kept), B,
-                Hkv, bs, nblk, bt.shape[1], max_ctx, new_bt.shape[1], keep, recent, sinks,
-                _stream(weights.device)))
+                weights.data_ptr(), bt.data_ptr(), ctx.data_ptr(), new_bt.data_ptr(),
+                new_lens.data_ptr(), kept.data_ptr(), B, Hkv, bs, nblk, maxb, max_ctx, new_maxb,
+                keep, recent, sinks, _raw_stream(dev)))
         return new_lens, kept
 
     # -------------------------------------------------------------- status

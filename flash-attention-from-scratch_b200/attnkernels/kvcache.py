@@ -32,71 +32,80 @@ import math
 
 import torch
 
-from . import load_extension, _check_decode, _decode_args
+from . import (CHUNK, decode_partition, load_extension, _check_decode, _decode_warps_per_sm,
+               _sm_count)
 
 _FLOATS = (torch.float16, torch.bfloat16)
+_ROW_BYTES = {64: 40, 128: 80}  # head_dim / 2 of codes, head_dim / 8 of scales and lows
+_HEAD_DIM = {v: k for k, v in _ROW_BYTES.items()}
 
 
 def kv4_row_bytes(head_dim):
     """Bytes of one 4-bit row: the last dim of a 4-bit cache (80 at head_dim 128, 40 at 64)."""
-    if head_dim not in (64, 128):
+    if head_dim not in _ROW_BYTES:
         raise ValueError("head_dim must be 64 or 128")
-    return head_dim // 2 + head_dim // 8
+    return _ROW_BYTES[head_dim]
 
 
-def _check_kv4_caches(k_cache, v_cache, head_dim=None):
-    """head_dim of a pair of 4-bit caches."""
-    dims = {kv4_row_bytes(d): d for d in (64, 128)}
-    for c in (k_cache, v_cache):
-        if c.dtype != torch.uint8 or c.dim() != 4 or c.shape[-1] not in dims:
-            raise ValueError("4-bit caches must be uint8 [num_blocks, H_kv, block_size, "
-                             "kv4_row_bytes(head_dim)]")
-        if not c.is_contiguous():
-            raise ValueError("4-bit caches must be contiguous")
-    if k_cache.shape != v_cache.shape:
+def _check_kv4_caches(k_cache, v_cache):
+    """(num_blocks, H_kv, block_size, head_dim) of a pair of 4-bit caches."""
+    shape = k_cache.shape
+    if len(shape) != 4 or shape[3] not in _HEAD_DIM or k_cache.dtype != torch.uint8 or \
+            v_cache.dtype != torch.uint8:
+        raise ValueError("4-bit caches must be uint8 [num_blocks, H_kv, block_size, "
+                         "kv4_row_bytes(head_dim)]")
+    if v_cache.shape != shape:
         raise ValueError("k_cache and v_cache must have the same shape")
-    d = dims[k_cache.shape[-1]]
-    if head_dim is not None and d != head_dim:
-        raise ValueError("head_dim must be 64 or 128 and match the cache")
-    return d
+    if not (k_cache.is_contiguous() and v_cache.is_contiguous()):
+        raise ValueError("4-bit caches must be contiguous")
+    nblk, hkv, bs, row = shape
+    return nblk, hkv, bs, _HEAD_DIM[row]
 
 
 def _check_weights(weights, num_blocks, hkv, block_size):
-    if weights.dtype != torch.float32 or tuple(weights.shape) != (num_blocks, hkv, block_size) \
+    if weights.dtype != torch.float32 or weights.shape != (num_blocks, hkv, block_size) \
             or not weights.is_contiguous():
         raise ValueError("weights must be contiguous fp32 [num_blocks, H_kv, block_size]")
 
 
-def _check_devices(*tensors):
-    if not all(t.is_cuda for t in tensors):
-        raise ValueError("tensors must be CUDA tensors")
-    if len({t.device for t in tensors}) != 1:
-        raise ValueError("tensors must be on one device")
+def _device_of(*tensors):
+    """Index of the one CUDA device that the tensors are on."""
+    dev = tensors[0].get_device()
+    for t in tensors:
+        if not t.is_cuda:
+            raise ValueError("tensors must be CUDA tensors")
+        if t.get_device() != dev:
+            raise ValueError("tensors must be on one device")
+    return dev
 
 
-def _check_lens(q_batch, block_tables, context_lens):
+def _check_lens(batch, block_tables, context_lens):
+    """max_blocks_per_seq."""
     if block_tables.dim() != 2 or context_lens.dim() != 1:
         raise ValueError("block_tables must be [B, max_blocks], context_lens [B]")
-    if block_tables.shape[0] != q_batch or context_lens.shape[0] != q_batch:
+    rows, blocks = block_tables.shape
+    if rows != batch or context_lens.shape[0] != batch:
         raise ValueError("block_tables and context_lens must have a row per sequence")
+    return blocks
 
 
-def _index32(t, device):
-    return t.to(device=device, dtype=torch.int32).contiguous()
+def _index(t, dev, device, dtype=torch.int32):
+    """t as a dense tensor of `dtype` on the device: itself where it is that already."""
+    if t.dtype == dtype and t.get_device() == dev and t.is_contiguous():
+        return t
+    return t.to(device=device, dtype=dtype).contiguous()
 
 
-def _check_slots(slots, tokens):
-    if slots.dim() != 1 or slots.dtype not in (torch.int32, torch.int64):
+def _check_slots(slots):
+    if slots.dim() != 1 or slots.dtype not in (torch.int64, torch.int32):
         raise ValueError("slots must be an int64 or int32 vector")
-    if tokens is not None and slots.shape[0] != tokens:
-        raise ValueError("slots must have one entry per token")
 
 
 def _dense_rows(t):
     """t, or a copy of it where its rows are not 16-byte pieces that the kernel can load."""
-    ok = t.stride(2) == 1 and t.stride(0) % 8 == 0 and t.stride(1) % 8 == 0 and \
-        t.data_ptr() % 16 == 0
-    return t if ok else t.contiguous()
+    s0, s1, s2 = t.stride()
+    return t if s2 == 1 and s0 % 8 == 0 and s1 % 8 == 0 and t.data_ptr() % 16 == 0 \
+        else t.contiguous()
 
 
 def paged_append_kv4(k, v, k_cache, v_cache, slots, weights=None):
@@ -113,38 +122,44 @@ def paged_append_kv4(k, v, k_cache, v_cache, slots, weights=None):
     nearest even. A group with an infinity, a NaN or a value beyond fp16's range reads back as
     NaN. A slot past the cache is not written and shows in device_status().
     """
-    if k.dtype not in _FLOATS or v.dtype != k.dtype or k.dim() != 3 or k.shape != v.shape:
+    shape = k.shape
+    if k.dtype not in _FLOATS or v.dtype != k.dtype or len(shape) != 3 or v.shape != shape:
         raise ValueError("k and v must be fp16 or bf16 tensors of one shape [T, H_kv, D]")
-    if k.shape[-1] not in (64, 128):
+    T, hkv, d = shape
+    if d not in _ROW_BYTES:
         raise ValueError("head_dim must be 64 or 128")
-    _check_kv4_caches(k_cache, v_cache, k.shape[-1])
-    if k_cache.shape[1] != k.shape[1]:
-        raise ValueError("k and the cache must have the same kv heads")
-    _check_slots(slots, k.shape[0])
-    tensors = [k, v, k_cache, v_cache, slots]
+    nblk, cache_hkv, bs, cache_d = _check_kv4_caches(k_cache, v_cache)
+    if (cache_hkv, cache_d) != (hkv, d):
+        raise ValueError("k and the cache must have the same kv heads and head_dim")
+    _check_slots(slots)
+    if slots.shape[0] != T:
+        raise ValueError("slots must have one entry per token")
+    dev = _device_of(k, v, k_cache, v_cache, slots)
     if weights is not None:
-        _check_weights(weights, *k_cache.shape[:3])
-        tensors.append(weights)
-    _check_devices(*tensors)
-    if k.shape[0] == 0:
+        _check_weights(weights, nblk, hkv, bs)
+        _device_of(k, weights)
+    if T == 0:
         return
-    load_extension().kv4_append(_dense_rows(k), _dense_rows(v), k_cache, v_cache,
-                                slots.to(torch.int64).contiguous(), weights)
+    load_extension().kv4_append(dev, _dense_rows(k), _dense_rows(v), k_cache, v_cache,
+                                _index(slots, dev, k.device, torch.int64), weights,
+                                (T, hkv, d, bs, nblk))
 
 
 def paged_read_kv4(k_cache, v_cache, slots, dtype=torch.float16):
     """Values of slots of a 4-bit paged cache: (k, v), each [T, H_kv, D] of `dtype` (fp16 or
     bf16), low + scale * code rounded once. A negative slot, or one past the cache (which also
     shows in device_status()), reads as zeros."""
-    d = _check_kv4_caches(k_cache, v_cache)
+    nblk, hkv, bs, d = _check_kv4_caches(k_cache, v_cache)
     if dtype not in _FLOATS:
         raise ValueError("dtype must be fp16 or bf16")
-    _check_slots(slots, None)
-    _check_devices(k_cache, v_cache, slots)
-    if slots.shape[0] == 0:
-        return tuple(torch.empty(0, k_cache.shape[1], d, dtype=dtype, device=k_cache.device)
-                     for _ in range(2))
-    return load_extension().kv4_read(k_cache, v_cache, slots.to(torch.int64).contiguous(), d, dtype)
+    _check_slots(slots)
+    dev = _device_of(k_cache, v_cache, slots)
+    T = slots.shape[0]
+    if T == 0:
+        return tuple(torch.empty(0, hkv, d, dtype=dtype, device=k_cache.device) for _ in range(2))
+    return load_extension().kv4_read(dev, k_cache, v_cache,
+                                     _index(slots, dev, k_cache.device, torch.int64), dtype,
+                                     (T, hkv, d, bs, nblk))
 
 
 def paged_decode_kv4(q, k_cache, v_cache, block_tables, context_lens, max_context_len,
@@ -162,32 +177,43 @@ def paged_decode_kv4(q, k_cache, v_cache, block_tables, context_lens, max_contex
     """
     if q.dtype not in _FLOATS:
         raise ValueError("q must be fp16 or bf16")
+    q3 = q
     if q.dim() == 4:
         if q.shape[2] != 1:
             raise ValueError("a 4-D decode q must be [B, H, 1, D]")
         q3 = q.reshape(q.shape[0], q.shape[1], q.shape[3])
-    elif q.dim() == 3:
-        q3 = q
-    else:
+    elif q.dim() != 3:
         raise ValueError("q must be [B, H, D] (or [B, H, 1, D])")
-    if q3.shape[-1] not in (64, 128):
+    B, H, D = q3.shape
+    nblk, hkv, bs, d = _check_kv4_caches(k_cache, v_cache)
+    if D != d:
         raise ValueError("head_dim must be 64 or 128 and match the cache")
-    _check_kv4_caches(k_cache, v_cache, q3.shape[-1])
-    _check_lens(q3.shape[0], block_tables, context_lens)
-    tensors = [q, k_cache, v_cache]
+    maxb = _check_lens(B, block_tables, context_lens)
+    dev = _device_of(q, k_cache, v_cache)
     if weights is not None:
-        _check_weights(weights, *k_cache.shape[:3])
-        tensors.append(weights)
-    _check_devices(*tensors)
-    if q3.shape[0] == 0 or max_context_len == 0:
+        _check_weights(weights, nblk, hkv, bs)
+        _device_of(q, weights)
+    max_context_len = int(max_context_len)
+    if B == 0 or max_context_len == 0:
         return torch.zeros_like(q)
-    scale = 1.0 / math.sqrt(q3.shape[-1]) if scale is None else scale
-    q3 = q3.contiguous()
-    if q3.data_ptr() % 16:
-        q3 = q3.clone()
-    return load_extension().kv4_decode(
-        q3, k_cache, v_cache, _index32(block_tables, q.device), _index32(context_lens, q.device),
-        int(max_context_len), weights, float(scale)).reshape(q.shape)
+    if not q3.is_contiguous() or q3.data_ptr() % 16:
+        q3 = q3.clone(memory_format=torch.contiguous_format)
+    out = load_extension().kv4_decode(
+        dev, q3, k_cache, v_cache, _index(block_tables, dev, q.device),
+        _index(context_lens, dev, q.device), weights, (B, H, hkv, D, bs, nblk, maxb),
+        max_context_len, 1.0 / math.sqrt(D) if scale is None else float(scale))
+    return out if q.dim() == 3 else out.reshape(q.shape)
+
+
+def _weights_partition(batch, hkv, max_context_len, dev, heads, head_dim):
+    """decode_partition's choice, doubled while that leaves six units per resident warp: fewer
+    parts to merge (64 ragged sequences of up to 8192 tokens, 32 query over 8 kv heads, d 128:
+    279 us at 256 tokens, 268 at 512, 305 at 1024, which leaves 3.5)."""
+    part = decode_partition(batch, hkv, max_context_len, dev, num_heads=heads, head_dim=head_dim)
+    units = 6 * _decode_warps_per_sm(heads // hkv, head_dim) * _sm_count(dev)
+    while batch * hkv * -(-max_context_len // (2 * part)) >= units:
+        part *= 2
+    return part
 
 
 def paged_decode_weights(q, k_cache, v_cache, block_tables, context_lens, max_context_len, weights,
@@ -200,18 +226,27 @@ def paged_decode_weights(q, k_cache, v_cache, block_tables, context_lens, max_co
     The other arguments and the result are paged_decode's; a length above max_context_len is cut
     to it.
     """
-    _check_decode(q, k_cache, v_cache)
-    if k_cache.dim() != 4 or k_cache.shape != v_cache.shape:
+    q3 = _check_decode(q, k_cache, v_cache)
+    shape = k_cache.shape
+    if len(shape) != 4 or v_cache.shape != shape:
         raise ValueError("k_cache and v_cache must be [num_blocks, H_kv, block_size, D]")
-    _check_weights(weights, *k_cache.shape[:3])
-    _check_lens(q.shape[0], block_tables, context_lens)
-    _check_devices(q, k_cache, v_cache, weights)
-    if q.shape[0] == 0 or max_context_len == 0:
+    nblk, hkv, bs, D = shape
+    B, H = q3.shape[:2]
+    _check_weights(weights, nblk, hkv, bs)
+    maxb = _check_lens(B, block_tables, context_lens)
+    dev = _device_of(q, k_cache, v_cache, weights)
+    if B == 0 or max_context_len == 0:
         return torch.zeros_like(q)
-    q3, kc, vc, bt, lens, max_ctx, scale, partition = _decode_args(
-        q, k_cache, v_cache, block_tables, context_lens, max_context_len, scale, partition_size)
-    return load_extension().paged_decode_weights(q3, kc, vc, bt, lens, max_ctx, weights, scale,
-                                                 partition).reshape(q.shape)
+    max_context_len = int(max_context_len)
+    if partition_size is None:
+        partition_size = _weights_partition(B, hkv, max_context_len, dev, H, D)
+    partition_size = -(-int(partition_size) // CHUNK) * CHUNK
+    out = load_extension().paged_decode_weights(
+        dev, q3.contiguous(), k_cache.contiguous(), v_cache.contiguous(),
+        _index(block_tables, dev, q.device), _index(context_lens, dev, q.device), weights,
+        (B, H, hkv, D, bs, nblk, maxb), max_context_len,
+        1.0 / math.sqrt(D) if scale is None else float(scale), partition_size)
+    return out if q.dim() == 3 else out.reshape(q.shape)
 
 
 def paged_evict(caches, weights, block_tables, context_lens, max_context_len, new_block_tables, keep,
@@ -237,29 +272,34 @@ def paged_evict(caches, weights, block_tables, context_lens, max_context_len, ne
     caches = tuple(caches)
     if not 1 <= len(caches) <= 8:
         raise ValueError("caches must be 1 to 8 tensors")
-    if weights.dim() != 3:
+    shape = weights.shape
+    if len(shape) != 3:
         raise ValueError("weights must be contiguous fp32 [num_blocks, H_kv, block_size]")
-    _check_weights(weights, *weights.shape)
+    nblk, hkv, bs = shape
+    _check_weights(weights, nblk, hkv, bs)
     row_bytes = []
     for c in caches:
-        if c.dim() < 3 or c.shape[:3] != weights.shape or not c.is_contiguous():
+        if c.dim() < 3 or c.shape[:3] != shape or not c.is_contiguous():
             raise ValueError("caches must be contiguous [num_blocks, H_kv, block_size, ...]")
         row = c.element_size() * math.prod(c.shape[3:])
         if not 0 < row <= 65536:
             raise ValueError("a cache row must have 1 to 65536 bytes")
         row_bytes.append(row)
-    _check_lens(block_tables.shape[0], block_tables, context_lens)
-    if new_block_tables.dim() != 2 or new_block_tables.shape[0] != block_tables.shape[0]:
+    if block_tables.dim() != 2:
+        raise ValueError("block_tables must be [B, max_blocks], context_lens [B]")
+    B = block_tables.shape[0]
+    maxb = _check_lens(B, block_tables, context_lens)
+    if new_block_tables.dim() != 2 or new_block_tables.shape[0] != B:
         raise ValueError("new_block_tables must be [B, new_max_blocks]")
     keep, recent, sinks = int(keep), int(recent), int(sinks)
     if keep < 1 or recent < 0 or sinks < 0 or recent + sinks > keep:
         raise ValueError("keep must be >= 1, sinks and recent >= 0 and together keep at most")
-    _check_devices(weights, *caches)
-    dev = weights.device
-    if block_tables.shape[0] == 0 or max_context_len == 0:
-        i32 = dict(dtype=torch.int32, device=dev)
-        return (torch.zeros(block_tables.shape[0], **i32),
-                torch.full((block_tables.shape[0], weights.shape[1], keep), -1, **i32))
+    dev, device = _device_of(weights, *caches), weights.device
+    max_context_len = int(max_context_len)
+    if B == 0 or max_context_len == 0:
+        return (torch.zeros(B, dtype=torch.int32, device=device),
+                torch.full((B, hkv, keep), -1, dtype=torch.int32, device=device))
     return load_extension().paged_evict(
-        caches, row_bytes, weights, _index32(block_tables, dev), _index32(context_lens, dev),
-        int(max_context_len), _index32(new_block_tables, dev), keep, recent, sinks)
+        dev, caches, row_bytes, weights, _index(block_tables, dev, device),
+        _index(context_lens, dev, device), _index(new_block_tables, dev, device),
+        (B, hkv, bs, nblk, maxb, new_block_tables.shape[1]), max_context_len, keep, recent, sinks)
