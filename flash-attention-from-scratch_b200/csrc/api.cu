@@ -627,14 +627,15 @@ int attn_kv4_decode(const void* q, int dtype, const void* k_cache, const void* v
     return fail(ATTN_ERR_UNSUPPORTED, "%s: num_heads / num_kv_heads must be 1 to 8", name);
   if (head_dim == 64 && block_size % 2 != 0)
     return fail(ATTN_ERR_UNSUPPORTED, "%s: head_dim 64 needs an even block_size", name);
-  // Tokens of a launch (up to 2048 sequences) over 32: counted in 31 bits.
-  if ((batch < 2048 ? batch : 2048) * ((max_context_len + 31) / 32) > 0x7fffffffLL)
-    return fail(ATTN_ERR_UNSUPPORTED, "%s: 2^36 tokens of context or more in 2048 sequences", name);
   if (num_kv_heads > 0x20000 || max_context_len > 0x40000000LL || max_blocks_per_seq > 0x7fffffffLL ||
       block_size > 0x10000 || num_blocks > 0x7fffffffLL || batch > 0x7fffffffLL ||
       num_heads > 0x7fffffffLL || batch * num_heads > 0x7fffffffLL)
     return fail(ATTN_ERR_UNSUPPORTED,
                 "%s: sizes must fit in 31 bits (max_context_len <= 2^30, block_size <= 65536)", name);
+  // 32-token stages of a launch (up to 2048 sequences), counted in 31 bits.
+  if ((batch < 2048 ? batch : 2048) * num_kv_heads * ((max_context_len + 31) / 32) > 0x7fffffffLL)
+    return fail(ATTN_ERR_UNSUPPORTED,
+                "%s: 2^36 tokens of context times kv heads, or more, in 2048 sequences", name);
   if (num_kv_heads * block_size * attn_kv4_row_bytes(head_dim) > 0x7fffffffLL)
     return fail(ATTN_ERR_UNSUPPORTED, "%s: a page of all kv heads must be below 2 GiB", name);
   if (max_context_len > max_blocks_per_seq * block_size)

@@ -27,7 +27,7 @@ struct FinishParams {
   const int* bt;
   void* out;
   DeviceStatus* status;
-  long long workers;
+  unsigned int workers;
   int partition, parts;
   int batch, hq, hkv, group, gp, bs, num_blocks, max_blocks, max_ctx;
   int merge_blocks;  // CTAs [0, merge_blocks) merge, the others add weights
@@ -51,17 +51,13 @@ __device__ __forceinline__ Parts parts_of(const FinishParams& p, int b, int kvh,
     r.head = p.parts;
     return r;
   }
-  const unsigned long long total = static_cast<unsigned long long>(p.first[p.batch]) * p.hkv;
   const int n = p.first[b + 1] - p.first[b];
   if (n == 0) return {0, 0, 0, 0};
-  const unsigned long long s0 =
-      static_cast<unsigned long long>(p.first[b]) * p.hkv + static_cast<unsigned long long>(kvh) * n;
-  // Worker i has the stages [i total / workers, (i + 1) total / workers).
-  const unsigned long long workers = min(static_cast<unsigned long long>(p.workers), total);
-  const long long i0 = static_cast<long long>(((s0 + 1) * workers - 1) / total);
-  const long long i1 = static_cast<long long>(((s0 + n) * workers - 1) / total);
+  const Runs runs(static_cast<unsigned int>(p.first[p.batch]) * p.hkv, p.workers);
+  const unsigned int s0 = static_cast<unsigned int>(p.first[b]) * p.hkv + kvh * n;
+  const unsigned int i0 = runs.of(s0), i1 = runs.of(s0 + n - 1);
   r.count = static_cast<int>(i1 - i0 + 1);
-  r.base = (i0 + static_cast<long long>(b) * p.hkv + kvh) * p.group;
+  r.base = (static_cast<long long>(i0) + b * p.hkv + kvh) * p.group;
   r.stride = p.group;
   r.head = 1;
   return r;
@@ -322,7 +318,7 @@ cudaError_t launch_finish(const FinishArgs& a, const LaunchCtx& ctx) {
   p.bt = a.block_tables;
   p.out = a.out;
   p.status = ctx.status;
-  p.workers = a.workers;
+  p.workers = static_cast<unsigned int>(a.workers);
   p.partition = static_cast<int>(a.partition);
   p.parts = static_cast<int>(a.parts);
   p.batch = static_cast<int>(a.batch);

@@ -39,6 +39,26 @@ struct FastDiv {
   }
 };
 
+// `total` stages dealt out in equal runs to n workers (one per stage, if that is
+// fewer): the first `more` workers have size + 1 stages, the others `size`.
+struct Runs {
+  unsigned int workers, size, more;
+  __device__ __forceinline__ Runs(unsigned int total, unsigned int n) {
+    workers = min(n, total);
+    size = workers == 0 ? 0 : total / workers;
+    more = total - size * workers;
+  }
+  // First stage of worker i.
+  __device__ __forceinline__ unsigned int begin(unsigned int i) const {
+    return size * i + min(i, more);
+  }
+  // The worker that has stage s.
+  __device__ __forceinline__ unsigned int of(unsigned int s) const {
+    const unsigned int big = more * (size + 1);
+    return s < big ? s / (size + 1) : more + (s - big) / size;
+  }
+};
+
 template <int D>
 struct Kv4Row {
   static constexpr int NG = D / 32;

@@ -7,11 +7,11 @@
 // laid out to spend few instructions on it.
 //
 //   * Warps are independent pipelines: bulk copies of whole page runs into a
-//     per-warp ring of 32-token stages, signalled by mbarriers.
+//     per-warp ring of stages (32 tokens at head_dim 128, 64 at 64), signalled by
+//     mbarriers.
 //   * The stages of all (sequence, kv head) rows, in that order, are dealt out to
-//     the resident warps in equal runs: warp i of n (at most S of them) takes stages
-//     [i S / n, (i + 1) S / n) of S. Every warp has the same work whatever the
-//     lengths are, without a work counter. A row that lies in one warp's run is
+//     the resident warps in equal runs (Runs, kv4.cuh): of S stages a warp takes
+//     S / n or one more, whatever the lengths are. A row that lies in one warp's run is
 //     written at once; of the others each warp leaves a part, in slot i + row,
 //     which no two (warp, row) pairs share, since along the runs one of the two
 //     grows at each step: n + rows slots are enough for any lengths.
@@ -44,12 +44,11 @@ namespace {
 
 enum : unsigned int { kSiteKv4Wait = 221, kSiteKv4Drain = 222, kSiteKv4Block = 223 };
 
-constexpr int kTok = 32;            // tokens per pipeline stage
 constexpr int kLaunchBatch = 2048;  // sequences per launch (their lengths live in shared memory)
 
-// Flags of a stage beside its tokens (at most 32): the first and the last of its
+// Flags of a stage beside its tokens (at most 64): the first and the last of its
 // row for this warp, and, with the last, the row lies wholly in this warp's run.
-enum : int { kTokens = 63, kFirst = 64, kLast = 128, kWhole = 256 };
+enum : int { kTokens = 127, kFirst = 128, kLast = 256, kWhole = 512 };
 
 #ifndef FAB_KV4_W
 #define FAB_KV4_W 16
@@ -65,9 +64,11 @@ struct Kv4Cfg {
   static constexpr int THREADS = W * 32;
   static constexpr int NG = R::NG;
   static constexpr int ROW = R::BYTES;
-  static constexpr int KV = kTok * ROW;  // K (or V) bytes of one stage
+  static constexpr int TOK = 4096 / D;  // tokens per stage: 5 KB of K and V either way
+  static constexpr int MT = TOK / 16;   // 16-token tiles of a stage
+  static constexpr int KV = TOK * ROW;  // K (or V) bytes of one stage
   static constexpr int STAGE = 2 * KV;
-  static constexpr int STAGES = D == 64 ? 2 * FAB_KV4_S : FAB_KV4_S;
+  static constexpr int STAGES = FAB_KV4_S;
   static constexpr int RING = STAGES * STAGE;
   static constexpr int BAR_OFF = W * RING;
   static constexpr int META_OFF = (BAR_OFF + W * STAGES * 8 + 15) / 16 * 16;
@@ -156,7 +157,7 @@ __device__ __forceinline__ float pow2i(int e) { return __int_as_float((e + 127) 
 template <int D, typename T, bool SCORED>
 __global__ void __launch_bounds__(Kv4Cfg<D>::THREADS, 1) kv4_decode_kernel(const Kv4DecParams p) {
   using C = Kv4Cfg<D>;
-  constexpr int NG = C::NG, ROW = C::ROW, CODES = C::R::CODES;
+  constexpr int NG = C::NG, ROW = C::ROW, CODES = C::R::CODES, kTok = C::TOK, MT = C::MT;
   extern __shared__ __align__(128) uint8_t smem[];
   // By a shuffle, which tells the compiler that it is the same in all lanes: the
   // producer's state then stays in uniform registers, which bulk copies are issued from.
@@ -213,16 +214,9 @@ __global__ void __launch_bounds__(Kv4Cfg<D>::THREADS, 1) kv4_decode_kernel(const
   // This warp's run of stages. Warps next to each other in number are on different
   // SMs, so that a small call spreads over all of them.
   const unsigned int worker = warp * gridDim.x + blockIdx.x;
-  const unsigned long long total = static_cast<unsigned long long>(prefix[p.batch]) * p.hkv;
-  // No more workers than stages: a worker between two others always has a part.
-  const unsigned long long workers =
-      min(static_cast<unsigned long long>(C::W * gridDim.x), total);
-  unsigned long long run0 = 0;
-  long long left = 0;
-  if (worker < workers) {
-    run0 = total * worker / workers;
-    left = static_cast<long long>(total * (worker + 1) / workers - run0);
-  }
+  const Runs runs(static_cast<unsigned int>(prefix[p.batch]) * p.hkv, C::W * gridDim.x);
+  const unsigned int run0 = runs.begin(worker);
+  unsigned int left = worker < runs.workers ? runs.begin(worker + 1) - run0 : 0u;
 
   // ---------------------------------------------------------- producer state
   int pb = 0, pkvh = 0, pst = 0, pnst = 0;  // the next stage: sequence, kv head, stage of that row
@@ -254,13 +248,13 @@ __global__ void __launch_bounds__(Kv4Cfg<D>::THREADS, 1) kv4_decode_kernel(const
     int lo = 0, hi = p.batch - 1;  // last sequence whose first stage is <= run0
     while (lo < hi) {
       const int mid = (lo + hi + 1) >> 1;
-      if (static_cast<unsigned long long>(prefix[mid]) * p.hkv <= run0) lo = mid; else hi = mid - 1;
+      if (static_cast<unsigned int>(prefix[mid]) * p.hkv <= run0) lo = mid; else hi = mid - 1;
     }
     pb = lo;
     pnst = prefix[lo + 1] - prefix[lo];
-    const unsigned long long in_seq = run0 - static_cast<unsigned long long>(prefix[lo]) * p.hkv;
-    pkvh = static_cast<int>(in_seq / pnst);
-    pst = static_cast<int>(in_seq - static_cast<unsigned long long>(pkvh) * pnst);
+    const unsigned int in_seq = run0 - static_cast<unsigned int>(prefix[lo]) * p.hkv;
+    pkvh = static_cast<int>(in_seq / static_cast<unsigned int>(pnst));
+    pst = static_cast<int>(in_seq) - pkvh * pnst;
     open_row();
   }
 
@@ -424,9 +418,9 @@ __global__ void __launch_bounds__(Kv4Cfg<D>::THREADS, 1) kv4_decode_kernel(const
 
     // Scores of the stage's tokens: s[i][0..1] token 16 i + tok_k, s[i][2..3] the
     // token after it.
-    float s[2][4];
+    float s[MT][4];
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < MT; ++i) {
       const uint8_t* ra = kst + (16 * i + tok_k) * ROW;
       const uint8_t* rb = ra + ROW;
       uint32_t xa[NG], xb[NG];
@@ -468,12 +462,12 @@ __global__ void __launch_bounds__(Kv4Cfg<D>::THREADS, 1) kv4_decode_kernel(const
       // Past the last token: no score; the ring's old bytes there must not reach
       // the products as a NaN scale or low either.
 #pragma unroll
-      for (int i = 0; i < 2; ++i)
+      for (int i = 0; i < MT; ++i)
 #pragma unroll
         for (int c = 0; c < 4; ++c)
           if (16 * i + tok_k + (c >> 1) >= nt) s[i][c] = -INFINITY;
-      if (lane >= nt) {
-        uint32_t* par = reinterpret_cast<uint32_t*>(vst + lane * ROW + CODES);
+      for (int r = nt + lane; r < kTok; r += 32) {
+        uint32_t* par = reinterpret_cast<uint32_t*>(vst + r * ROW + CODES);
 #pragma unroll
         for (int w = 0; w < NG; ++w) par[w] = 0u;
       }
@@ -482,7 +476,7 @@ __global__ void __launch_bounds__(Kv4Cfg<D>::THREADS, 1) kv4_decode_kernel(const
     if constexpr (SCORED) {
       if (2 * t4 < p.gp) {
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
+        for (int i = 0; i < MT; ++i)
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             const int tok = 16 * i + tok_k + h;
@@ -496,13 +490,15 @@ __global__ void __launch_bounds__(Kv4Cfg<D>::THREADS, 1) kv4_decode_kernel(const
           }
       }
     }
-    // Online softmax: per head the maximum over the 8 lanes of its 32 scores. P is
+    // Online softmax: per head the maximum over the 8 lanes of its scores. P is
     // held times 4, which keeps small P * scale in fp16's normal range longer and
     // cannot overflow (a scale is at most 8734).
     float alpha[2], shift[2];  // shift: 2 - m
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      float mx = fmaxf(fmaxf(s[0][h], s[0][h + 2]), fmaxf(s[1][h], s[1][h + 2]));
+      float mx = fmaxf(s[0][h], s[0][h + 2]);
+#pragma unroll
+      for (int i = 1; i < MT; ++i) mx = fmaxf(mx, fmaxf(s[i][h], s[i][h + 2]));
       mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
       mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
       mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
@@ -511,11 +507,11 @@ __global__ void __launch_bounds__(Kv4Cfg<D>::THREADS, 1) kv4_decode_kernel(const
       m[h] = mx;
       shift[h] = 2.f - mx;
     }
-    uint32_t pf[2][2];  // P^T as B fragments: tokens of rows 2 t4, 2 t4 + 1 (+ 8), head g4
+    uint32_t pf[MT][2];  // P^T as B fragments: tokens of rows 2 t4, 2 t4 + 1 (+ 8), head g4
     uint64_t add = f2_pack(0.f, 0.f);
     const uint64_t sh = f2_pack(shift[0], shift[1]);
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < MT; ++i) {
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
         float e0, e1;
@@ -543,7 +539,7 @@ __global__ void __launch_bounds__(Kv4Cfg<D>::THREADS, 1) kv4_decode_kernel(const
     }
     // O^T += V^T P^T.
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < MT; ++i) {
       const uint8_t* ra = vst + (16 * i + 2 * t4) * ROW;  // rows 2 t4 and (below, + ROW) 2 t4 + 8
       const uint8_t* rb = vst + (16 * i + tok_v) * ROW;   // rows 2 t4 + 1 and 2 t4 + 9
       uint32_t va[NG / 2], vb[NG / 2], vc[NG / 2], vd[NG / 2];
@@ -714,6 +710,7 @@ cudaError_t launch_kv4_decode(const Kv4DecodeArgs& a, const LaunchCtx& ctx) {
     return cudaMemsetAsync(a.out, 0, static_cast<size_t>(a.batch) * a.hq * a.d * 2, ctx.stream);
   Workspace w = carve(a.workspace, a.batch, a.hq, a.hkv, a.d, 0);
   const int64_t warps = a.d == 64 ? Kv4Cfg<64>::W : Kv4Cfg<128>::W;
+  const int64_t tok = a.d == 64 ? Kv4Cfg<64>::TOK : Kv4Cfg<128>::TOK;
   for (int64_t b0 = 0; b0 < a.batch; b0 += kLaunchBatch) {
     const int64_t nb = std::min<int64_t>(kLaunchBatch, a.batch - b0);
     const int64_t row_bytes = a.d / 2 + a.d / 8, row0 = b0 * a.hq;
@@ -743,7 +740,7 @@ cudaError_t launch_kv4_decode(const Kv4DecodeArgs& a, const LaunchCtx& ctx) {
     p.max_ctx = static_cast<int>(a.max_ctx);
     p.scale_log2 = a.scale * kLog2e;
     // One CTA per SM, or one per stage when there cannot be that many.
-    const int64_t stages = nb * a.hkv * ((a.max_ctx + kTok - 1) / kTok);
+    const int64_t stages = nb * a.hkv * ((a.max_ctx + tok - 1) / tok);
     const int grid = static_cast<int>(
         std::min<int64_t>(std::min<int64_t>(ctx.sm_count, kMaxWorkers / warps), stages));
     cudaError_t e;
@@ -759,7 +756,7 @@ cudaError_t launch_kv4_decode(const Kv4DecodeArgs& a, const LaunchCtx& ctx) {
     f.context_lens = p.ctx;
     f.first = w.first;
     f.workers = static_cast<int64_t>(grid) * warps;
-    f.partition = kTok;
+    f.partition = tok;
     f.parts = 0;
     f.scores = p.scores;
     f.weights = a.weights;
