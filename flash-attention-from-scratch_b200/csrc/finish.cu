@@ -63,9 +63,10 @@ __device__ __forceinline__ Parts parts_of(const FinishParams& p, int b, int kvh,
   return r;
 }
 
-// WPR warps per row (1 or 8) merge: lane owns D / 32 columns; each warp folds
+// WPR warps per row (1, 8 or 32) merge: lane owns D / 32 columns; each warp folds
 // chunks of 8 parts into a running (max, sum, numerator), and the warps of a row
-// combine in shared memory.
+// combine in shared memory. A chunk is one round trip to memory, so rows with many
+// parts (few rows, a long context) take more warps.
 template <int D, int WPR, typename T>
 __device__ void merge_row(const FinishParams& p, long long row, bool live, const Parts& r, int g) {
   constexpr int DV = D / 32;
@@ -123,7 +124,7 @@ __device__ void merge_row(const FinishParams& p, long long row, bool live, const
     }
   }
   if constexpr (WPR > 1) {
-    __shared__ float red[8][D + 2];
+    __shared__ float red[WPR][D + 2];
 #pragma unroll
     for (int j = 0; j < DV; ++j) red[warp][lane * DV + j] = num[j];
     if (lane == 0) {
@@ -154,13 +155,17 @@ __device__ void merge_row(const FinishParams& p, long long row, bool live, const
   for (int j = 0; j < DV; j += 2) dst[j / 2] = pack2<T>(num[j] * inv, num[j + 1] * inv);
 }
 
+// Threads of a CTA.
+template <int WPR>
+constexpr int kThreads = WPR == 32 ? 1024 : 256;
+
 constexpr int kAddTokens = 1024;  // tokens a CTA adds at a time
 
 // The totals of up to kAddTokens tokens of one (sequence, kv head), GP scores a
 // token. A CTA's scores are on their way while it finds M and L of its query heads.
-template <int GP>
+template <int GP, int THREADS>
 __device__ void add_weights(const FinishParams& p) {
-  constexpr int U = kAddTokens / 256;  // tokens per thread
+  constexpr int U = kAddTokens / THREADS;  // tokens per thread
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int at = blockIdx.x - p.merge_blocks;
   const int pair = at / p.add_chunks, chunk = at - pair * p.add_chunks;
@@ -177,7 +182,7 @@ __device__ void add_weights(const FinishParams& p) {
   auto load = [&]() {
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const long long t = t0 + u * 256 + threadIdx.x;
+      const long long t = t0 + u * THREADS + threadIdx.x;
       page[u] = -1;
       if (t >= ctx) continue;
       const float* src = sc + t * GP;
@@ -225,7 +230,7 @@ __device__ void add_weights(const FinishParams& p) {
   for (;;) {
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const long long t = t0 + u * 256 + threadIdx.x;
+      const long long t = t0 + u * THREADS + threadIdx.x;
       if (t >= ctx) continue;
       float w = 0.f;
 #pragma unroll
@@ -248,11 +253,12 @@ __device__ void add_weights(const FinishParams& p) {
 // Launched as a programmatic dependent of the decode: it waits for that launch's
 // end before it reads what the decode wrote.
 template <int D, int WPR, typename T>
-__global__ void __launch_bounds__(256) finish_kernel(const FinishParams p) {
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+__global__ void __launch_bounds__(kThreads<WPR>) finish_kernel(const FinishParams p) {
+  constexpr int THREADS = kThreads<WPR>;
+  const int warp = threadIdx.x >> 5;
   asm volatile("griddepcontrol.wait;" ::: "memory");
   if (static_cast<int>(blockIdx.x) < p.merge_blocks) {
-    const long long row = static_cast<long long>(blockIdx.x) * (8 / WPR) + warp / WPR;
+    const long long row = static_cast<long long>(blockIdx.x) * (THREADS / 32 / WPR) + warp / WPR;
     bool live = row < static_cast<long long>(p.batch) * p.hq;
     Parts r = {0, 0, 0, 0};
     int g = 0;
@@ -267,10 +273,10 @@ __global__ void __launch_bounds__(256) finish_kernel(const FinishParams p) {
     return;
   }
   switch (p.gp) {
-    case 1: add_weights<1>(p); break;
-    case 2: add_weights<2>(p); break;
-    case 4: add_weights<4>(p); break;
-    default: add_weights<8>(p); break;
+    case 1: add_weights<1, THREADS>(p); break;
+    case 2: add_weights<2, THREADS>(p); break;
+    case 4: add_weights<4, THREADS>(p); break;
+    default: add_weights<8, THREADS>(p); break;
   }
 }
 
@@ -278,7 +284,7 @@ template <int D, int WPR, typename T>
 cudaError_t launch(const FinishParams& p, unsigned grid, cudaStream_t stream) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(grid);
-  cfg.blockDim = dim3(256);
+  cfg.blockDim = dim3(kThreads<WPR>);
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -292,6 +298,14 @@ template <int D, int WPR>
 cudaError_t by_type(const FinishParams& p, unsigned grid, bool bf16, cudaStream_t stream) {
   return bf16 ? launch<D, WPR, __nv_bfloat16>(p, grid, stream)
               : launch<D, WPR, __half>(p, grid, stream);
+}
+
+template <int D>
+cudaError_t by_warps(const FinishParams& p, unsigned grid, int wpr, bool bf16,
+                     cudaStream_t stream) {
+  return wpr == 32  ? by_type<D, 32>(p, grid, bf16, stream)
+         : wpr == 8 ? by_type<D, 8>(p, grid, bf16, stream)
+                    : by_type<D, 1>(p, grid, bf16, stream);
 }
 
 }  // namespace
@@ -332,13 +346,13 @@ cudaError_t launch_finish(const FinishArgs& a, const LaunchCtx& ctx) {
   p.max_blocks = static_cast<int>(a.max_blocks);
   p.max_ctx = static_cast<int>(a.max_ctx);
   const int64_t rows = a.batch * a.hq;
-  // Eight warps per row where a row can have 32 parts or more (four per warp).
+  // Warps per row by the parts a row can have: up to four chunks of 8 a warp.
   const int64_t per_row = a.first == nullptr
                               ? a.parts
                               : std::min((a.max_ctx + a.partition - 1) / a.partition,
                                          a.workers / (a.batch * a.hkv) + 1);
-  const bool wide = per_row >= 32;
-  const int64_t merge = wide ? rows : (rows + 7) / 8;
+  const int wpr = per_row >= 128 ? 32 : per_row >= 32 ? 8 : 1;
+  const int64_t merge = wpr == 1 ? (rows + 7) / 8 : rows;
   // CTAs that add: one per 1024 tokens of a pair, fewer (each then walks on) where
   // that would be more than a launch's grid holds.
   const int64_t pairs = a.batch * a.hkv;
@@ -351,11 +365,8 @@ cudaError_t launch_finish(const FinishArgs& a, const LaunchCtx& ctx) {
   p.merge_blocks = static_cast<int>(merge);
   p.add_chunks = static_cast<int>(chunks);
   const unsigned grid = static_cast<unsigned>(merge + pairs * chunks);
-  if (a.d == 64)
-    return wide ? by_type<64, 8>(p, grid, a.bf16, ctx.stream)
-                : by_type<64, 1>(p, grid, a.bf16, ctx.stream);
-  return wide ? by_type<128, 8>(p, grid, a.bf16, ctx.stream)
-              : by_type<128, 1>(p, grid, a.bf16, ctx.stream);
+  return a.d == 64 ? by_warps<64>(p, grid, wpr, a.bf16, ctx.stream)
+                   : by_warps<128>(p, grid, wpr, a.bf16, ctx.stream);
 }
 
 }  // namespace fab
