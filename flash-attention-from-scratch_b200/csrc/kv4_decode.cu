@@ -7,7 +7,7 @@
 // laid out to spend few instructions on it.
 //
 //   * Warps are independent pipelines: bulk copies of whole page runs into a
-//     per-warp ring of stages (32 tokens at head_dim 128, 64 at 64), signalled by
+//     per-warp ring of stages (48 tokens at head_dim 128, 64 at 64), signalled by
 //     mbarriers.
 //   * The stages of all (sequence, kv head) rows, in that order, are dealt out to
 //     the resident warps in equal runs (Runs, kv4.cuh): of S stages a warp takes
@@ -51,7 +51,7 @@ constexpr int kLaunchBatch = 2048;  // sequences per launch (their lengths live 
 enum : int { kTokens = 127, kFirst = 128, kLast = 256, kWhole = 512 };
 
 #ifndef FAB_KV4_W
-#define FAB_KV4_W 16
+#define FAB_KV4_W 12
 #endif
 #ifndef FAB_KV4_S
 #define FAB_KV4_S 2
@@ -64,7 +64,11 @@ struct Kv4Cfg {
   static constexpr int THREADS = W * 32;
   static constexpr int NG = R::NG;
   static constexpr int ROW = R::BYTES;
-  static constexpr int TOK = 4096 / D;  // tokens per stage: 5 KB of K and V either way
+  // Tokens per stage. Measured (us, 64 ragged sequences of up to 8192 tokens / 8 of
+  // 131072, 8 kv heads, d 128): 16 warps of 32 tokens 91.0 / 241.6, 12 of 48
+  // 89.1 / 241.2, 8 of 64 97.4 / 268.9, 20 of 32 (registers spill) 102 / 265; one
+  // sequence of 700 tokens 9.5, 8.4, 8.7.
+  static constexpr int TOK = D == 64 ? 64 : 48;
   static constexpr int MT = TOK / 16;   // 16-token tiles of a stage
   static constexpr int KV = TOK * ROW;  // K (or V) bytes of one stage
   static constexpr int STAGE = 2 * KV;
