@@ -171,34 +171,38 @@ __device__ void add_weights(const FinishParams& p) {
   const int pair = at / p.add_chunks, chunk = at - pair * p.add_chunks;
   const int b = pair / p.hkv, kvh = pair - b * p.hkv;
   const int ctx = min(max(p.ctx[b], 0), p.max_ctx);
-  const long long stride = static_cast<long long>(p.add_chunks) * kAddTokens;
-  long long t0 = static_cast<long long>(chunk) * kAddTokens;
-  if (t0 >= ctx) return;
+  // Lengths are below 2^31, a chunk past the end of one below 2^32.
+  unsigned int t0 = static_cast<unsigned int>(chunk) * kAddTokens;
+  const unsigned int stride = static_cast<unsigned int>(p.add_chunks) * kAddTokens;
+  const unsigned int end = static_cast<unsigned int>(ctx);
+  if (t0 >= end) return;
   __shared__ float mx[8], inv[8];
   const int* bt = p.bt + static_cast<size_t>(b) * p.max_blocks;
   const float* sc = p.scores + static_cast<size_t>(pair) * p.max_ctx * GP;
+  float* totals = p.weights + static_cast<size_t>(kvh) * p.bs;
+  const unsigned int page_stride = static_cast<unsigned int>(p.hkv) * p.bs;
   float s[U][GP];
   int page[U];
   auto load = [&]() {
+    const float* src = sc + (static_cast<size_t>(t0) + threadIdx.x) * GP;
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const long long t = t0 + u * THREADS + threadIdx.x;
-      page[u] = -1;
-      if (t >= ctx) continue;
-      const float* src = sc + t * GP;
+      const unsigned int t = t0 + u * THREADS + threadIdx.x;
+      if (t >= end) break;
+      const float* at = src + u * THREADS * GP;
       if constexpr (GP == 1) {
-        s[u][0] = *src;
+        s[u][0] = *at;
       } else if constexpr (GP == 2) {
-        const float2 x = *reinterpret_cast<const float2*>(src);
+        const float2 x = *reinterpret_cast<const float2*>(at);
         s[u][0] = x.x; s[u][1] = x.y;
       } else {
 #pragma unroll
         for (int i = 0; i < GP; i += 4) {
-          const float4 x = *reinterpret_cast<const float4*>(src + i);
+          const float4 x = *reinterpret_cast<const float4*>(at + i);
           s[u][i] = x.x; s[u][i + 1] = x.y; s[u][i + 2] = x.z; s[u][i + 3] = x.w;
         }
       }
-      page[u] = bt[p.by_bs.quotient(static_cast<uint32_t>(t))];
+      page[u] = bt[p.by_bs.quotient(t)];
     }
   };
   load();
@@ -230,8 +234,8 @@ __device__ void add_weights(const FinishParams& p) {
   for (;;) {
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const long long t = t0 + u * THREADS + threadIdx.x;
-      if (t >= ctx) continue;
+      const unsigned int t = t0 + u * THREADS + threadIdx.x;
+      if (t >= end) break;
       float w = 0.f;
 #pragma unroll
       for (int g = 0; g < GP; ++g)
@@ -240,12 +244,12 @@ __device__ void add_weights(const FinishParams& p) {
         report_status(p.status, 2u /* ATTN_DEVICE_BAD_BLOCK */, kSiteWeightBlock);
         continue;
       }
-      const uint32_t n = static_cast<uint32_t>(t), off = n - p.by_bs.quotient(n) * p.bs;
       // A page can stand in several sequences (a shared prefix): their adds all count.
-      atomicAdd(p.weights + (static_cast<size_t>(page[u]) * p.hkv + kvh) * p.bs + off, w);
+      atomicAdd(totals + static_cast<unsigned long long>(static_cast<unsigned>(page[u])) * page_stride +
+                    (t - p.by_bs.quotient(t) * p.bs), w);
     }
     t0 += stride;
-    if (t0 >= ctx) break;
+    if (t0 >= end) break;
     load();
   }
 }
@@ -353,13 +357,15 @@ cudaError_t launch_finish(const FinishArgs& a, const LaunchCtx& ctx) {
                                          a.workers / (a.batch * a.hkv) + 1);
   const int wpr = per_row >= 128 ? 32 : per_row >= 32 ? 8 : 1;
   const int64_t merge = wpr == 1 ? (rows + 7) / 8 : rows;
-  // CTAs that add: one per 1024 tokens of a pair, fewer (each then walks on) where
-  // that would be more than a launch's grid holds.
+  // CTAs that add: one per 1024 tokens of a pair, but no more than about six per SM,
+  // each then walking on: finding M and L costs a CTA as much as the tokens of one
+  // such step (64 ragged sequences of up to 8192 tokens, 8 kv heads of 4 query heads,
+  // fp16 / 4-bit decode with weights, us: 263 / 117; one step per CTA 265 / 122).
   const int64_t pairs = a.batch * a.hkv;
   int64_t chunks = 0;
   if (a.scores != nullptr) {
     chunks = std::max<int64_t>(1, (a.max_ctx + kAddTokens - 1) / kAddTokens);
-    chunks = std::min(chunks, std::max<int64_t>(1, (int64_t(1) << 30) / pairs));
+    chunks = std::min(chunks, std::max<int64_t>(1, 6 * int64_t(ctx.sm_count) / pairs));
   }
   if (merge + pairs * chunks > 0x7fffffffLL) return cudaErrorInvalidConfiguration;
   p.merge_blocks = static_cast<int>(merge);

@@ -52,6 +52,20 @@ __device__ __forceinline__ uint32_t min2_nan(uint32_t a, uint32_t b, __nv_bfloat
                                        *reinterpret_cast<__nv_bfloat162*>(&b));
   return *reinterpret_cast<const uint32_t*>(&r);
 }
+__device__ __forceinline__ uint32_t max2_nan(uint32_t a, uint32_t b, __half) {
+  const __half2 r = __hmax2_nan(*reinterpret_cast<__half2*>(&a), *reinterpret_cast<__half2*>(&b));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+__device__ __forceinline__ uint32_t max2_nan(uint32_t a, uint32_t b, __nv_bfloat16) {
+  const __nv_bfloat162 r = __hmax2_nan(*reinterpret_cast<__nv_bfloat162*>(&a),
+                                       *reinterpret_cast<__nv_bfloat162*>(&b));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+__device__ __forceinline__ float approx_rcp(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
 __device__ __forceinline__ void unpack2(uint32_t v, float& lo, float& hi, __half) {
   const float2 f = __half22float2(*reinterpret_cast<__half2*>(&v));
   lo = f.x;
@@ -80,8 +94,8 @@ __device__ __forceinline__ void append_row(uint8_t* dst, uint4 raw, bool real, i
   using R = Kv4Row<D>;
   // min and -max (the sign flipped) of the group, together in one register.
   uint32_t lo2 = min2_nan(min2_nan(raw.x, raw.y, T()), min2_nan(raw.z, raw.w, T()), T());
-  uint32_t hi2 = min2_nan(min2_nan(raw.x ^ 0x80008000u, raw.y ^ 0x80008000u, T()),
-                          min2_nan(raw.z ^ 0x80008000u, raw.w ^ 0x80008000u, T()), T());
+  uint32_t hi2 =
+      max2_nan(max2_nan(raw.x, raw.y, T()), max2_nan(raw.z, raw.w, T()), T()) ^ 0x80008000u;
   uint32_t ends = min2_nan(__byte_perm(lo2, hi2, 0x5410), __byte_perm(lo2, hi2, 0x7632), T());
   ends = min2_nan(ends, __shfl_xor_sync(0xffffffffu, ends, 1), T());
   ends = min2_nan(ends, __shfl_xor_sync(0xffffffffu, ends, 2), T());
@@ -100,50 +114,48 @@ __device__ __forceinline__ void append_row(uint8_t* dst, uint4 raw, bool real, i
   if (!(fabsf(lo) <= 65504.f && fabsf(neg_hi) <= 65504.f))
     lo_h = scale_h = __ushort_as_half(0x7fff);  // NaN
   const float scale = __half2float(scale_h);
-  uint32_t word = 0;
-  if (scale > 0.f) {
-    const float inv = __fdividef(1.f, scale);
-    float x[8];
-    unpack2(raw.x, x[0], x[1], T());
-    unpack2(raw.y, x[2], x[3], T());
-    unpack2(raw.z, x[4], x[5], T());
-    unpack2(raw.w, x[6], x[7], T());
-    // Codes by adding 1.5 2^23, which rounds the quotient to a whole number in the
-    // sum's low bits; the sums' other bits add up to a constant.
-    constexpr float kBig = 12582912.f;
-    constexpr uint32_t kBits = 0x4B400000u;
-    constexpr uint32_t kAll = kBits * 0x11111111u;  // kBits << 0, 4, ..., 28
-    const uint64_t low2 = f2_pack(-low, -low), inv2 = f2_pack(inv, inv);
-    const uint64_t big2 = f2_pack(kBig, kBig), unbig2 = f2_pack(-kBig, -kBig);
-    const uint64_t minus2 = f2_pack(-1.f, -1.f);
-    float d[8];
-    uint32_t sum = 0;
+  const bool live = scale > 0.f;  // not 0, not NaN
+  const float inv = live ? approx_rcp(scale) : 0.f;
+  float x[8];
+  unpack2(raw.x, x[0], x[1], T());
+  unpack2(raw.y, x[2], x[3], T());
+  unpack2(raw.z, x[4], x[5], T());
+  unpack2(raw.w, x[6], x[7], T());
+  // Codes by adding 1.5 2^23, which rounds the quotient to a whole number in the
+  // sum's low bits; the sums' other bits add up to a constant.
+  constexpr float kBig = 12582912.f;
+  constexpr uint32_t kBits = 0x4B400000u;
+  constexpr uint32_t kAll = kBits * 0x11111111u;  // kBits << 0, 4, ..., 28
+  const uint64_t low2 = f2_pack(-low, -low), inv2 = f2_pack(inv, inv);
+  const uint64_t big2 = f2_pack(kBig, kBig), unbig2 = f2_pack(-kBig, -kBig);
+  const uint64_t minus2 = f2_pack(-1.f, -1.f);
+  float d[8], off = 0.f;
+  uint32_t sum = 0;
 #pragma unroll
-    for (int i = 0; i < 8; i += 2) {
-      const uint64_t r = f2_mul(f2_add(f2_pack(x[i], x[i + 1]), low2), inv2);
-      const uint64_t n = f2_add(r, big2);
-      float n0, n1;
-      f2_unpack(f2_fma(f2_add(n, unbig2), minus2, r), d[i], d[i + 1]);
-      f2_unpack(n, n0, n1);
-      sum += __float_as_uint(n0) * (1u << (4 * i));
-      sum += __float_as_uint(n1) * (1u << (4 * i + 4));
-    }
-    word = sum - kAll;
-    // The quotient above is off by a few fp32 roundings (below 2^-17 of a code). Next
-    // to a half it is the sign of x - low - (n + 1/2) scale that decides, exact in 64
-    // bits, and of an exact half the even code stands.
-    float off = 0.f;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) off = fmaxf(off, fabsf(d[i]));
+  for (int i = 0; i < 8; i += 2) {
+    const uint64_t r = f2_mul(f2_add(f2_pack(x[i], x[i + 1]), low2), inv2);
+    const uint64_t n = f2_add(r, big2);
+    float n0, n1;
+    f2_unpack(f2_fma(f2_add(n, unbig2), minus2, r), d[i], d[i + 1]);
+    f2_unpack(n, n0, n1);
+    sum += __float_as_uint(n0) * (1u << (4 * i));
+    sum += __float_as_uint(n1) * (1u << (4 * i + 4));
+    off = fmaxf(off, fmaxf(fabsf(d[i]), fabsf(d[i + 1])));
+  }
+  uint32_t word = live ? sum - kAll : 0u;
+  // The quotient above is off by a few fp32 roundings (below 2^-17 of a code). Next
+  // to a half it is the sign of x - low - (n + 1/2) scale that decides, exact in 64
+  // bits, and of an exact half the even code stands. A scale below fp16's normal
+  // range is rounded so coarsely that quotients can pass 15.5.
+  if (live && (off > 0.5f - 0x1p-16f || scale < 0x1p-14f)) {
     if (scale < 0x1p-14f) {
-      // A scale rounded that coarsely lets quotients pass 15.5.
       word = 0;
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         const double q = (static_cast<double>(x[i]) - low) / static_cast<double>(scale);
         word |= static_cast<uint32_t>(fmin(fmax(rint(q), 0.0), 15.0)) << (4 * i);
       }
-    } else if (off > 0.5f - 0x1p-16f) {
+    } else {
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         if (fabsf(d[i]) <= 0.5f - 0x1p-16f) continue;
@@ -175,7 +187,9 @@ __device__ __forceinline__ void append_row(uint8_t* dst, uint4 raw, bool real, i
 }
 
 // A lane takes its 8 values of K and of V of one (token, head): the slot and its
-// row in the cache are found once for both.
+// row in the cache are found once for both. Bound by the instructions it issues (330
+// for the two, half of them the codes): 32768 tokens of 32 heads, d 128, bf16, B200:
+// 209 us for 705 MB (3.4 TB/s); with 64-bit divisions and one tensor per thread 628.
 template <int D, typename T>
 __global__ void __launch_bounds__(256) kv4_append_kernel(const Kv4CopyParams p) {
   using R = Kv4Row<D>;
@@ -254,7 +268,7 @@ __device__ __forceinline__ uint4 values_of(uint32_t v, uint16_t scale_h, uint16_
 
 // Lane (w, t) of a row reads the word of its codes (of V the word that it traded
 // when writing) and its group's scale and low of K and of V. Slots below 0 read as
-// zeros.
+// zeros. The shape above: 142 us (5.0 TB/s).
 template <int D, typename T>
 __global__ void __launch_bounds__(256) kv4_read_kernel(const Kv4CopyParams p) {
   using R = Kv4Row<D>;
