@@ -28,9 +28,16 @@
 //     the end.
 //   * A group's scale stays outside the product over the codes: K has one fp32
 //     accumulator per group, combined as sum_w scale_w acc_w in fp32; V's scales
-//     multiply P (in fp16) before each group's columns. The lows are one product
-//     more: low . (sum of q over the group), with that sum as two fp16 terms (22
-//     bits), and P . low for V.
+//     multiply P before each group's columns. The lows are one product more:
+//     low . (sum of q over the group), with that sum as two fp16 terms (22 bits).
+//   * The sums over a long context are kept centred. sum p v is near 0 where
+//     sum p scale code and sum p low are not, so V is summed as
+//         sum (p scale) (code - c) + sum p (low + c scale),   c = 8, 7 in turn:
+//     one product with the constants -c per tile and accumulator, and fp16 middles in
+//     the lows' place. (Summing codes and lows as they are left outputs of 131072
+//     tokens off by 0.8 %, from the tensor cores' rounding of the large sums alone.)
+//     P is two fp16 terms, P scale one, rounded once from both: the one rounding of
+//     a token's weight, like P's in fp16 attention.
 //   * q of a head is scaled by the power of two that brings its largest value into
 //     [2^7, 2^8), so that fp16 holds every bit that matters of an fp16 or bf16 q.
 #include <algorithm>
@@ -68,7 +75,10 @@ struct Kv4Cfg {
   // 131072, 8 kv heads, d 128): 16 warps of 32 tokens 91.0 / 241.6, 12 of 48
   // 89.1 / 241.2, 8 of 64 97.4 / 268.9, 20 of 32 (registers spill) 102 / 265; one
   // sequence of 700 tokens 9.5, 8.4, 8.7.
-  static constexpr int TOK = D == 64 ? 64 : 48;
+#ifndef FAB_T
+#define FAB_T 48
+#endif
+  static constexpr int TOK = D == 64 ? 64 : FAB_T;
   static constexpr int MT = TOK / 16;   // 16-token tiles of a stage
   static constexpr int KV = TOK * ROW;  // K (or V) bytes of one stage
   static constexpr int STAGE = 2 * KV;
@@ -78,7 +88,8 @@ struct Kv4Cfg {
   static constexpr int META_OFF = (BAR_OFF + W * STAGES * 8 + 15) / 16 * 16;
   static constexpr int PREFIX_OFF = META_OFF + W * STAGES * 16;
   static constexpr int CTX_OFF = PREFIX_OFF + (kLaunchBatch + 1) * 4;
-  static constexpr int SMEM = (CTX_OFF + kLaunchBatch * 4 + 15) / 16 * 16 + 16;  // + the abort flag
+  static constexpr int CENTRE_OFF = (CTX_OFF + kLaunchBatch * 4 + 15) / 16 * 16;
+  static constexpr int SMEM = CENTRE_OFF + 32 + 16;  // + the abort flag
   static_assert(STAGE % 16 == 0 && KV % 16 == 0 && BAR_OFF % 16 == 0, "bulk copy alignment");
   static_assert(SMEM <= 227 * 1024, "shared memory per CTA");
 };
@@ -141,6 +152,18 @@ __device__ __forceinline__ uint32_t hmul2(uint32_t a, uint32_t b) {
   return *reinterpret_cast<const uint32_t*>(&r);
 }
 
+__device__ __forceinline__ uint32_t hfma2(uint32_t a, uint32_t b, uint32_t c) {
+  const __half2 r = __hfma2(*reinterpret_cast<__half2*>(&a), *reinterpret_cast<__half2*>(&b),
+                            *reinterpret_cast<__half2*>(&c));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+
+// Pairs of fp16: 8 and 7; and what centres an even and an odd row of V (8 and 7 codes
+// below, so that the middle of the codes is 0 on average), in the codes' unit 2^-24
+// and times 16.
+constexpr uint32_t kEight = 0x48004800u, kSeven = 0x47004700u;
+constexpr uint32_t kCentre = 0x80078008u, kCentre16 = 0x80708080u;
+
 // N 32-bit words (1, 2 or 4) of shared memory in one load.
 template <int N>
 __device__ __forceinline__ void load_words(uint32_t (&r)[N], const uint8_t* p) {
@@ -184,6 +207,9 @@ __global__ void __launch_bounds__(Kv4Cfg<D>::THREADS, 1) kv4_decode_kernel(const
     ctx_s[b] = min(max(p.ctx[b], 0), p.max_ctx);
   if (threadIdx.x < C::W * C::STAGES)
     mbar_init(reinterpret_cast<uint64_t*>(smem + C::BAR_OFF) + threadIdx.x, 1);
+  if (threadIdx.x < 8)
+    reinterpret_cast<uint32_t*>(smem + C::CENTRE_OFF)[threadIdx.x] =
+        threadIdx.x < 4 ? kCentre : kCentre16;
   if (threadIdx.x == 0) {
     *abort_flag = 0;
     fence_mbar_init();
@@ -226,15 +252,32 @@ __global__ void __launch_bounds__(Kv4Cfg<D>::THREADS, 1) kv4_decode_kernel(const
   int pb = 0, pkvh = 0, pst = 0, pnst = 0;  // the next stage: sequence, kv head, stage of that row
   int ppg = 0, poff = 0;                    // page of the row and token in it where it begins
   bool pfirst = true, pwhole = true;        // it is this warp's first of the row; from the row's first
-  // Block-table entries [bt_base, bt_base + 32) and the next 32, one per lane:
-  // the second window is on its way while the first is used.
-  int bt_base = 0, bt_cur = 0, bt_next = 0;
-  const uint8_t *pk = nullptr, *pv = nullptr;  // the row's kv head in page 0
+  // K rows of the kv head in pages [bt_base, bt_base + 32) of the sequence, one page per
+  // lane, and the block-table entries of the next 32, which are on their way meanwhile.
+  int bt_base = 0, bt_next = 0;
+  unsigned long long bt_rows = 0;
+  const unsigned long long v_less_k =
+      reinterpret_cast<unsigned long long>(p.vc) - reinterpret_cast<unsigned long long>(p.kc);
+  bool fresh = false;  // the row's first window is still to be taken
   unsigned int p_slot = 0, c_slot = 0, c_parity = 0, ahead = 0;
   const bool leader = elect_one();
 
   auto table = [&](int pg) {
     return pg < p.max_blocks ? p.bt[static_cast<size_t>(pb) * p.max_blocks + pg] : 0;
+  };
+  // Takes the entries of bt_next, those of pages bt_base + lane, and asks for the next.
+  auto window = [&]() {
+    unsigned int page = static_cast<unsigned int>(bt_next);
+    if (page >= static_cast<unsigned int>(p.num_blocks)) {  // never read outside the cache
+      // An entry past the sequence's last page is not looked at.
+      if ((bt_base + lane) * static_cast<long long>(p.bs) < ctx_s[pb])
+        report_status(p.status, 2u /* ATTN_DEVICE_BAD_BLOCK */, kSiteKv4Block);
+      page = 0;
+    }
+    bt_rows = reinterpret_cast<unsigned long long>(p.kc) +
+              static_cast<unsigned long long>(page) * p.block_stride +
+              static_cast<unsigned long long>(pkvh) * p.bs * ROW;
+    bt_next = table(bt_base + 32 + lane);
   };
   auto open_row = [&]() {
     pfirst = true;
@@ -242,10 +285,8 @@ __global__ void __launch_bounds__(Kv4Cfg<D>::THREADS, 1) kv4_decode_kernel(const
     ppg = pst * kTok / p.bs;
     poff = pst * kTok - ppg * p.bs;
     bt_base = ppg;
-    bt_cur = table(bt_base + lane);
-    bt_next = table(bt_base + 32 + lane);
-    pk = p.kc + static_cast<long long>(pkvh) * p.bs * ROW;
-    pv = p.vc + static_cast<long long>(pkvh) * p.bs * ROW;
+    bt_next = table(bt_base + lane);
+    fresh = true;
   };
 
   if (left > 0) {
@@ -264,7 +305,8 @@ __global__ void __launch_bounds__(Kv4Cfg<D>::THREADS, 1) kv4_decode_kernel(const
 
   // Issue the copies of the producer's next stage into its ring slot, page by page
   // from one elected lane, with operands that are the same in all lanes. (With a
-  // page per lane the compiler puts a loop over the lanes around each copy.)
+  // page per lane the compiler puts a loop over the lanes around each copy.) Addresses
+  // come 32 pages at a time, one per lane, and are handed out by shuffles.
   auto produce = [&]() {
     if (left == 0) return;
     uint8_t* dst = ring + p_slot * C::STAGE;
@@ -281,26 +323,21 @@ __global__ void __launch_bounds__(Kv4Cfg<D>::THREADS, 1) kv4_decode_kernel(const
                                nt | (pfirst ? kFirst : 0) | (row_end || left == 1 ? kLast : 0) |
                                    (row_end && pwhole ? kWhole : 0));
     }
-    if (ppg - bt_base >= 32) {
-      bt_base += 32;
-      bt_cur = bt_next;
-      bt_next = table(bt_base + 32 + lane);
+    if (fresh) {
+      window();
+      fresh = false;
     }
     do {
-      const int rel = ppg - bt_base;  // below 64
-      int page = __shfl_sync(0xffffffffu, rel < 32 ? bt_cur : bt_next, rel & 31);
-      if (static_cast<unsigned int>(page) >= static_cast<unsigned int>(p.num_blocks)) {
-        // Never read outside the cache.
-        if (leader) report_status(p.status, 2u /* ATTN_DEVICE_BAD_BLOCK */, kSiteKv4Block);
-        page = 0;
+      if (ppg - bt_base >= 32) {
+        bt_base += 32;
+        window();
       }
+      const unsigned long long src = __shfl_sync(0xffffffffu, bt_rows, ppg - bt_base) +
+                                     static_cast<unsigned int>(poff * ROW);
       const int rows = min(p.bs - poff, todo);
-      const unsigned long long src =
-          static_cast<unsigned long long>(static_cast<unsigned int>(page)) * p.block_stride +
-          static_cast<unsigned int>(poff * ROW);
       if (leader) {
-        bulk_g2s(dst, pk + src, rows * ROW, bar);
-        bulk_g2s(dst + C::KV, pv + src, rows * ROW, bar);
+        bulk_g2s(dst, reinterpret_cast<const void*>(src), rows * ROW, bar);
+        bulk_g2s(dst + C::KV, reinterpret_cast<const void*>(src + v_less_k), rows * ROW, bar);
       }
       dst += rows * ROW;
       todo -= rows;
@@ -343,6 +380,12 @@ __global__ void __launch_bounds__(Kv4Cfg<D>::THREADS, 1) kv4_decode_kernel(const
   float* sc = nullptr;  // SCORED: the scores of the stage's first token
   const int tok_k = (g4 & 1) ? ((g4 + 3) & 7) + 8 : g4;  // tau(g4)
   const int tok_v = ((2 * t4 + 4) & 7) + 8;              // tau(2 t4 + 1)
+
+  // The centring operands, by way of shared memory: operands that the compiler knows to
+  // be constant it writes out, four moves, before each of their products.
+  uint32_t ca[4], cb[4];
+  load_words<4>(ca, smem + C::CENTRE_OFF);
+  load_words<4>(cb, smem + C::CENTRE_OFF + 16);
 
   auto load_q = [&](int b, int kvh) {
     const bool real = g4 < p.group;
@@ -511,7 +554,9 @@ __global__ void __launch_bounds__(Kv4Cfg<D>::THREADS, 1) kv4_decode_kernel(const
       m[h] = mx;
       shift[h] = 2.f - mx;
     }
-    uint32_t pf[MT][2];  // P^T as B fragments: tokens of rows 2 t4, 2 t4 + 1 (+ 8), head g4
+    // P^T as B fragments: tokens of rows 2 t4, 2 t4 + 1 (+ 8), head g4; and what rounding
+    // it to fp16 left over.
+    uint32_t pf[MT][2], pl[MT][2];
     uint64_t add = f2_pack(0.f, 0.f);
     const uint64_t sh = f2_pack(shift[0], shift[1]);
 #pragma unroll
@@ -523,7 +568,12 @@ __global__ void __launch_bounds__(Kv4Cfg<D>::THREADS, 1) kv4_decode_kernel(const
         e0 = fast_exp2(e0);
         e1 = fast_exp2(e1);
         add = f2_add(add, f2_pack(e0, e1));
-        pf[i][c] = transpose8(pack_half2(e0, e1));
+        const uint32_t hi = pack_half2(e0, e1);
+        const float2 back = __half22float2(*reinterpret_cast<const __half2*>(&hi));
+        float r0, r1;
+        f2_unpack(f2_fma(f2_pack(back.x, back.y), f2_pack(-1.f, -1.f), f2_pack(e0, e1)), r0, r1);
+        pf[i][c] = transpose8(hi);
+        pl[i][c] = transpose8(pack_half2(r0, r1));
       }
     }
     float add0, add1;
@@ -556,21 +606,35 @@ __global__ void __launch_bounds__(Kv4Cfg<D>::THREADS, 1) kv4_decode_kernel(const
       load_words<NG>(sb, rb + CODES);
       load_words<NG>(sc2, ra + ROW + CODES);
       load_words<NG>(sd, rb + ROW + CODES);
-      // P . low: row g4 has the lows of group g4 % 2, row g4 + 8 those of group
-      // 2 + g4 % 2.
+      // P . (low + c scale): row g4 has the middles of group g4 % 2, row g4 + 8 those
+      // of group 2 + g4 % 2.
       const uint32_t pick = (g4 & 1) ? 0x7632u : 0x5410u;
       constexpr int L = NG / 2;
-      mma_k16(z, __byte_perm(sa[L], sb[L], pick), __byte_perm(sa[NG - 1], sb[NG - 1], pick),
-              __byte_perm(sc2[L], sd[L], pick), __byte_perm(sc2[NG - 1], sd[NG - 1], pick),
-              pf[i][0], pf[i][1]);
+      uint32_t ma[2], mb[2], mc[2], md2[2];
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const int k = j * (L - 1);
+        ma[j] = hfma2(sa[k], kEight, sa[L + k]);
+        mb[j] = hfma2(sb[k], kSeven, sb[L + k]);
+        mc[j] = hfma2(sc2[k], kEight, sc2[L + k]);
+        md2[j] = hfma2(sd[k], kSeven, sd[L + k]);
+      }
+      const uint32_t z0 = __byte_perm(ma[0], mb[0], pick), z1 = __byte_perm(ma[1], mb[1], pick);
+      const uint32_t z2 = __byte_perm(mc[0], md2[0], pick), z3 = __byte_perm(mc[1], md2[1], pick);
+      mma_k16(z, z0, z1, z2, z3, pf[i][0], pf[i][1]);
+      mma_k16(z, z0, z1, z2, z3, pl[i][0], pl[i][1]);
 #pragma unroll
       for (int w = 0; w < NG; ++w) {
         const uint32_t half = w % 2 == 0 ? 0x5410u : 0x7632u;
-        const uint32_t b0 = hmul2(pf[i][0], __byte_perm(sa[w / 2], sb[w / 2], half));
-        const uint32_t b1 = hmul2(pf[i][1], __byte_perm(sc2[w / 2], sd[w / 2], half));
+        const uint32_t s0 = __byte_perm(sa[w / 2], sb[w / 2], half);
+        const uint32_t s1 = __byte_perm(sc2[w / 2], sd[w / 2], half);
+        const uint32_t b0 = hfma2(pf[i][0], s0, hmul2(pl[i][0], s0));
+        const uint32_t b1 = hfma2(pf[i][1], s1, hmul2(pl[i][1], s1));
         const uint32_t x = __byte_perm(va[w / 2], vb[w / 2], half);
         const uint32_t y = __byte_perm(vc[w / 2], vd[w / 2], half);
         const uint32_t x8 = x >> 8, y8 = y >> 8;
+        mma_k16(acc[w][0], ca[0], ca[1], ca[2], ca[3], b0, b1);
+        mma_k16(acc[w][1], cb[0], cb[1], cb[2], cb[3], b0, b1);
         mma_k16(acc[w][0], x & 0x000F000Fu, x8 & 0x000F000Fu, y & 0x000F000Fu, y8 & 0x000F000Fu,
                 b0, b1);
         mma_k16(acc[w][1], x & 0x00F000F0u, x8 & 0x00F000F0u, y & 0x00F000F0u, y8 & 0x00F000F0u,

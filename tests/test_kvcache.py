@@ -1,15 +1,18 @@
 """The 4-bit paged cache and eviction on the GPU against oracle/kvcache.py (64 bits).
 
 Tolerances of the decode tests are bounds, computed per output from the exact
-values. With u = 2^-11 (half an fp16 step, relative) and p a token's weight:
+values. With u = 2^-11 (half an fp16 step, relative), p a token's weight and
+mid = low + 8 scale:
 
-    P is rounded to fp16, and P * scale again:      2 u sum p scale code + u sum p |low|
-    both below fp16's normal range (P <= 4, l >= 1): N 2^-25 (15 + 15 scale + |low|) / (4 L)
-    fp32 sums over the N tokens, 16 at a time:       (N / 16 + 8) 2^-23 sum p (scale code + |low|)
+    P * scale is rounded to fp16, and so is mid:  u sum p scale |code - 8| + u sum p |mid|
+    P (two fp16 terms, at most 4, l >= 1), its second term times scale, and P * scale,
+    each below fp16's normal range:               N 2^-25 (15 scale + |mid| + 16) / (4 L)
+    fp32 sums over the N tokens, two products of 16 at a time:
+                                                  (N / 8 + 8) 2^-23 sum p (15 scale + |low|)
     the score's fp32 sum of D products, in units of the exponent:
         d = (D + 32) 2^-24 scale_qk sum |q| (15 scale + |low|) + 2^-22 |s|
       moves p by 2 d + 2^-21 relative (exponential and normaliser)
-    the output's own rounding:                       finfo(dtype).eps / 2 |o| + 2^-25
+    the output's own rounding:                    finfo(dtype).eps / 2 |o| + 2^-25
 
 (L = sum 2^(s - max s); terms that multiply each other are covered by a factor 1.1.)
 A total of weights moves by (2 d + 2^-21) p, the sum over the group and the add.
@@ -85,10 +88,11 @@ def check_decode4(lens, hq, hkv, d, bs, dtype=torch.float16, seed=0, spread=1.0,
             delta = ((d + 32) * 2.0 ** -24 * sc * (qd.abs() @ (15 * kscale + klow.abs()).T)
                      + 2.0 ** -22 * s.abs()).amax(-1, keepdim=True)
             big_l = torch.exp(s - s.amax(-1, keepdim=True)).sum(-1, keepdim=True)
-            mass = p @ (vscale * vcode + vlow.abs())
-            tol = 2 * u * (p @ (vscale * vcode)) + u * (p @ vlow.abs())
-            tol += n * 2.0 ** -25 * (15 + 15 * vscale.max() + vlow.abs().max()) / (4 * big_l)
-            tol += (n / 16 + 8) * 2.0 ** -23 * mass + (2 * delta + 2.0 ** -21) * 2 * mass
+            mid = vlow + 8 * vscale
+            mass = p @ (15 * vscale + vlow.abs())
+            tol = u * (p @ (vscale * (vcode - 8).abs())) + u * (p @ mid.abs())
+            tol += n * 2.0 ** -25 * (15 * vscale.max() + mid.abs().max() + 16) / (4 * big_l)
+            tol += (n / 8 + 8) * 2.0 ** -23 * mass + (2 * delta + 2.0 ** -21) * 2 * mass
             tol = 1.1 * tol + torch.finfo(dtype).eps / 2 * o.abs() + 2.0 ** -25
             bad = (out[b, heads] - o).abs() > tol
             assert not bad.any(), (b, h, (out[b, heads] - o).abs().max(), tol.min())
@@ -306,6 +310,26 @@ def test_decode4_many_sequences():
         got = out[b].double()
         assert torch.equal(got.isnan(), o.isnan()), b
         assert ((got - o).abs() < 1e-2)[~o.isnan()].all(), b
+
+
+@pytest.mark.parametrize("d,bs", [(128, 1), (128, 3), (64, 2), (64, 6), (128, 40)])
+def test_decode4_long_runs_of_small_pages(d, bs):
+    """Several stages of a row per warp, each of more pages than a window of the block table
+    holds in part, so that windows end inside stages."""
+    torch.manual_seed(d + bs)
+    n, length = 900, 397
+    pool = 3 * (64 // bs + 2)
+    kc, vc = (ora.pack(torch.randn(pool, 1, bs, d).half(), v) for v in (False, True))
+    bt = torch.randint(0, pool, (n, -(-length // bs)), dtype=torch.int32)
+    lens = torch.full((n,), length, dtype=torch.int32)
+    q = torch.randn(n, 3, d).half()
+    out = ak.paged_decode_kv4(q.cuda(), kc.cuda(), vc.cuda(), bt.cuda(), lens.cuda(), length).cpu()
+    for b in range(0, n, 41):
+        o, _ = ora.attend(q[b], ora.unpack(ora.rows_of(kc, bt[b], length, 0), False),
+                          ora.unpack(ora.rows_of(vc, bt[b], length, 0), True))
+        # The module's bound for values of a few units.
+        assert (out[b].double() - o).abs().max() < 4e-3, b
+    ak.check_device_status()
 
 
 def test_decode4_cuts_lengths_above_max():
