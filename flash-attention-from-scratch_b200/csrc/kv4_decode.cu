@@ -57,32 +57,23 @@ constexpr int kLaunchBatch = 2048;  // sequences per launch (their lengths live 
 // row for this warp, and, with the last, the row lies wholly in this warp's run.
 enum : int { kTokens = 127, kFirst = 128, kLast = 256, kWhole = 512 };
 
-#ifndef FAB_KV4_W
-#define FAB_KV4_W 12
-#endif
-#ifndef FAB_KV4_S
-#define FAB_KV4_S 2
-#endif
-
 template <int D>
 struct Kv4Cfg {
   using R = Kv4Row<D>;
-  static constexpr int W = FAB_KV4_W;  // warps per CTA, one CTA per SM
+  // Warps per CTA (one CTA per SM) and tokens per stage. Measured at head_dim 128 (us,
+  // 64 ragged sequences of up to 8192 tokens / 8 of 131072, 8 kv heads; one of 700):
+  // 12 warps of 48 tokens 100 / 267, 8.9; 16 of 32 (128 registers, some spilled) 100 /
+  // 268, 10.2; 8 of 64 106 / 292, 9.0. At 64 (64 x 8192, 64 query over 8 kv heads): 16
+  // warps of 64 tokens 66, 12 70, 8 78.
+  static constexpr int W = D == 64 ? 16 : 12;
   static constexpr int THREADS = W * 32;
   static constexpr int NG = R::NG;
   static constexpr int ROW = R::BYTES;
-  // Tokens per stage. Measured (us, 64 ragged sequences of up to 8192 tokens / 8 of
-  // 131072, 8 kv heads, d 128): 16 warps of 32 tokens 91.0 / 241.6, 12 of 48
-  // 89.1 / 241.2, 8 of 64 97.4 / 268.9, 20 of 32 (registers spill) 102 / 265; one
-  // sequence of 700 tokens 9.5, 8.4, 8.7.
-#ifndef FAB_T
-#define FAB_T 48
-#endif
-  static constexpr int TOK = D == 64 ? 64 : FAB_T;
+  static constexpr int TOK = D == 64 ? 64 : 48;
   static constexpr int MT = TOK / 16;   // 16-token tiles of a stage
   static constexpr int KV = TOK * ROW;  // K (or V) bytes of one stage
   static constexpr int STAGE = 2 * KV;
-  static constexpr int STAGES = FAB_KV4_S;
+  static constexpr int STAGES = 2;
   static constexpr int RING = STAGES * STAGE;
   static constexpr int BAR_OFF = W * RING;
   static constexpr int META_OFF = (BAR_OFF + W * STAGES * 8 + 15) / 16 * 16;
