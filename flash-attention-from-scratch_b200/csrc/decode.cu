@@ -895,12 +895,9 @@ template <int D, int G, bool SCORED>
 cudaError_t launch_decode_kernel(const DecParams& prm, int64_t upper_units, const LaunchCtx& ctx) {
   using C = DecCfg<D, G>;
   auto kern = paged_decode_kernel<D, G, SCORED>;
-  static std::once_flag once;
-  static cudaError_t attr_err = cudaSuccess;
-  std::call_once(once, [&] {
-    attr_err = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
-  });
-  if (attr_err != cudaSuccess) return attr_err;
+  static SmemLimit limit;
+  cudaError_t e = allow_smem(kern, C::SMEM, limit);
+  if (e != cudaSuccess) return e;
   // One CTA per SM, or one per unit when there are fewer units than SMs.
   const int grid = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(ctx.sm_count, upper_units)));
   kern<<<grid, C::THREADS, C::SMEM, ctx.stream>>>(prm);

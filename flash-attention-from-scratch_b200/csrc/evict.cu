@@ -3,7 +3,6 @@
 // totals of the rest, ties to the lower index), then their rows moved, in order,
 // into the sequence's new pages.
 #include <algorithm>
-#include <mutex>
 
 #include <cooperative_groups.h>
 
@@ -337,22 +336,9 @@ cudaError_t launch_select(const SelectParams& s, unsigned pairs, int ranks, cons
   // Room for a share rounded up to whole runs of 128 keys per warp.
   const int64_t share = (static_cast<int64_t>(s.max_ctx) + ranks - 1) / ranks;
   const int64_t keys = HELD ? (share + 4 * T - 1) / (4 * T) * (4 * T) : 0;
-  // Per device: a function's attributes belong to the device that is current.
-  static std::mutex mu;
-  static bool done[64] = {};
-  int dev = 0;
-  cudaError_t e = cudaGetDevice(&dev);
+  static SmemLimit limit;
+  cudaError_t e = allow_smem(evict_select_kernel<T, HELD>, kMaxKeys * 4, limit);
   if (e != cudaSuccess) return e;
-  if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
-  {
-    std::lock_guard<std::mutex> lock(mu);
-    if (!done[dev]) {
-      e = cudaFuncSetAttribute(evict_select_kernel<T, HELD>,
-                               cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxKeys * 4);
-      if (e != cudaSuccess) return e;
-      done[dev] = true;
-    }
-  }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(pairs * static_cast<unsigned>(ranks));
   cfg.blockDim = dim3(T);

@@ -41,7 +41,6 @@
 //   * q of a head is scaled by the power of two that brings its largest value into
 //     [2^7, 2^8), so that fp16 holds every bit that matters of an fp16 or bf16 q.
 #include <algorithm>
-#include <mutex>
 
 #include "kv4.cuh"
 #include "launch.h"
@@ -728,21 +727,9 @@ template <int D, typename T, bool SCORED>
 cudaError_t launch_kernel(const Kv4DecParams& p, int grid, const LaunchCtx& ctx) {
   using C = Kv4Cfg<D>;
   auto kern = kv4_decode_kernel<D, T, SCORED>;
-  // Per device: a function's attributes belong to the device that is current.
-  static std::mutex mu;
-  static bool done[64] = {};
-  int dev = 0;
-  cudaError_t e = cudaGetDevice(&dev);
+  static SmemLimit limit;
+  cudaError_t e = allow_smem(kern, C::SMEM, limit);
   if (e != cudaSuccess) return e;
-  if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
-  {
-    std::lock_guard<std::mutex> lock(mu);
-    if (!done[dev]) {
-      e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
-      if (e != cudaSuccess) return e;
-      done[dev] = true;
-    }
-  }
   kern<<<grid, C::THREADS, C::SMEM, ctx.stream>>>(p);
   return cudaGetLastError();
 }

@@ -5,6 +5,7 @@
 
 #include <cstddef>
 #include <cstdint>
+#include <mutex>
 #include <string>
 
 #include <cuda_runtime.h>
@@ -19,6 +20,26 @@ struct LaunchCtx {
   unsigned long long timeout_ns; // limit of every bounded wait
   int sm_count;                  // SMs of the current device
 };
+
+// Allow a kernel `bytes` of dynamic shared memory on the current device, once per
+// device (a function's attributes belong to the device that is current). `done` is
+// the kernel's own, static.
+struct SmemLimit {
+  std::mutex mu;
+  bool done[64] = {};
+};
+template <typename Kernel>
+cudaError_t allow_smem(Kernel kernel, int bytes, SmemLimit& limit) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
+  std::lock_guard<std::mutex> lock(limit.mu);
+  if (limit.done[dev]) return cudaSuccess;
+  e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  limit.done[dev] = e == cudaSuccess;
+  return e;
+}
 
 // tcgen05 FlashAttention forward; q, k, v, o fp16 [bh, n, d], d in {64, 128}.
 cudaError_t launch_flash_tc(const void* q, const void* k, const void* v, void* o, int64_t bh,

@@ -696,3 +696,117 @@ def test_append_and_evict_in_a_graph():
     rk, _ = ak.paged_read_kv4(kc, vc, slot)
     assert ((rk.cpu().double() - ora.unpack(ora.pack(k.cpu(), False), False)).abs() < 4e-3).all()
     assert set(range(7 * 16, 8 * 16)) <= set(kept[0, 0].tolist())
+
+
+# ----------------------------------------------------------------- hard corners
+
+def test_negative_lengths_and_unused_table_entries():
+    """A negative length is an empty sequence; table entries past a sequence's pages may hold
+    anything and are not reported."""
+    kc, vc, bt = cache4([100, 40], 2, 128, 16)
+    bt = torch.cat([bt, torch.full((2, 40), -7, dtype=torch.int32)], 1)
+    bt[1, 3:] = 1 << 30
+    q = torch.randn(2, 4, 128).half().cuda()
+    w = torch.rand(kc.shape[:3], device="cuda")
+    args = (kc.cuda(), vc.cuda(), bt.cuda())
+    lens = torch.tensor([100, 40]).cuda()
+    want = ak.paged_decode_kv4(q, *args, lens, 500, weights=w)
+    assert want.isfinite().all()
+    out = ak.paged_decode_kv4(q, *args, torch.tensor([100, -5]).cuda(), 500)
+    assert (out[1] == 0).all()
+    f16 = torch.randn(2, kc.shape[0], 2, 16, 128, device="cuda").half()
+    out = ak.paged_decode_weights(q, f16[0], f16[1], args[2], torch.tensor([100, -5]).cuda(), 500, w)
+    assert (out[1] == 0).all() and out[0].isfinite().all()
+    new = torch.zeros(2, 40, dtype=torch.int32).cuda()
+    new_lens, kept = ak.paged_evict((f16[0],), w, args[2], torch.tensor([-5, 0]).cuda(), 500, new, 600)
+    assert new_lens.tolist() == [0, 0] and (kept == -1).all()
+    ak.check_device_status()
+
+
+def test_caches_beyond_4_gib():
+    """Pages whose byte offsets pass 32 bits, in every operator."""
+    hkv, bs, d = 8, 16, 128
+    blocks = (1 << 32) // (hkv * bs * 80) + 500
+    kc, vc = (torch.empty(blocks, hkv, bs, 80, dtype=torch.uint8, device="cuda") for _ in range(2))
+    assert kc.numel() > 1 << 32
+    w = torch.empty(blocks, hkv, bs, device="cuda")
+    pages = torch.arange(blocks - 1, blocks - 41, -1, dtype=torch.int32, device="cuda").view(2, 20)
+    n = 150
+    slots = (pages.long()[:, :, None] * bs + torch.arange(bs, device="cuda")).flatten(1)[:, :n]
+    k, v = (torch.randn(2 * n, hkv, d).half() for _ in range(2))
+    ak.paged_append_kv4(k.cuda(), v.cuda(), kc, vc, slots.flatten(), weights=w)
+    assert (w.view(blocks, hkv, bs)[slots.flatten() // bs, :, slots.flatten() % bs] == 0).all()
+    rk, rv = ak.paged_read_kv4(kc, vc, slots.flatten())
+    for got, x, value in ((rk, k, False), (rv, v, True)):
+        exact = ora.unpack(ora.pack(x, value), value)
+        assert ((got.cpu().double() - exact).abs() <= 2.0 ** -10 * exact.abs() + 2.0 ** -24).all()
+    q = torch.randn(2, 2 * hkv, d).half()
+    lens = torch.tensor([n, n - 3], dtype=torch.int32, device="cuda")
+    out = ak.paged_decode_kv4(q.cuda(), kc, vc, pages, lens, n, weights=w).cpu().double()
+    kd, vd = (ora.unpack(ora.pack(x, i == 1), i == 1).view(2, n, hkv, d) for i, x in enumerate((k, v)))
+    for b in range(2):
+        for h in range(hkv):
+            m = int(lens[b])
+            o, p = ora.attend(q[b, 2 * h:2 * h + 2], kd[b, :m, h], vd[b, :m, h])
+            assert (out[b, 2 * h:2 * h + 2] - o).abs().max() < 4e-3
+            got = w[slots[b] // bs, h, slots[b] % bs][:m].cpu().double()
+            assert (got - p.sum(0)).abs().max() < 1e-5
+    new = torch.tensor([[blocks - 60], [blocks - 70]], dtype=torch.int32, device="cuda")
+    src = kc[pages[0, 0].item(), 3, 2].clone()
+    w[pages[0, 0].item(), 3, 2] = 9.0
+    new_lens, kept = ak.paged_evict((kc, vc), w, pages, lens, n, new, 16, recent=4)
+    at = kept[0, 3].tolist().index(2)
+    assert torch.equal(kc[blocks - 60, 3, at], src) and w[blocks - 60, 3, at] == 9.0
+    ak.check_device_status()
+
+
+def test_fp16_weights_cache_beyond_4_gib():
+    hkv, bs, d = 8, 16, 128
+    blocks = (1 << 32) // (hkv * bs * d * 2) + 50
+    kc, vc = (torch.empty(blocks, hkv, bs, d, dtype=torch.float16, device="cuda") for _ in range(2))
+    pages = torch.arange(blocks - 1, blocks - 7, -1, dtype=torch.int32, device="cuda")[None]
+    kc[pages[0].long()] = torch.randn(6, hkv, bs, d).half().cuda()
+    vc[pages[0].long()] = torch.randn(6, hkv, bs, d).half().cuda()
+    w = torch.zeros(blocks, hkv, bs, device="cuda")
+    q = torch.randn(1, hkv, d).half().cuda()
+    lens = torch.tensor([90], dtype=torch.int32, device="cuda")
+    out = ak.paged_decode_weights(q, kc, vc, pages, lens, 90, w)
+    sub = [c[pages[0].long()].contiguous() for c in (kc, vc)]
+    ws = torch.zeros(6, hkv, bs, device="cuda")
+    small = ak.paged_decode_weights(q, *sub, torch.arange(6, dtype=torch.int32, device="cuda")[None],
+                                    lens, 90, ws)
+    assert torch.equal(out, small) and torch.equal(w[pages[0].long()], ws)
+
+
+def test_repeated_calls_give_the_same_bits():
+    """The split goes by sizes alone, and a total with one adder has one order: bit for bit."""
+    lens = [900, 33, 512]
+    kc, vc, bt = [t.cuda() for t in cache4(lens, 4, 128, 16)]
+    f16 = torch.randn(2, kc.shape[0], 4, 16, 128, device="cuda").half()
+    q = torch.randn(3, 16, 128).half().cuda()
+    lt = torch.tensor(lens).cuda()
+    first = None
+    for _ in range(5):
+        w4, w16 = (torch.zeros(kc.shape[:3], device="cuda") for _ in range(2))
+        got = (ak.paged_decode_kv4(q, kc, vc, bt, lt, 900, weights=w4), w4,
+               ak.paged_decode_weights(q, f16[0], f16[1], bt, lt, 900, w16), w16)
+        if first is None:
+            first = got
+        assert all(torch.equal(a, b) for a, b in zip(first, got))
+
+
+def test_tensors_made_on_another_stream():
+    """Inputs produced on a side stream that the call's stream has waited for."""
+    side = torch.cuda.Stream()
+    kc, vc, bt = cache4([200], 2, 64, 16)
+    with torch.cuda.stream(side):
+        q = torch.randn(1, 4, 64, device="cuda").half()
+        args = [t.cuda(non_blocking=True) for t in (kc, vc, bt)] + \
+            [torch.tensor([200], device="cuda"), 200]
+    torch.cuda.current_stream().wait_stream(side)
+    here = ak.paged_decode_kv4(q, *args)
+    with torch.cuda.stream(side):
+        side.wait_stream(torch.cuda.current_stream())
+        there = ak.paged_decode_kv4(q, *args)
+    torch.cuda.synchronize()
+    assert torch.equal(here, there)
