@@ -43,6 +43,17 @@ __device__ __forceinline__ uint32_t key_of(float w) {
   return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
 }
 
+// Sum of v over the lanes before this one.
+__device__ __forceinline__ int before_of(int v, int lane) {
+  int incl = v;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int y = __shfl_up_sync(0xffffffffu, incl, o);
+    if (lane >= o) incl += y;
+  }
+  return incl - v;
+}
+
 // One cluster per (sequence, kv head); CTA r of it has the r-th share of the
 // candidates. The need-th largest key comes by a radix select, 11, 11 and 10 bits
 // at a time: every CTA counts its keys, adds up the cluster's counts and finds the
@@ -59,7 +70,7 @@ __global__ void __launch_bounds__(T) evict_select_kernel(const SelectParams p) {
   namespace cg = cooperative_groups;
   extern __shared__ __align__(16) uint32_t keys[];
   __shared__ int hist[2][kBins];
-  __shared__ int warp_sum_s[T / 32];
+  __shared__ int coarse[2][kBins / 32];
   __shared__ int warp_gt[T / 32], warp_eq[T / 32];
   __shared__ int share_gt, share_eq;
   __shared__ uint32_t s_digit;
@@ -158,41 +169,45 @@ __global__ void __launch_bounds__(T) evict_select_kernel(const SelectParams p) {
       if (k.z != 0u && (k.z & mask) == prefix) atomicAdd(&h[(k.z >> shift) & digits], 1);
       if (k.w != 0u && (k.w & mask) == prefix) atomicAdd(&h[(k.w >> shift) & digits], 1);
     }
+    __syncthreads();
+    // Sums of 32 bins each. The cluster's counts are looked up in two steps, of these
+    // sums and then of the 32 bins in question: reading all bins of the other CTAs
+    // took 9500 cycles a pass, half of the kernel.
+#pragma unroll 1
+    for (int c = warp; c < kBins / 32; c += T / 32) {
+      const int sum = __reduce_add_sync(0xffffffffu, h[32 * c + lane]);
+      if (lane == 0) coarse[pass & 1][c] = sum;
+    }
     cluster.sync();
-    // Bins from the top, kBins / T a thread: the cluster's counts, and the bin where
-    // the running count reaches `left`.
-    constexpr int B = kBins / T;
-    int c[B], sum = 0;
-#pragma unroll
-    for (int j = 0; j < B; ++j) c[j] = 0;
-#pragma unroll 4
-    for (int r = 0; r < ranks; ++r) {
-      const int* other = cluster.map_shared_rank(h, r);
-#pragma unroll
-      for (int j = 0; j < B; ++j) c[j] += other[kBins - 1 - (tid * B + j)];
-    }
-#pragma unroll
-    for (int j = 0; j < B; ++j) sum += c[j];
-    int incl = sum;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int y = __shfl_up_sync(0xffffffffu, incl, o);
-      if (lane >= o) incl += y;
-    }
-    if (lane == 31) warp_sum_s[warp] = incl;
     // The other buffer is counted into in the next pass; no CTA reads it any more
     // (all have passed the cluster barrier above).
 #pragma unroll 1
     for (int j = tid; j < kBins; j += T) hist[(pass & 1) ^ 1][j] = 0;
-    __syncthreads();
-    int above = incl - sum + __reduce_add_sync(0xffffffffu, lane < warp ? warp_sum_s[lane] : 0);
-#pragma unroll
-    for (int j = 0; j < B; ++j) {
-      if (above < left && left <= above + c[j]) {
-        s_digit = static_cast<uint32_t>(kBins - 1 - (tid * B + j));
-        s_left = left - above;
+    if (warp == 0) {
+      // From the top, the sum and then the bin where the running count reaches `left`.
+      int c0 = 0, c1 = 0, one = 0;
+      const int top = kBins / 32 - 1 - 2 * lane;  // lane's sums: top, top - 1
+#pragma unroll 4
+      for (int r = 0; r < ranks; ++r) {
+        const int* other = cluster.map_shared_rank(&coarse[pass & 1][0], r);
+        c0 += other[top];
+        c1 += other[top - 1];
       }
-      above += c[j];
+      int above = before_of(c0 + c1, lane);
+      const bool first_sum = above < left && left <= above + c0;
+      const bool second_sum = above + c0 < left && left <= above + c0 + c1;
+      const unsigned found = __ballot_sync(0xffffffffu, first_sum || second_sum);
+      const int from = __ffs(found) - 1;
+      const int block = __shfl_sync(0xffffffffu, first_sum ? top : top - 1, from);
+      int rest = __shfl_sync(0xffffffffu, left - above - (first_sum ? 0 : c0), from);
+#pragma unroll 4
+      for (int r = 0; r < ranks; ++r)
+        one += cluster.map_shared_rank(h, r)[32 * block + 31 - lane];
+      above = before_of(one, lane);
+      if (above < rest && rest <= above + one) {
+        s_digit = static_cast<uint32_t>(32 * block + 31 - lane);
+        s_left = rest - above;
+      }
     }
     __syncthreads();
     prefix |= s_digit << shift;
