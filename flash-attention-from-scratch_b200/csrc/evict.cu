@@ -286,6 +286,7 @@ __global__ void __launch_bounds__(T) evict_select_kernel(const SelectParams p) {
 struct MoveParams {
   uint8_t* arrays[kMaxEvictArrays];  // [num_blocks, hkv, bs, row bytes]
   int row_vecs[kMaxEvictArrays];     // row bytes / 16, 8, 4, 2 or 1
+  FastDiv by_row[kMaxEvictArrays];
   int num_arrays;
   float* weights;
   const int* kept;
@@ -294,46 +295,66 @@ struct MoveParams {
   const int* new_bt;
   DeviceStatus* status;
   int hkv, bs, num_blocks, max_blocks, new_max_blocks, keep;
+  FastDiv by_bs;
 };
 
 constexpr int kMoveRows = 64;
 
+// 64 rows of one (sequence, kv head) at a time. Four pieces a thread are read before
+// they are written: a load does not pass a store that could be to the same address.
 template <typename V>
 __global__ void __launch_bounds__(256) evict_move_kernel(const MoveParams p) {
+  constexpr int U = 4;
   __shared__ long long from[kMoveRows], to[kMoveRows];  // row numbers; from < 0: not moved
   const int kvh = blockIdx.x % p.hkv, b = blockIdx.x / p.hkv;
   const int n = p.new_lens[b];
   for (long long j0 = static_cast<long long>(blockIdx.y) * kMoveRows; j0 < n;
        j0 += static_cast<long long>(gridDim.y) * kMoveRows) {
-  __syncthreads();
-  if (threadIdx.x < kMoveRows) {
-    const int j = static_cast<int>(j0) + threadIdx.x;
-    long long f = -1, t = 0;
-    if (j < n) {
-      const int i = p.kept[static_cast<size_t>(blockIdx.x) * p.keep + j];
-      const int src = p.bt[static_cast<size_t>(b) * p.max_blocks + i / p.bs];
-      const int dst = p.new_bt[static_cast<size_t>(b) * p.new_max_blocks + j / p.bs];
-      if (src < 0 || src >= p.num_blocks || dst < 0 || dst >= p.num_blocks) {
-        report_status(p.status, 2u, kSiteMoveBlock);
-      } else {
-        f = (static_cast<long long>(src) * p.hkv + kvh) * p.bs + i % p.bs;
-        t = (static_cast<long long>(dst) * p.hkv + kvh) * p.bs + j % p.bs;
-        if (f == t) f = -1;
+    __syncthreads();
+    if (threadIdx.x < kMoveRows) {
+      const int j = static_cast<int>(j0) + threadIdx.x;
+      long long f = -1, t = 0;
+      if (j < n) {
+        const int i = p.kept[static_cast<size_t>(blockIdx.x) * p.keep + j];
+        const int in = p.by_bs.quotient(i), out = p.by_bs.quotient(j);
+        const int src = p.bt[static_cast<size_t>(b) * p.max_blocks + in];
+        const int dst = p.new_bt[static_cast<size_t>(b) * p.new_max_blocks + out];
+        if (src < 0 || src >= p.num_blocks || dst < 0 || dst >= p.num_blocks) {
+          report_status(p.status, 2u /* ATTN_DEVICE_BAD_BLOCK */, kSiteMoveBlock);
+        } else {
+          f = (static_cast<long long>(src) * p.hkv + kvh) * p.bs + (i - in * p.bs);
+          t = (static_cast<long long>(dst) * p.hkv + kvh) * p.bs + (j - out * p.bs);
+          if (f == t) f = -1;
+        }
+      }
+      from[threadIdx.x] = f;
+      to[threadIdx.x] = t;
+      if (f >= 0) p.weights[t] = p.weights[f];
+    }
+    __syncthreads();
+    for (int a = 0; a < p.num_arrays; ++a) {
+      const int rv = p.row_vecs[a];
+      V* base = reinterpret_cast<V*>(p.arrays[a]);
+      for (int x0 = threadIdx.x; x0 < kMoveRows * rv; x0 += U * 256) {
+        V v[U];
+        long long at[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          const int x = x0 + u * 256;
+          at[u] = -1;
+          if (x < kMoveRows * rv) {
+            const int r = p.by_row[a].quotient(x), c = x - r * rv;
+            if (from[r] >= 0) {
+              v[u] = base[from[r] * rv + c];
+              at[u] = to[r] * rv + c;
+            }
+          }
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+          if (at[u] >= 0) base[at[u]] = v[u];
       }
     }
-    from[threadIdx.x] = f;
-    to[threadIdx.x] = t;
-    if (f >= 0) p.weights[t] = p.weights[f];
-  }
-  __syncthreads();
-  for (int a = 0; a < p.num_arrays; ++a) {
-    const int rv = p.row_vecs[a];
-    V* base = reinterpret_cast<V*>(p.arrays[a]);
-    for (int x = threadIdx.x; x < kMoveRows * rv; x += 256) {
-      const int r = x / rv, c = x - r * rv;
-      if (from[r] >= 0) base[to[r] * rv + c] = base[from[r] * rv + c];
-    }
-  }
   }
 }
 
@@ -408,7 +429,11 @@ cudaError_t launch_evict(const EvictArgs& a, const LaunchCtx& ctx) {
     while (a.row_bytes[i] % vec != 0 || reinterpret_cast<uintptr_t>(a.arrays[i]) % vec != 0) vec /= 2;
     m.arrays[i] = static_cast<uint8_t*>(a.arrays[i]);
   }
-  for (int i = 0; i < a.num_arrays; ++i) m.row_vecs[i] = static_cast<int>(a.row_bytes[i] / vec);
+  for (int i = 0; i < a.num_arrays; ++i) {
+    m.row_vecs[i] = static_cast<int>(a.row_bytes[i] / vec);
+    m.by_row[i] = FastDiv(m.row_vecs[i]);
+  }
+  m.by_bs = s.by_bs;
   m.num_arrays = a.num_arrays;
   m.weights = a.weights;
   m.kept = a.kept;
