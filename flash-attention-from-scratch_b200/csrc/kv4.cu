@@ -189,9 +189,10 @@ __device__ __forceinline__ void append_row(uint8_t* dst, uint4 raw, bool real, i
 // A lane takes its 8 values of K and of V of one (token, head): the slot and its
 // row in the cache are found once for both. Bound by the instructions it issues (330
 // for the two, half of them the codes): 32768 tokens of 32 heads, d 128, bf16, B200:
-// 209 us for 705 MB (3.4 TB/s); with 64-bit divisions and one tensor per thread 628.
+// 200 us for 705 MB (3.5 TB/s; six CTAs per SM, 209 with five); with 64-bit divisions and
+// one tensor per thread 628.
 template <int D, typename T>
-__global__ void __launch_bounds__(256) kv4_append_kernel(const Kv4CopyParams p) {
+__global__ void __launch_bounds__(256, 6) kv4_append_kernel(const Kv4CopyParams p) {
   using R = Kv4Row<D>;
   constexpr int LPR = D / 8;  // lanes per row
   const int lane_row = threadIdx.x % LPR;
