@@ -132,12 +132,15 @@ def _on(device: torch.device):
     return torch.cuda.device(idx)
 
 
-_SAME_DEVICE = contextlib.nullcontext()
-
-
-def _on_index(idx: int):
-    """_on for a device index."""
-    return _SAME_DEVICE if torch.cuda.current_device() == idx else torch.cuda.device(idx)
+def _call(dev: int, fn, *args) -> None:
+    """A library call with device `dev` current."""
+    if torch.cuda.current_device() == dev:
+        rc = fn(*args)
+    else:
+        with torch.cuda.device(dev):
+            rc = fn(*args)
+    if rc != 0:
+        _check(rc)
 
 
 def _workspace(nbytes: int, device: torch.device) -> torch.Tensor:
@@ -167,6 +170,10 @@ class _StreamWorkspaces:
                     self._bufs[key] = buf
         return buf
 
+    def kept(self, dev: int, stream: int):
+        """The buffer of (device, stream), or None."""
+        return self._bufs.get((dev, stream))
+
     def clear(self) -> None:
         with self._lock:
             self._bufs.clear()
@@ -175,13 +182,16 @@ class _StreamWorkspaces:
 _decode_ws = _StreamWorkspaces()
 
 
-def _call_workspace(nbytes: int, device: torch.device, stream: int) -> torch.Tensor:
+def _call_workspace(nbytes: int, dev: int, stream: int) -> torch.Tensor:
     """The stream's kept scratch, or, while a graph is captured, scratch of the
     capture's own: a graph must not hold an address that a later call may give
     back, nor share it with another graph."""
     if torch.cuda.is_current_stream_capturing():
-        return _workspace(nbytes, device)
-    return _decode_ws.get(nbytes, device, stream)
+        return _workspace(nbytes, torch.device("cuda", dev))
+    buf = _decode_ws.kept(dev, stream)
+    if buf is not None and buf.numel() >= nbytes:
+        return buf
+    return _decode_ws.get(nbytes, torch.device("cuda", dev), stream)
 
 
 @functools.lru_cache(maxsize=4096)
@@ -293,50 +303,41 @@ class Extension:
     def paged_decode_weights(self, dev, q, kc, vc, bt, ctx, weights, sizes, max_ctx, scale,
                              partition):
         out = torch.empty_like(q)
-        lib = self.lib
         B, H, Hkv, D = sizes[:4]
-        with _on_index(dev):
-            stream = _raw_stream(dev)
-            ws = _call_workspace(_workspace_bytes("attn_paged_decode_weights_workspace_bytes", B, H,
-                                                  Hkv, D, max_ctx, partition), q.device, stream)
-            _check(lib.attn_paged_decode_weights(
-                q.data_ptr(), kc.data_ptr(), vc.data_ptr(), bt.data_ptr(), ctx.data_ptr(),
-                out.data_ptr(), weights.data_ptr(), *sizes, max_ctx, scale, partition,
-                ws.data_ptr(), ws.numel(), stream))
+        stream = _raw_stream(dev)
+        ws = _call_workspace(_workspace_bytes("attn_paged_decode_weights_workspace_bytes", B, H,
+                                              Hkv, D, max_ctx, partition), dev, stream)
+        _call(dev, self.lib.attn_paged_decode_weights, q.data_ptr(), kc.data_ptr(), vc.data_ptr(),
+              bt.data_ptr(), ctx.data_ptr(), out.data_ptr(), weights.data_ptr(), *sizes, max_ctx,
+              scale, partition, ws.data_ptr(), ws.numel(), stream)
         return out
 
     # ------------------------------------------------- 4-bit cache, eviction
     def kv4_append(self, dev, k, v, kc, vc, slots, weights, sizes):
         T, Hkv, D, bs, nblk = sizes
         ks, vs = k.stride(), v.stride()
-        with _on_index(dev):
-            _check(self.lib.attn_kv4_append(
-                k.data_ptr(), v.data_ptr(), _DTYPES[k.dtype], kc.data_ptr(), vc.data_ptr(),
-                slots.data_ptr(), None if weights is None else weights.data_ptr(), T, Hkv, D,
-                ks[0], ks[1], vs[0], vs[1], bs, nblk, _raw_stream(dev)))
+        _call(dev, self.lib.attn_kv4_append, k.data_ptr(), v.data_ptr(), _DTYPES[k.dtype],
+              kc.data_ptr(), vc.data_ptr(), slots.data_ptr(),
+              None if weights is None else weights.data_ptr(), T, Hkv, D, ks[0], ks[1], vs[0],
+              vs[1], bs, nblk, _raw_stream(dev))
 
     def kv4_read(self, dev, kc, vc, slots, dtype, sizes):
-        T, Hkv, D, bs, nblk = sizes
-        k = kc.new_empty((T, Hkv, D), dtype=dtype)
+        k = kc.new_empty(sizes[:3], dtype=dtype)
         v = torch.empty_like(k)
-        with _on_index(dev):
-            _check(self.lib.attn_kv4_read(
-                kc.data_ptr(), vc.data_ptr(), slots.data_ptr(), k.data_ptr(), v.data_ptr(),
-                _DTYPES[dtype], T, Hkv, D, bs, nblk, _raw_stream(dev)))
+        _call(dev, self.lib.attn_kv4_read, kc.data_ptr(), vc.data_ptr(), slots.data_ptr(),
+              k.data_ptr(), v.data_ptr(), _DTYPES[dtype], *sizes, _raw_stream(dev))
         return k, v
 
     def kv4_decode(self, dev, q, kc, vc, bt, ctx, weights, sizes, max_ctx, scale):
         out = torch.empty_like(q)
         B, H, Hkv, D = sizes[:4]
-        with _on_index(dev):
-            stream = _raw_stream(dev)
-            ws = _call_workspace(_workspace_bytes("attn_kv4_decode_workspace_bytes", B, H, Hkv, D,
-                                                  max_ctx, 0 if weights is None else 1),
-                                 q.device, stream)
-            _check(self.lib.attn_kv4_decode(
-                q.data_ptr(), _DTYPES[q.dtype], kc.data_ptr(), vc.data_ptr(), bt.data_ptr(),
-                ctx.data_ptr(), out.data_ptr(), None if weights is None else weights.data_ptr(),
-                *sizes, max_ctx, scale, ws.data_ptr(), ws.numel(), stream))
+        stream = _raw_stream(dev)
+        ws = _call_workspace(_workspace_bytes("attn_kv4_decode_workspace_bytes", B, H, Hkv, D,
+                                              max_ctx, 0 if weights is None else 1), dev, stream)
+        _call(dev, self.lib.attn_kv4_decode, q.data_ptr(), _DTYPES[q.dtype], kc.data_ptr(),
+              vc.data_ptr(), bt.data_ptr(), ctx.data_ptr(), out.data_ptr(),
+              None if weights is None else weights.data_ptr(), *sizes, max_ctx, scale,
+              ws.data_ptr(), ws.numel(), stream)
         return out
 
     def paged_evict(self, dev, caches, row_bytes, weights, bt, ctx, new_bt, sizes, max_ctx, keep,
@@ -345,12 +346,10 @@ class Extension:
         new_lens = torch.empty(B, dtype=torch.int32, device=weights.device)
         kept = torch.empty((B, Hkv, keep), dtype=torch.int32, device=weights.device)
         n = len(caches)
-        with _on_index(dev):
-            _check(self.lib.attn_paged_evict(
-                (_vp * n)(*(c.data_ptr() for c in caches)), (_i64 * n)(*row_bytes), n,
-                weights.data_ptr(), bt.data_ptr(), ctx.data_ptr(), new_bt.data_ptr(),
-                new_lens.data_ptr(), kept.data_ptr(), B, Hkv, bs, nblk, maxb, max_ctx, new_maxb,
-                keep, recent, sinks, _raw_stream(dev)))
+        _call(dev, self.lib.attn_paged_evict, (_vp * n)(*(c.data_ptr() for c in caches)),
+              (_i64 * n)(*row_bytes), n, weights.data_ptr(), bt.data_ptr(), ctx.data_ptr(),
+              new_bt.data_ptr(), new_lens.data_ptr(), kept.data_ptr(), B, Hkv, bs, nblk, maxb,
+              max_ctx, new_maxb, keep, recent, sinks, _raw_stream(dev))
         return new_lens, kept
 
     # -------------------------------------------------------------- status

@@ -70,11 +70,11 @@ def _check_weights(weights, num_blocks, hkv, block_size):
 
 def _device_of(*tensors):
     """Index of the one CUDA device that the tensors are on."""
-    dev = tensors[0].get_device()
+    dev = tensors[0].get_device()  # -1: on the CPU
     for t in tensors:
-        if not t.is_cuda:
-            raise ValueError("tensors must be CUDA tensors")
-        if t.get_device() != dev:
+        if t.get_device() != dev or dev < 0:
+            if not all(t.is_cuda for t in tensors):
+                raise ValueError("tensors must be CUDA tensors")
             raise ValueError("tensors must be on one device")
     return dev
 
