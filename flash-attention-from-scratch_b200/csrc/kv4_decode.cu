@@ -33,8 +33,8 @@
 //   * The sums over a long context are kept centred. sum p v is near 0 where
 //     sum p scale code and sum p low are not, so V is summed as
 //         sum (p scale) (code - c) + sum p (low + c scale),   c = 8, 7 in turn:
-//     one product with the constants -c per tile and accumulator, and fp16 middles in
-//     the lows' place. (Summing codes and lows as they are left outputs of 131072
+//     one product with the constants -c per tile and group, added once a stage, and
+//     fp16 middles in the lows' place. (Summing codes and lows as they are left outputs of 131072
 //     tokens off by 0.8 %, from the tensor cores' rounding of the large sums alone.)
 //     P is two fp16 terms, P scale one, rounded once from both: the one rounding of
 //     a token's weight, like P's in fp16 attention.
@@ -63,7 +63,8 @@ struct Kv4Cfg {
   // 64 ragged sequences of up to 8192 tokens / 8 of 131072, 8 kv heads; one of 700):
   // 12 warps of 48 tokens 100 / 267, 8.9; 16 of 32 (128 registers, some spilled) 100 /
   // 268, 10.2; 8 of 64 106 / 292, 9.0. At 64 (64 x 8192, 64 query over 8 kv heads): 16
-  // warps of 64 tokens 66, 12 70, 8 78.
+  // warps of 64 tokens 66, 12 70, 8 78. (Before the centring product was one per group:
+  // the 12 of 48 are at 97 / 263, 8.8 with it, the 16 of 64 at 65.)
   static constexpr int W = D == 64 ? 16 : 12;
   static constexpr int THREADS = W * 32;
   static constexpr int NG = R::NG;
@@ -79,7 +80,7 @@ struct Kv4Cfg {
   static constexpr int PREFIX_OFF = META_OFF + W * STAGES * 16;
   static constexpr int CTX_OFF = PREFIX_OFF + (kLaunchBatch + 1) * 4;
   static constexpr int CENTRE_OFF = (CTX_OFF + kLaunchBatch * 4 + 15) / 16 * 16;
-  static constexpr int SMEM = CENTRE_OFF + 32 + 16;  // + the abort flag
+  static constexpr int SMEM = CENTRE_OFF + 16 + 16;  // + the abort flag
   static_assert(STAGE % 16 == 0 && KV % 16 == 0 && BAR_OFF % 16 == 0, "bulk copy alignment");
   static_assert(SMEM <= 227 * 1024, "shared memory per CTA");
 };
@@ -149,10 +150,8 @@ __device__ __forceinline__ uint32_t hfma2(uint32_t a, uint32_t b, uint32_t c) {
 }
 
 // Pairs of fp16: 8 and 7; and what centres an even and an odd row of V (8 and 7 codes
-// below, so that the middle of the codes is 0 on average), in the codes' unit 2^-24
-// and times 16.
-constexpr uint32_t kEight = 0x48004800u, kSeven = 0x47004700u;
-constexpr uint32_t kCentre = 0x80078008u, kCentre16 = 0x80708080u;
+// below, so that the middle of the codes is 0 on average), in the codes' unit 2^-24.
+constexpr uint32_t kEight = 0x48004800u, kSeven = 0x47004700u, kCentre = 0x80078008u;
 
 // N 32-bit words (1, 2 or 4) of shared memory in one load.
 template <int N>
@@ -197,9 +196,8 @@ __global__ void __launch_bounds__(Kv4Cfg<D>::THREADS, 1) kv4_decode_kernel(const
     ctx_s[b] = min(max(p.ctx[b], 0), p.max_ctx);
   if (threadIdx.x < C::W * C::STAGES)
     mbar_init(reinterpret_cast<uint64_t*>(smem + C::BAR_OFF) + threadIdx.x, 1);
-  if (threadIdx.x < 8)
-    reinterpret_cast<uint32_t*>(smem + C::CENTRE_OFF)[threadIdx.x] =
-        threadIdx.x < 4 ? kCentre : kCentre16;
+  if (threadIdx.x < 4)
+    reinterpret_cast<uint32_t*>(smem + C::CENTRE_OFF)[threadIdx.x] = kCentre;
   if (threadIdx.x == 0) {
     *abort_flag = 0;
     fence_mbar_init();
@@ -371,11 +369,10 @@ __global__ void __launch_bounds__(Kv4Cfg<D>::THREADS, 1) kv4_decode_kernel(const
   const int tok_k = (g4 & 1) ? ((g4 + 3) & 7) + 8 : g4;  // tau(g4)
   const int tok_v = ((2 * t4 + 4) & 7) + 8;              // tau(2 t4 + 1)
 
-  // The centring operands, by way of shared memory: operands that the compiler knows to
-  // be constant it writes out, four moves, before each of their products.
-  uint32_t ca[4], cb[4];
+  // The centring operand, by way of shared memory: an operand that the compiler knows to
+  // be constant it writes out, four moves, before each of its products.
+  uint32_t ca[4];
   load_words<4>(ca, smem + C::CENTRE_OFF);
-  load_words<4>(cb, smem + C::CENTRE_OFF + 16);
 
   auto load_q = [&](int b, int kvh) {
     const bool real = g4 < p.group;
@@ -581,7 +578,8 @@ __global__ void __launch_bounds__(Kv4Cfg<D>::THREADS, 1) kv4_decode_kernel(const
 #pragma unroll
       for (int i = 0; i < 4; ++i) z[i] *= alpha[i & 1];
     }
-    // O^T += V^T P^T.
+    // O^T += V^T P^T. centre: - c P scale of the stage, the same in every column.
+    float centre[NG][4];
 #pragma unroll
     for (int i = 0; i < MT; ++i) {
       const uint8_t* ra = vst + (16 * i + 2 * t4) * ROW;  // rows 2 t4 and (below, + ROW) 2 t4 + 8
@@ -623,12 +621,25 @@ __global__ void __launch_bounds__(Kv4Cfg<D>::THREADS, 1) kv4_decode_kernel(const
         const uint32_t x = __byte_perm(va[w / 2], vb[w / 2], half);
         const uint32_t y = __byte_perm(vc[w / 2], vd[w / 2], half);
         const uint32_t x8 = x >> 8, y8 = y >> 8;
-        mma_k16(acc[w][0], ca[0], ca[1], ca[2], ca[3], b0, b1);
-        mma_k16(acc[w][1], cb[0], cb[1], cb[2], cb[3], b0, b1);
+        if (i == 0)
+          mma_k16_new(centre[w], ca[0], ca[1], ca[2], ca[3], b0, b1);
+        else
+          mma_k16(centre[w], ca[0], ca[1], ca[2], ca[3], b0, b1);
         mma_k16(acc[w][0], x & 0x000F000Fu, x8 & 0x000F000Fu, y & 0x000F000Fu, y8 & 0x000F000Fu,
                 b0, b1);
         mma_k16(acc[w][1], x & 0x00F000F0u, x8 & 0x00F000F0u, y & 0x00F000F0u, y8 & 0x00F000F0u,
                 b0, b1);
+      }
+    }
+#pragma unroll
+    for (int w = 0; w < NG; ++w) {
+      const uint64_t c2 = f2_pack(centre[w][0], centre[w][1]), up = f2_pack(16.f, 16.f);
+#pragma unroll
+      for (int i = 0; i < 4; i += 2) {
+        f2_unpack(f2_add(f2_pack(acc[w][0][i], acc[w][0][i + 1]), c2), acc[w][0][i],
+                  acc[w][0][i + 1]);
+        f2_unpack(f2_fma(c2, up, f2_pack(acc[w][1][i], acc[w][1][i + 1])), acc[w][1][i],
+                  acc[w][1][i + 1]);
       }
     }
     if (md.w & kLast) {
