@@ -104,8 +104,10 @@ def _check_slots(slots):
 def _dense_rows(t):
     """t, or a copy of it where its rows are not 16-byte pieces that the kernel can load."""
     s0, s1, s2 = t.stride()
-    return t if s2 == 1 and s0 % 8 == 0 and s1 % 8 == 0 and t.data_ptr() % 16 == 0 \
-        else t.contiguous()
+    if s2 == 1 and s0 % 8 == 0 and s1 % 8 == 0 and t.data_ptr() % 16 == 0:
+        return t
+    # Not contiguous(): a dim of size 1 may have any stride there, and the address stays.
+    return t.clone(memory_format=torch.contiguous_format)
 
 
 def paged_append_kv4(k, v, k_cache, v_cache, slots, weights=None):

@@ -267,8 +267,9 @@ int attn_paged_decode_weights(const void* q, const void* k_cache, const void* v_
  * read or write otherwise; a sequence that is not cut may give its old pages
  * again, and is then not moved. Every other row of the arrays stays as it is, so
  * old pages (which other sequences may share) are the caller's to free.
- * sinks + recent <= keep. Lengths above max_context_len are cut to it. The
- * selection walks a sequence's totals in one CTA per (sequence, kv head).
+ * sinks + recent <= keep. Lengths above max_context_len are cut to it. A table
+ * entry outside the cache is reported as ATTN_DEVICE_BAD_BLOCK: its tokens count
+ * with the lowest total, and rows from or to it are not moved.
  * No counterpart in the reference.
  */
 int attn_paged_evict(void* const* arrays, const int64_t* row_bytes, int num_arrays, float* weights,

@@ -216,6 +216,17 @@ def test_append_strided(make):
     assert torch.equal(vc.cpu()[s // 16, :, s % 16], rv)
 
 
+def test_append_one_row_of_a_wider_tensor():
+    """A single token and head: its strides may be anything, its address unaligned."""
+    x = torch.randn(5, 4, 259).half().cuda()
+    for at in (0, 1, 3):
+        k = x[2:3, 1:2, at:at + 128]
+        kc, vc = (torch.zeros(1, 1, 16, 80, dtype=torch.uint8, device="cuda") for _ in range(2))
+        ak.paged_append_kv4(k, k, kc, vc, torch.tensor([7]).cuda())
+        assert torch.equal(kc[0, 0, 7].cpu(), ora.pack(k.cpu(), False)[0, 0])
+        assert torch.equal(vc[0, 0, 7].cpu(), ora.pack(k.cpu(), True)[0, 0])
+
+
 def test_append_and_read_report_slots_past_the_cache():
     k = torch.randn(3, 2, 64).half().cuda()
     kc = torch.zeros(2, 2, 16, 40, dtype=torch.uint8, device="cuda")
@@ -310,6 +321,32 @@ def test_decode4_many_sequences():
         got = out[b].double()
         assert torch.equal(got.isnan(), o.isnan()), b
         assert ((got - o).abs() < 1e-2)[~o.isnan()].all(), b
+
+
+def test_weights_of_many_sequences():
+    """Totals over more sequences than a launch takes, every page in one sequence."""
+    torch.manual_seed(2)
+    n, bs, d, hkv, g = 2300, 16, 64, 2, 2
+    bt = torch.randperm(2 * n).to(torch.int32).view(n, 2)
+    lens = torch.randint(0, 33, (n,), dtype=torch.int32)
+    x = torch.randn(2, 2 * n, hkv, bs, d).half()
+    rows = [ora.pack(x[i], i == 1) for i in range(2)]
+    q = torch.randn(n, hkv * g, d).half()
+    w4, w16 = (torch.zeros(2 * n, hkv, bs, device="cuda") for _ in range(2))
+    args = (bt.cuda(), lens.cuda(), 32)
+    ak.paged_decode_kv4(q.cuda(), rows[0].cuda(), rows[1].cuda(), *args, weights=w4)
+    ak.paged_decode_weights(q.cuda(), x[0].cuda(), x[1].cuda(), *args, w16)
+    for b in list(range(0, n, 57)) + [2047, 2048, n - 1]:
+        m = int(lens[b])
+        s = ora.slots_of(bt[b], 32, bs)
+        for h in range(hkv):
+            for w, k in ((w4, ora.unpack(ora.rows_of(rows[0], bt[b], m, h), False)),
+                         (w16, ora.rows_of(x[0], bt[b], m, h).double())):
+                got = w[s // bs, h, s % bs].cpu().double()
+                _, p = ora.attend(q[b, g * h:g * h + g], k, k)
+                # p moves by 2 d + 2^-21 relative, d below 1e-5 for values of a few units.
+                assert ((got[:m] - p.sum(0)).abs() <= 3e-5 * p.sum(0)).all()
+                assert (got[m:] == 0).all()
 
 
 @pytest.mark.parametrize("d,bs", [(128, 1), (128, 3), (64, 2), (64, 6), (128, 40)])
@@ -548,9 +585,18 @@ def test_evict_cuts_lengths_above_max():
     check_evict([500, 80], 2, 16, 64, 8, 2, max_ctx=300)
 
 
-@pytest.mark.parametrize("n", [20000, 70000])
-def test_evict_long(n):
-    check_evict([n], 1, 16, n // 3, 100, 4, rows=((4,),))
+@pytest.mark.parametrize("n,bs", [(20000, 16), (70000, 16), (70000, 30), (420000, 16),
+                                  (420000, 63)])
+def test_evict_long(n, bs):
+    """One sequence over a cluster of CTAs, up to more totals than their shared memory holds."""
+    check_evict([n], 1, bs, n // 3, 100, 4, rows=((4,),))
+
+
+def test_evict_many_sequences():
+    """More (sequence, head) pairs than the GPU has SMs, lengths from nothing to a few thousand."""
+    g = torch.Generator().manual_seed(5)
+    check_evict(torch.randint(0, 2500, (60,), generator=g).tolist(), 4, 16, 300, 20, 3,
+                rows=((8,),))
 
 
 def test_evict_reports_bad_blocks():
