@@ -103,14 +103,14 @@ __device__ __forceinline__ void append_row(uint8_t* dst, uint4 raw, bool real, i
   unpack2(ends, lo, neg_hi, T());
   __half lo_h = __float2half_rn(lo);
   const float low = __half2float(lo_h);
-  // The range over 15: by a product, which is off by two fp32 steps at most, and by
-  // the division where those could change the fp16 result (within 2 of a midpoint
-  // of fp16's steps, or below its normal range).
+  // The range over 15, correctly rounded: with y = RN(1 / 15) and q = RN(range y), the
+  // residual range - 15 q is exact in an fma and RN(q + residual y) is the quotient
+  // (P. Markstein, IBM Journal of Research and Development 34, 1990).
   const float range = -neg_hi - low;
-  float fifteenth = range * (1.f / 15.f);
-  if ((__float_as_uint(fifteenth) & 0x1FFFu) - 0xFFEu <= 4u || !(fifteenth >= 0x1p-14f))
-    fifteenth = __fdiv_rn(range, 15.f);
-  __half scale_h = __float2half_rn(fifteenth);
+  constexpr float kFifteenth = 1.f / 15.f;
+  const float about = range * kFifteenth;
+  __half scale_h =
+      __float2half_rn(fmaf(fmaf(-15.f, about, range), kFifteenth, about));
   if (!(fabsf(lo) <= 65504.f && fabsf(neg_hi) <= 65504.f))
     lo_h = scale_h = __ushort_as_half(0x7fff);  // NaN
   const float scale = __half2float(scale_h);
