@@ -28,6 +28,7 @@ tables are used in place and must be contiguous.
 """
 from __future__ import annotations
 
+import functools
 import math
 
 import torch
@@ -207,6 +208,7 @@ def paged_decode_kv4(q, k_cache, v_cache, block_tables, context_lens, max_contex
     return out if q.dim() == 3 else out.reshape(q.shape)
 
 
+@functools.lru_cache(maxsize=4096)
 def _weights_partition(batch, hkv, max_context_len, dev, heads, head_dim):
     """decode_partition's choice, doubled while that leaves six units per resident warp: fewer
     parts to merge (64 ragged sequences of up to 8192 tokens, 32 query over 8 kv heads, d 128:

@@ -75,6 +75,7 @@ __global__ void __launch_bounds__(T) evict_select_kernel(const SelectParams p) {
   __shared__ int share_gt, share_eq;
   __shared__ uint32_t s_digit;
   __shared__ int s_left;
+  __shared__ bool s_whole;
   cg::cluster_group cluster = cg::this_cluster();
   const int ranks = static_cast<int>(cluster.num_blocks());
   const int rank = static_cast<int>(cluster.block_rank());
@@ -207,12 +208,20 @@ __global__ void __launch_bounds__(T) evict_select_kernel(const SelectParams p) {
       if (above < rest && rest <= above + one) {
         s_digit = static_cast<uint32_t>(32 * block + 31 - lane);
         s_left = rest - above;
+        s_whole = rest - above == one;
       }
     }
     __syncthreads();
     prefix |= s_digit << shift;
     left = s_left;
     mask |= digits << shift;
+    if (s_whole) {
+      // The whole bin stays (of distinct totals a bin of the second pass mostly holds
+      // one): all above the key before its first, and the passes are over.
+      prefix -= 1u;
+      left = 0;
+      break;
+    }
   }
 
   // Above the key: all; at it: the first `left` of the candidates.
