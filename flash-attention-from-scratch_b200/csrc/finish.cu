@@ -176,6 +176,7 @@ __device__ void add_weights(const FinishParams& p) {
   const unsigned int stride = static_cast<unsigned int>(p.add_chunks) * kAddTokens;
   const unsigned int end = static_cast<unsigned int>(ctx);
   if (t0 >= end) return;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   __shared__ float mx[8], inv[8];
   const int* bt = p.bt + static_cast<size_t>(b) * p.max_blocks;
   const float* sc = p.scores + static_cast<size_t>(pair) * p.max_ctx * GP;
@@ -255,22 +256,22 @@ __device__ void add_weights(const FinishParams& p) {
 }
 
 // Launched as a programmatic dependent of the decode: it waits for that launch's
-// end before it reads what the decode wrote.
+// end before it reads what the decode wrote (lengths are an input of both).
 template <int D, int WPR, typename T>
 __global__ void __launch_bounds__(kThreads<WPR>) finish_kernel(const FinishParams p) {
   constexpr int THREADS = kThreads<WPR>;
   const int warp = threadIdx.x >> 5;
-  asm volatile("griddepcontrol.wait;" ::: "memory");
   if (static_cast<int>(blockIdx.x) < p.merge_blocks) {
     const long long row = static_cast<long long>(blockIdx.x) * (THREADS / 32 / WPR) + warp / WPR;
     bool live = row < static_cast<long long>(p.batch) * p.hq;
     Parts r = {0, 0, 0, 0};
-    int g = 0;
+    const int b = live ? static_cast<int>(row / p.hq) : 0;
+    const int head = live ? static_cast<int>(row - static_cast<long long>(b) * p.hq) : 0;
+    const int kvh = head / p.group, g = head - kvh * p.group;
+    const int ctx = min(max(p.ctx[b], 0), p.max_ctx);  // an input of the decode too
+    asm volatile("griddepcontrol.wait;" ::: "memory");
     if (live) {
-      const int b = static_cast<int>(row / p.hq), head = static_cast<int>(row - static_cast<long long>(b) * p.hq);
-      const int kvh = head / p.group;
-      g = head - kvh * p.group;
-      r = parts_of(p, b, kvh, min(max(p.ctx[b], 0), p.max_ctx));
+      r = parts_of(p, b, kvh, ctx);
       if (p.first != nullptr && r.count == 1) live = false;  // written by the decode
     }
     merge_row<D, WPR, T>(p, row, live, r, g);
