@@ -153,11 +153,16 @@ class _StreamWorkspaces:
     when a call needs more, like a BLAS library's workspace: calls on one stream
     run in order, so each may reuse the bytes of the one before. The buffer is
     allocated while its stream is current, so the caching allocator never hands
-    its memory to another stream while a kernel may still use it."""
+    its memory to another stream while a kernel may still use it.
+
+    A call holds `launching` from taking the buffer to its last launch: library
+    calls run without the GIL, and a second thread's launches on the same stream
+    must not come between the launch that fills the buffer and the one that reads it."""
 
     def __init__(self):
         self._bufs: dict[tuple[int, int], torch.Tensor] = {}
         self._lock = threading.Lock()
+        self.launching = threading.RLock()
 
     def get(self, nbytes: int, device: torch.device, stream: int) -> torch.Tensor:
         key = (device.index if device.index is not None else torch.cuda.current_device(), stream)
@@ -246,7 +251,7 @@ class Extension:
     def paged_decode(self, q, kc, vc, bt, ctx, max_ctx, scale, partition):
         out = torch.empty_like(q)
         B, H, Hkv, D, bs, nblk, maxb = self._decode_sizes(q, kc, bt)
-        with _on(q.device):
+        with _on(q.device), _decode_ws.launching:
             stream = _stream(q.device)
             ws = _decode_ws.get(
                 self.lib.attn_paged_decode_workspace_bytes(B, H, D, max_ctx, partition),
@@ -264,7 +269,7 @@ class Extension:
         o = torch.empty(B, H, D, **f32) if o is None else o
         m = torch.empty(B, H, **f32) if m is None else m
         l = torch.empty(B, H, **f32) if l is None else l
-        with _on(q.device):
+        with _on(q.device), _decode_ws.launching:
             stream = _stream(q.device)
             ws = _decode_ws.get(
                 self.lib.attn_paged_decode_workspace_bytes(B, H, D, max_ctx, partition),
@@ -305,11 +310,14 @@ class Extension:
         out = torch.empty_like(q)
         B, H, Hkv, D = sizes[:4]
         stream = _raw_stream(dev)
-        ws = _call_workspace(_workspace_bytes("attn_paged_decode_weights_workspace_bytes", B, H,
-                                              Hkv, D, max_ctx, partition), dev, stream)
-        _call(dev, self.lib.attn_paged_decode_weights, q.data_ptr(), kc.data_ptr(), vc.data_ptr(),
-              bt.data_ptr(), ctx.data_ptr(), out.data_ptr(), weights.data_ptr(), *sizes, max_ctx,
-              scale, partition, ws.data_ptr(), ws.numel(), stream)
+        nbytes = _workspace_bytes("attn_paged_decode_weights_workspace_bytes", B, H, Hkv, D,
+                                  max_ctx, partition)
+        with _decode_ws.launching:
+            ws = _call_workspace(nbytes, dev, stream)
+            _call(dev, self.lib.attn_paged_decode_weights, q.data_ptr(), kc.data_ptr(),
+                  vc.data_ptr(), bt.data_ptr(), ctx.data_ptr(), out.data_ptr(),
+                  weights.data_ptr(), *sizes, max_ctx, scale, partition, ws.data_ptr(),
+                  ws.numel(), stream)
         return out
 
     # ------------------------------------------------- 4-bit cache, eviction
@@ -332,12 +340,14 @@ class Extension:
         out = torch.empty_like(q)
         B, H, Hkv, D = sizes[:4]
         stream = _raw_stream(dev)
-        ws = _call_workspace(_workspace_bytes("attn_kv4_decode_workspace_bytes", B, H, Hkv, D,
-                                              max_ctx, 0 if weights is None else 1), dev, stream)
-        _call(dev, self.lib.attn_kv4_decode, q.data_ptr(), _DTYPES[q.dtype], kc.data_ptr(),
-              vc.data_ptr(), bt.data_ptr(), ctx.data_ptr(), out.data_ptr(),
-              None if weights is None else weights.data_ptr(), *sizes, max_ctx, scale,
-              ws.data_ptr(), ws.numel(), stream)
+        nbytes = _workspace_bytes("attn_kv4_decode_workspace_bytes", B, H, Hkv, D, max_ctx,
+                                  0 if weights is None else 1)
+        with _decode_ws.launching:
+            ws = _call_workspace(nbytes, dev, stream)
+            _call(dev, self.lib.attn_kv4_decode, q.data_ptr(), _DTYPES[q.dtype], kc.data_ptr(),
+                  vc.data_ptr(), bt.data_ptr(), ctx.data_ptr(), out.data_ptr(),
+                  None if weights is None else weights.data_ptr(), *sizes, max_ctx, scale,
+                  ws.data_ptr(), ws.numel(), stream)
         return out
 
     def paged_evict(self, dev, caches, row_bytes, weights, bt, ctx, new_bt, sizes, max_ctx, keep,

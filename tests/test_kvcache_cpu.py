@@ -171,3 +171,63 @@ def test_abi_weights_refusals(lib):
     assert need == base + 2 * 8 * 80 * 4
     assert weights(w=None) == 1 and weights(hq=24) == 2 and weights(max_ctx=81) == 1
     assert weights(ws_bytes=base) == 4 and "paged_decode_weights" in err(lib)
+
+
+class _OneAtATime:
+    """A library whose decode calls take a while and record whether two of them had
+    the same workspace at once, as a second thread's launches between two of the
+    first one's would."""
+
+    def __init__(self):
+        import threading
+        self.inside, self.overlap, self.guard = set(), False, threading.Lock()
+
+    def _decode(self, *args):
+        import time
+        ws = args[-3]
+        with self.guard:
+            self.overlap |= ws in self.inside
+            self.inside.add(ws)
+        time.sleep(0.01)
+        with self.guard:
+            self.inside.discard(ws)
+        return 0
+
+    attn_kv4_decode = attn_paged_decode_weights = _decode
+
+
+def _fake_extension(monkeypatch):
+    """An Extension over _OneAtATime: no GPU, workspaces of 1 KiB and more on the CPU."""
+    ext = _native.Extension.__new__(_native.Extension)
+    ext.lib = _OneAtATime()
+    monkeypatch.setattr(_native, "_raw_stream", lambda dev: 0)
+    monkeypatch.setattr(_native, "_workspace", lambda n, device: torch.empty(n, dtype=torch.uint8))
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    ak.release_workspaces()
+    return ext
+
+
+def test_threads_on_one_stream_take_turns(monkeypatch):
+    import threading
+    ext = _fake_extension(monkeypatch)
+    q = torch.zeros(1, 8, 64, dtype=torch.float16)
+    kc = torch.zeros(1, 8, 16, 40, dtype=torch.uint8)
+    t, w = torch.zeros(1, 1, dtype=torch.int32), torch.zeros(1, 8, 16)
+    sizes = (1, 8, 8, 64, 16, 1, 1)
+
+    def four_bit():
+        for _ in range(5):
+            ext.kv4_decode(0, q, kc, kc, t, t[0], None, sizes, 16, 1.0)
+
+    def weights():
+        for _ in range(5):
+            ext.paged_decode_weights(0, q, kc, kc, t, t[0], w, sizes, 16, 1.0, 128)
+
+    threads = [threading.Thread(target=f) for f in (four_bit, weights, four_bit, weights)]
+    for th in threads:
+        th.start()
+    for th in threads:
+        th.join()
+    ak.release_workspaces()
+    assert not ext.lib.overlap
