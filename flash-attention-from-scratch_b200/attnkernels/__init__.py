@@ -255,6 +255,7 @@ def release_workspaces():
     split-K partials), so the caching allocator can reuse or free their memory.
     Call it when no decode is in flight on those streams."""
     _native._decode_ws.clear()
+    _native._cache_ws.clear()
 
 
 def device_status(device=None):

@@ -185,6 +185,10 @@ class _StreamWorkspaces:
 
 
 _decode_ws = _StreamWorkspaces()
+# Of the 4-bit decode and the decode with weights. Not the same buffers: a captured
+# paged_decode replays on the buffer that it was captured with, which another
+# operator's larger call must not replace.
+_cache_ws = _StreamWorkspaces()
 
 
 def _call_workspace(nbytes: int, dev: int, stream: int) -> torch.Tensor:
@@ -193,10 +197,10 @@ def _call_workspace(nbytes: int, dev: int, stream: int) -> torch.Tensor:
     back, nor share it with another graph."""
     if torch.cuda.is_current_stream_capturing():
         return _workspace(nbytes, torch.device("cuda", dev))
-    buf = _decode_ws.kept(dev, stream)
+    buf = _cache_ws.kept(dev, stream)
     if buf is not None and buf.numel() >= nbytes:
         return buf
-    return _decode_ws.get(nbytes, torch.device("cuda", dev), stream)
+    return _cache_ws.get(nbytes, torch.device("cuda", dev), stream)
 
 
 @functools.lru_cache(maxsize=4096)
@@ -312,7 +316,7 @@ class Extension:
         stream = _raw_stream(dev)
         nbytes = _workspace_bytes("attn_paged_decode_weights_workspace_bytes", B, H, Hkv, D,
                                   max_ctx, partition)
-        with _decode_ws.launching:
+        with _cache_ws.launching:
             ws = _call_workspace(nbytes, dev, stream)
             _call(dev, self.lib.attn_paged_decode_weights, q.data_ptr(), kc.data_ptr(),
                   vc.data_ptr(), bt.data_ptr(), ctx.data_ptr(), out.data_ptr(),
@@ -342,7 +346,7 @@ class Extension:
         stream = _raw_stream(dev)
         nbytes = _workspace_bytes("attn_kv4_decode_workspace_bytes", B, H, Hkv, D, max_ctx,
                                   0 if weights is None else 1)
-        with _decode_ws.launching:
+        with _cache_ws.launching:
             ws = _call_workspace(nbytes, dev, stream)
             _call(dev, self.lib.attn_kv4_decode, q.data_ptr(), _DTYPES[q.dtype], kc.data_ptr(),
                   vc.data_ptr(), bt.data_ptr(), ctx.data_ptr(), out.data_ptr(),

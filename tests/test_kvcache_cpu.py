@@ -231,3 +231,19 @@ def test_threads_on_one_stream_take_turns(monkeypatch):
         th.join()
     ak.release_workspaces()
     assert not ext.lib.overlap
+
+
+def test_paged_decode_keeps_its_scratch(monkeypatch):
+    """A captured paged_decode holds the address of its buffer."""
+    ext = _fake_extension(monkeypatch)
+    kept = _native._decode_ws.get(1 << 20, torch.device("cuda", 0), 0)
+    q = torch.zeros(512, 8, 64, dtype=torch.float16)
+    kc = torch.zeros(1, 8, 16, 40, dtype=torch.uint8)
+    t = torch.zeros(512, 64, dtype=torch.int32)
+    w = torch.zeros(1, 8, 16)
+    ext.kv4_decode(0, q, kc, kc, t, t[:, 0], w, (512, 8, 8, 64, 16, 1, 64), 1024, 1.0)
+    assert _native._workspace_bytes("attn_kv4_decode_workspace_bytes", 512, 8, 8, 64, 1024,
+                                    1) > kept.numel()
+    assert _native._decode_ws.kept(0, 0) is kept
+    ak.release_workspaces()
+    assert _native._decode_ws._bufs == {} == _native._cache_ws._bufs
