@@ -63,7 +63,11 @@ __device__ __forceinline__ Parts parts_of(const FinishParams& p, int b, int kvh,
   return r;
 }
 
-// WPR warps per row (1, 8 or 32) merge: lane owns D / 32 columns; each warp folds
+// Threads of a CTA.
+template <int WPR>
+constexpr int kThreads = WPR == 32 ? 1024 : 256;
+
+// WPR warps per row (a power of two) merge: lane owns D / 32 columns; each warp folds
 // chunks of 8 parts into a running (max, sum, numerator), and the warps of a row
 // combine in shared memory. A chunk is one round trip to memory, so rows with many
 // parts (few rows, a long context) take more warps.
@@ -124,7 +128,8 @@ __device__ void merge_row(const FinishParams& p, long long row, bool live, const
     }
   }
   if constexpr (WPR > 1) {
-    __shared__ float red[WPR][D + 2];
+    __shared__ float red[kThreads<WPR> / 32][D + 2];
+    const int row0 = warp - sub;  // the row's first warp
 #pragma unroll
     for (int j = 0; j < DV; ++j) red[warp][lane * DV + j] = num[j];
     if (lane == 0) {
@@ -134,17 +139,17 @@ __device__ void merge_row(const FinishParams& p, long long row, bool live, const
     __syncthreads();
     if (!live || sub != 0) return;
     float big = mw;
-    for (int w = 1; w < WPR; ++w) big = fmaxf(big, red[w][D + 1]);
+    for (int w = 1; w < WPR; ++w) big = fmaxf(big, red[row0 + w][D + 1]);
     den = 0.f;
 #pragma unroll
     for (int j = 0; j < DV; ++j) num[j] = 0.f;
     for (int w = 0; w < WPR; ++w) {
-      const float mx = red[w][D + 1];
+      const float mx = red[row0 + w][D + 1];
       if (mx == -INFINITY) continue;  // a warp without parts
       const float a = fast_exp2(mx - big);
-      den = fmaf(a, red[w][D], den);
+      den = fmaf(a, red[row0 + w][D], den);
 #pragma unroll
-      for (int j = 0; j < DV; ++j) num[j] = fmaf(a, red[w][lane * DV + j], num[j]);
+      for (int j = 0; j < DV; ++j) num[j] = fmaf(a, red[row0 + w][lane * DV + j], num[j]);
     }
   }
   if (!live) return;
@@ -154,10 +159,6 @@ __device__ void merge_row(const FinishParams& p, long long row, bool live, const
 #pragma unroll
   for (int j = 0; j < DV; j += 2) dst[j / 2] = pack2<T>(num[j] * inv, num[j + 1] * inv);
 }
-
-// Threads of a CTA.
-template <int WPR>
-constexpr int kThreads = WPR == 32 ? 1024 : 256;
 
 constexpr int kAddTokens = 1024;  // tokens a CTA adds at a time
 
@@ -310,6 +311,8 @@ cudaError_t by_warps(const FinishParams& p, unsigned grid, int wpr, bool bf16,
                      cudaStream_t stream) {
   return wpr == 32  ? by_type<D, 32>(p, grid, bf16, stream)
          : wpr == 8 ? by_type<D, 8>(p, grid, bf16, stream)
+         : wpr == 4 ? by_type<D, 4>(p, grid, bf16, stream)
+         : wpr == 2 ? by_type<D, 2>(p, grid, bf16, stream)
                     : by_type<D, 1>(p, grid, bf16, stream);
 }
 
@@ -351,13 +354,19 @@ cudaError_t launch_finish(const FinishArgs& a, const LaunchCtx& ctx) {
   p.max_blocks = static_cast<int>(a.max_blocks);
   p.max_ctx = static_cast<int>(a.max_ctx);
   const int64_t rows = a.batch * a.hq;
-  // Warps per row by the parts a row can have: up to four chunks of 8 a warp.
+  // Warps per row by the parts a row can have: up to four chunks of 8 a warp; more warps
+  // where few rows leave SMs idle meanwhile (4-bit decode, head_dim 128, 8 kv heads of 4
+  // query heads, one / up to 8 warps a row, us: 8 x 1728 tokens 17.1 / 12.6, 16 x 1152
+  // 15.6 / 14.1, 16 x 2304 19.8 / 18.7), but fewer of them where CTAs that add weights
+  // wait behind them (16 x 1152 with weights: by the first rule 17.5, by the second 16.0).
   const int64_t per_row = a.first == nullptr
                               ? a.parts
                               : std::min((a.max_ctx + a.partition - 1) / a.partition,
                                          a.workers / (a.batch * a.hkv) + 1);
-  const int wpr = per_row >= 128 ? 32 : per_row >= 32 ? 8 : 1;
-  const int64_t merge = wpr == 1 ? (rows + 7) / 8 : rows;
+  int wpr = per_row >= 128 ? 32 : per_row >= 32 ? 8 : 1;
+  const int64_t chunk = a.scores == nullptr ? 4 : 8, most = a.scores == nullptr ? 2048 : 1024;
+  while (wpr < 8 && per_row > chunk * wpr && 2 * rows * wpr <= most) wpr *= 2;
+  const int64_t merge = wpr == 32 ? rows : (rows * wpr + 7) / 8;
   // CTAs that add: one per 1024 tokens of a pair, but no more than about six per SM,
   // each then walking on: finding M and L costs a CTA as much as the tokens of one
   // such step (64 ragged sequences of up to 8192 tokens, 8 kv heads of 4 query heads,

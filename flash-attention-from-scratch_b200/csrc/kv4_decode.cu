@@ -15,6 +15,8 @@
 //     written at once; of the others each warp leaves a part, in slot i + row,
 //     which no two (warp, row) pairs share, since along the runs one of the two
 //     grows at each step: n + rows slots are enough for any lengths.
+//     Where there are few short rows, a CTA has one, its warps share out the stages and
+//     it merges their parts itself (JOIN): one launch instead of two.
 //   * Both products run on the tensor cores (mma.sync m16n8k16) with the cached
 //     rows as the 16-row operand A and the query heads of the kv head as the 8
 //     columns of B, so up to 8 heads cost what one does:
@@ -75,6 +77,8 @@ struct Kv4Cfg {
   static constexpr int STAGE = 2 * KV;
   static constexpr int STAGES = 2;
   static constexpr int RING = STAGES * STAGE;
+  static constexpr int ML_OFF = 8 * D * 4;  // JOIN: a part's m and l, behind its o, in the ring
+  static_assert(ML_OFF + 8 * 8 <= RING, "a part in the ring");
   static constexpr int BAR_OFF = W * RING;
   static constexpr int META_OFF = (BAR_OFF + W * STAGES * 8 + 15) / 16 * 16;
   static constexpr int PREFIX_OFF = META_OFF + W * STAGES * 16;
@@ -97,6 +101,8 @@ struct Kv4DecParams {
   float* l_part;
   int* first;             // [batch + 1]: stages of one head before each sequence
   float* scores;          // SCORED: [batch, hkv, max_ctx, gp] log2-unit scores
+  float* weights;         // SCORED and JOIN: [num_blocks, hkv, bs]
+  FastDiv by_bs;
   DeviceStatus* status;
   unsigned long long timeout_ns;
   unsigned int block_stride;  // bytes between physical blocks
@@ -170,7 +176,9 @@ __device__ __forceinline__ void load_words(uint32_t (&r)[N], const uint8_t* p) {
 // 2^e as a float, -126 <= e <= 127.
 __device__ __forceinline__ float pow2i(int e) { return __int_as_float((e + 127) << 23); }
 
-template <int D, typename T, bool SCORED>
+// JOIN: a CTA has one (sequence, kv head) row, dealt out in equal runs to its warps,
+// and merges their parts itself, in shared memory.
+template <int D, typename T, bool SCORED, bool JOIN>
 __global__ void __launch_bounds__(Kv4Cfg<D>::THREADS, 1) kv4_decode_kernel(const Kv4DecParams p) {
   using C = Kv4Cfg<D>;
   constexpr int NG = C::NG, ROW = C::ROW, CODES = C::R::CODES, kTok = C::TOK, MT = C::MT;
@@ -188,12 +196,19 @@ __global__ void __launch_bounds__(Kv4Cfg<D>::THREADS, 1) kv4_decode_kernel(const
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + C::SMEM - 16);
   // The merge that follows may be scheduled now; it waits for this launch's end
   // before it reads the parts.
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  if constexpr (!JOIN) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
   // Lengths and the stages of one head before each sequence, which the finish
   // kernel goes by too.
-  for (int b = threadIdx.x; b < p.batch; b += C::THREADS)
-    ctx_s[b] = min(max(p.ctx[b], 0), p.max_ctx);
+  const int my_b = static_cast<int>(blockIdx.x) / p.hkv;  // JOIN
+  int my_len = 0;
+  if constexpr (JOIN) {
+    my_len = min(max(p.ctx[my_b], 0), p.max_ctx);
+  } else {
+    for (int b = threadIdx.x; b < p.batch; b += C::THREADS)
+      ctx_s[b] = min(max(p.ctx[b], 0), p.max_ctx);
+  }
+  auto len_of = [&](int b) { return JOIN ? my_len : ctx_s[b]; };
   if (threadIdx.x < C::W * C::STAGES)
     mbar_init(reinterpret_cast<uint64_t*>(smem + C::BAR_OFF) + threadIdx.x, 1);
   if (threadIdx.x < 4)
@@ -203,36 +218,40 @@ __global__ void __launch_bounds__(Kv4Cfg<D>::THREADS, 1) kv4_decode_kernel(const
     fence_mbar_init();
   }
   __syncthreads();
-  if (warp == 0) {
-    const int per = (p.batch + 31) / 32;
-    const int b0 = lane * per;
-    int sum = 0;
-    for (int i = 0; i < per; ++i)
-      if (b0 + i < p.batch) sum += (ctx_s[b0 + i] + kTok - 1) / kTok;
-    int incl = sum;
+  if constexpr (!JOIN) {
+    if (warp == 0) {
+      const int per = (p.batch + 31) / 32;
+      const int b0 = lane * per;
+      int sum = 0;
+      for (int i = 0; i < per; ++i)
+        if (b0 + i < p.batch) sum += (ctx_s[b0 + i] + kTok - 1) / kTok;
+      int incl = sum;
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int y = __shfl_up_sync(0xffffffffu, incl, o);
-      if (lane >= o) incl += y;
-    }
-    int run = incl - sum;
-    for (int i = 0; i < per; ++i) {
-      if (b0 + i < p.batch) {
-        prefix[b0 + i] = run;
-        run += (ctx_s[b0 + i] + kTok - 1) / kTok;
+      for (int o = 1; o < 32; o <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, incl, o);
+        if (lane >= o) incl += y;
       }
+      int run = incl - sum;
+      for (int i = 0; i < per; ++i) {
+        if (b0 + i < p.batch) {
+          prefix[b0 + i] = run;
+          run += (ctx_s[b0 + i] + kTok - 1) / kTok;
+        }
+      }
+      if (lane == 31) prefix[p.batch] = incl;
     }
-    if (lane == 31) prefix[p.batch] = incl;
-  }
-  __syncthreads();
-  if (blockIdx.x == 0) {
-    for (int b = threadIdx.x; b <= p.batch; b += C::THREADS) p.first[b] = prefix[b];
+    __syncthreads();
+    if (blockIdx.x == 0) {
+      for (int b = threadIdx.x; b <= p.batch; b += C::THREADS) p.first[b] = prefix[b];
+    }
   }
 
   // This warp's run of stages. Warps next to each other in number are on different
   // SMs, so that a small call spreads over all of them.
-  const unsigned int worker = warp * gridDim.x + blockIdx.x;
-  const Runs runs(static_cast<unsigned int>(prefix[p.batch]) * p.hkv, C::W * gridDim.x);
+  const unsigned int worker = JOIN ? warp : warp * gridDim.x + blockIdx.x;
+  const Runs runs(JOIN ? (my_len + kTok - 1) / kTok
+                       : static_cast<unsigned int>(prefix[p.batch]) * p.hkv,
+                  JOIN ? C::W : C::W * gridDim.x);
   const unsigned int run0 = runs.begin(worker);
   unsigned int left = worker < runs.workers ? runs.begin(worker + 1) - run0 : 0u;
 
@@ -258,7 +277,7 @@ __global__ void __launch_bounds__(Kv4Cfg<D>::THREADS, 1) kv4_decode_kernel(const
     unsigned int page = static_cast<unsigned int>(bt_next);
     if (page >= static_cast<unsigned int>(p.num_blocks)) {  // never read outside the cache
       // An entry past the sequence's last page is not looked at.
-      if ((bt_base + lane) * static_cast<long long>(p.bs) < ctx_s[pb])
+      if ((bt_base + lane) * static_cast<long long>(p.bs) < len_of(pb))
         report_status(p.status, 2u /* ATTN_DEVICE_BAD_BLOCK */, kSiteKv4Block);
       page = 0;
     }
@@ -277,7 +296,13 @@ __global__ void __launch_bounds__(Kv4Cfg<D>::THREADS, 1) kv4_decode_kernel(const
     fresh = true;
   };
 
-  if (left > 0) {
+  if constexpr (JOIN) {
+    pb = my_b;
+    pkvh = static_cast<int>(blockIdx.x) - my_b * p.hkv;
+    pnst = (my_len + kTok - 1) / kTok;
+    pst = static_cast<int>(run0);
+    if (left > 0) open_row();
+  } else if (left > 0) {
     int lo = 0, hi = p.batch - 1;  // last sequence whose first stage is <= run0
     while (lo < hi) {
       const int mid = (lo + hi + 1) >> 1;
@@ -300,7 +325,7 @@ __global__ void __launch_bounds__(Kv4Cfg<D>::THREADS, 1) kv4_decode_kernel(const
     uint8_t* dst = ring + p_slot * C::STAGE;
     uint64_t* bar = full + p_slot;
     const int t0 = pst * kTok;
-    const int nt = min(kTok, ctx_s[pb] - t0);
+    const int nt = min(kTok, len_of(pb) - t0);
     // Copies are of whole 16 bytes: where a row is not (40 bytes), an odd last token
     // brings the row after it along, which is in its page (the block size is even).
     int todo = ROW % 16 != 0 ? nt + (nt & 1) : nt;
@@ -340,7 +365,7 @@ __global__ void __launch_bounds__(Kv4Cfg<D>::THREADS, 1) kv4_decode_kernel(const
     --left;
     pfirst = false;
     ++pst;
-    if (row_end && left > 0) {
+    if (!JOIN && row_end && left > 0) {
       pst = 0;
       if (++pkvh == p.hkv) {
         pkvh = 0;
@@ -660,8 +685,12 @@ __global__ void __launch_bounds__(Kv4Cfg<D>::THREADS, 1) kv4_decode_kernel(const
           o[1] = fmaf(acc[w][1][h], 0x1p20f, low) * inv;
           o[2] = fmaf(acc[w][0][h + 2], 0x1p24f, low) * inv;
           o[3] = fmaf(acc[w][1][h + 2], 0x1p20f, low) * inv;
-          if (head < p.group) {
-            const int col = 32 * w + 4 * g4;
+          const int col = 32 * w + 4 * g4;
+          if constexpr (JOIN) {
+            // The ring holds no copy any more: this was the warp's last stage.
+            *reinterpret_cast<float4*>(ring + (head * D + col) * 4) =
+                make_float4(o[0], o[1], o[2], o[3]);
+          } else if (head < p.group) {
             if (md.w & kWhole)
               *reinterpret_cast<uint2*>(static_cast<T*>(p.out) + row * D + col) =
                   make_uint2(pack2<T>(o[0], o[1]), pack2<T>(o[2], o[3]));
@@ -670,9 +699,13 @@ __global__ void __launch_bounds__(Kv4Cfg<D>::THREADS, 1) kv4_decode_kernel(const
                   make_float4(o[0], o[1], o[2], o[3]);
           }
         }
-        if (head < p.group && g4 == 0 && (SCORED || !(md.w & kWhole))) {
-          // A part whose scores are all NaN has no maximum, yet is not an empty one.
-          p.m_part[pr] = l[h] != l[h] ? fmaxf(m[h], 0.f) : m[h];
+        // A part whose scores are all NaN has no maximum, yet is not an empty one.
+        const float mh = l[h] != l[h] ? fmaxf(m[h], 0.f) : m[h];
+        if constexpr (JOIN) {
+          if (g4 == 0)
+            *reinterpret_cast<float2*>(ring + C::ML_OFF + head * 8) = make_float2(mh, 0.25f * l[h]);
+        } else if (head < p.group && g4 == 0 && (SCORED || !(md.w & kWhole))) {
+          p.m_part[pr] = mh;
           p.l_part[pr] = 0.25f * l[h];
         }
       }
@@ -699,6 +732,51 @@ __global__ void __launch_bounds__(Kv4Cfg<D>::THREADS, 1) kv4_decode_kernel(const
     if (++c_slot == C::STAGES) {
       c_slot = 0;
       c_parity ^= 1u;
+    }
+  }
+  if constexpr (JOIN) {
+    // o = sum_w l_w 2^(m_w - M) o_w / L, L = sum_w l_w 2^(m_w - M), M the largest m_w;
+    // the first runs.workers warps have parts. An empty sequence has none: zeros.
+    float2* total = reinterpret_cast<float2*>(smem + C::PREFIX_OFF);  // M and 1 / L per head
+    const int kvh = static_cast<int>(blockIdx.x) - my_b * p.hkv;
+    const int parts = static_cast<int>(runs.workers);
+    __syncthreads();
+    for (int x = threadIdx.x; x < p.group * (D / 2); x += C::THREADS) {
+      const int head = x / (D / 2), col = 2 * (x % (D / 2));
+      const uint8_t* ml = smem + C::ML_OFF + head * 8;
+      float big = -INFINITY;
+      for (int w = 0; w < parts; ++w)
+        big = fmaxf(big, *reinterpret_cast<const float*>(ml + w * C::RING));
+      float den = 0.f, n0 = 0.f, n1 = 0.f;
+      for (int w = 0; w < parts; ++w) {
+        const float2 mw = *reinterpret_cast<const float2*>(ml + w * C::RING);
+        const float2 o = *reinterpret_cast<const float2*>(smem + w * C::RING + (head * D + col) * 4);
+        const float e = mw.y * fast_exp2(mw.x - big);
+        den += e;
+        n0 = fmaf(e, o.x, n0);
+        n1 = fmaf(e, o.y, n1);
+      }
+      const float inv = parts == 0 ? 0.f : 1.f / den;
+      if (SCORED && col == 0) total[head] = make_float2(big, inv);
+      *reinterpret_cast<uint32_t*>(static_cast<T*>(p.out) +
+                                   (static_cast<size_t>(my_b) * p.hq + kvh * p.group + head) * D +
+                                   col) = pack2<T>(n0 * inv, n1 * inv);
+    }
+    if constexpr (SCORED) {
+      // Each token's weight, summed over the heads, to its slot's total.
+      __syncthreads();
+      const float* row = p.scores + static_cast<size_t>(blockIdx.x) * p.max_ctx * p.gp;
+      for (int t = threadIdx.x; t < my_len; t += C::THREADS) {
+        float w = 0.f;
+        for (int g = 0; g < p.group; ++g)
+          w = fmaf(fast_exp2(row[t * p.gp + g] - total[g].x), total[g].y, w);
+        const int in = p.by_bs.quotient(t);
+        const int page = p.bt[static_cast<size_t>(my_b) * p.max_blocks + in];
+        // A page outside the cache was reported where its rows were to be read.
+        if (static_cast<unsigned>(page) < static_cast<unsigned>(p.num_blocks))
+          atomicAdd(p.weights + (static_cast<size_t>(page) * p.hkv + kvh) * p.bs + (t - in * p.bs),
+                    w);
+      }
     }
   }
 }
@@ -734,10 +812,10 @@ Workspace carve(void* base, int64_t batch, int64_t hq, int64_t hkv, int64_t d, s
   return w;
 }
 
-template <int D, typename T, bool SCORED>
+template <int D, typename T, bool SCORED, bool JOIN>
 cudaError_t launch_kernel(const Kv4DecParams& p, int grid, const LaunchCtx& ctx) {
   using C = Kv4Cfg<D>;
-  auto kern = kv4_decode_kernel<D, T, SCORED>;
+  auto kern = kv4_decode_kernel<D, T, SCORED, JOIN>;
   static SmemLimit limit;
   cudaError_t e = allow_smem(kern, C::SMEM, limit);
   if (e != cudaSuccess) return e;
@@ -746,9 +824,12 @@ cudaError_t launch_kernel(const Kv4DecParams& p, int grid, const LaunchCtx& ctx)
 }
 
 template <int D, typename T>
-cudaError_t dispatch(const Kv4DecParams& p, int grid, const LaunchCtx& ctx) {
-  return p.scores != nullptr ? launch_kernel<D, T, true>(p, grid, ctx)
-                             : launch_kernel<D, T, false>(p, grid, ctx);
+cudaError_t dispatch(const Kv4DecParams& p, int grid, bool join, const LaunchCtx& ctx) {
+  if (join)
+    return p.scores != nullptr ? launch_kernel<D, T, true, true>(p, grid, ctx)
+                               : launch_kernel<D, T, false, true>(p, grid, ctx);
+  return p.scores != nullptr ? launch_kernel<D, T, true, false>(p, grid, ctx)
+                             : launch_kernel<D, T, false, false>(p, grid, ctx);
 }
 
 }  // namespace
@@ -784,6 +865,8 @@ cudaError_t launch_kv4_decode(const Kv4DecodeArgs& a, const LaunchCtx& ctx) {
     p.first = w.first;
     p.gp = static_cast<int>(score_heads(group));
     p.scores = scored ? w.scores : nullptr;
+    p.weights = a.weights;
+    p.by_bs = FastDiv(a.bs);
     p.status = ctx.status;
     p.timeout_ns = ctx.timeout_ns;
     p.block_stride = static_cast<unsigned int>(a.hkv * a.bs * row_bytes);
@@ -796,16 +879,27 @@ cudaError_t launch_kv4_decode(const Kv4DecodeArgs& a, const LaunchCtx& ctx) {
     p.num_blocks = static_cast<int>(a.num_blocks);
     p.max_ctx = static_cast<int>(a.max_ctx);
     p.scale_log2 = a.scale * kLog2e;
-    // One CTA per SM, or one per stage when there cannot be that many.
-    const int64_t stages = nb * a.hkv * ((a.max_ctx + tok - 1) / tok);
+    // One CTA per SM, or one per stage when there cannot be that many; or one per row
+    // (JOIN), in one launch, where that makes no warp's chain of stages longer: no more
+    // rows than SMs, at most two stages a warp and no more than equal runs over all
+    // resident warps would give. (Equal runs and finish / JOIN, us, 8 kv heads of 4 query
+    // heads, head_dim 128: 1 x 64 tokens 7.4 / 4.6, 8 x 200 9.0 / 5.6, 18 x 576
+    // 11.3 / 7.7, 18 x 1152 14.7 / 10.8, with weights 16.5 / 13.1; outside the rule
+    // 1 x 1152 8.8 / 9.6, 8 x 2304 14.1 / 15.3, 24 x 576 12.8 / 13.8.)
+    const int64_t row_stages = (a.max_ctx + tok - 1) / tok, stages = nb * a.hkv * row_stages;
+    const int64_t chain = (row_stages + warps - 1) / warps, resident = ctx.sm_count * warps;
+    const bool join = nb * a.hkv <= ctx.sm_count && chain <= 2 &&
+                      chain <= std::max<int64_t>(1, (stages + resident - 1) / resident);
     const int grid = static_cast<int>(
-        std::min<int64_t>(std::min<int64_t>(ctx.sm_count, kMaxWorkers / warps), stages));
+        join ? nb * a.hkv
+             : std::min<int64_t>(std::min<int64_t>(ctx.sm_count, kMaxWorkers / warps), stages));
     cudaError_t e;
     if (a.d == 64)
-      e = a.bf16 ? dispatch<64, __nv_bfloat16>(p, grid, ctx) : dispatch<64, __half>(p, grid, ctx);
+      e = a.bf16 ? dispatch<64, __nv_bfloat16>(p, grid, join, ctx) : dispatch<64, __half>(p, grid, join, ctx);
     else
-      e = a.bf16 ? dispatch<128, __nv_bfloat16>(p, grid, ctx) : dispatch<128, __half>(p, grid, ctx);
+      e = a.bf16 ? dispatch<128, __nv_bfloat16>(p, grid, join, ctx) : dispatch<128, __half>(p, grid, join, ctx);
     if (e != cudaSuccess) return e;
+    if (join) continue;
     FinishArgs f;
     f.o = w.o;
     f.m = w.m;

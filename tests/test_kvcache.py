@@ -369,6 +369,52 @@ def test_decode4_long_runs_of_small_pages(d, bs):
     ak.check_device_status()
 
 
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("group", [1, 3, 4, 8])
+@pytest.mark.parametrize("weights", [False, True])
+def test_decode4_short_rows_beside_a_long_one(d, group, weights):
+    """The lengths of test_decode4_lengths where a row is too long for one CTA: runs over all
+    warps, parts merged by the finish kernel."""
+    check_decode4(EDGES + [2500], 2 * group, 2, d, 16, seed=group, weights=weights)
+
+
+@pytest.mark.parametrize("d,most", [(64, 2048), (128, 1152)])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("weights", [False, True])
+def test_decode4_a_row_per_cta(d, most, dtype, weights):
+    """Up to two stages for each warp of a CTA, 144 rows; one token more is past that."""
+    lens = [most, most - 1, 0, 1, most // 2, most // 2 + 1, most // 2 - 1, 47, 48, 49, 64, 65,
+            most - 48, most - 65, 700, 333, most, 2]
+    check_decode4(lens, 16, 8, d, 16, dtype=dtype, weights=weights)
+    check_decode4(lens[1:] + [most + 1], 16, 8, d, 32, dtype=dtype, weights=weights)
+
+
+@pytest.mark.parametrize("n", [36, 37, 38])
+def test_decode4_about_a_row_per_sm(n):
+    """144, 148 and 152 rows."""
+    check_decode4([(37 * i) % 150 for i in range(n)], 12, 4, 128, 24, seed=n)
+
+
+def test_decode4_row_per_cta_at_empty_and_shared_pages():
+    """No tokens at all; and pages in several sequences, whose totals get every add."""
+    check_decode4([1, 0, 0], 4, 2, 64, 16, max_ctx=1)
+    q = torch.randn(2, 4, 128).half().cuda()
+    kc, vc, bt = cache4([200], 2, 128, 16)
+    kc, vc, bt = kc.cuda(), vc.cuda(), bt.cuda()
+    args = (q, kc, vc, bt.expand(2, -1).contiguous())
+    w = torch.zeros(kc.shape[:3], device="cuda")
+    zero = ak.paged_decode_kv4(*args, torch.tensor([0, 0]).cuda(), 200, weights=w)
+    assert (zero == 0).all() and (w == 0).all()
+    ak.paged_decode_kv4(*args, torch.tensor([200, 200]).cuda(), 200, weights=w)
+    each = torch.zeros_like(w)
+    for i in range(2):
+        ak.paged_decode_kv4(q[i:i + 1], kc, vc, bt, torch.tensor([200]).cuda(), 200, weights=each)
+    # Two fp32 adds to a total of at most 4, in either order: half a step of 2^-22 for each
+    # of the two sides' roundings.
+    assert (w - each).abs().max() <= 2.0 ** -22
+    assert abs(w.sum().item() - 8) < 8 * 200 * 2.0 ** -22 + 1e-4
+
+
 def test_decode4_cuts_lengths_above_max():
     kc, vc, bt = cache4([300], 2, 128, 16)
     q = torch.randn(1, 8, 128).half().cuda()
