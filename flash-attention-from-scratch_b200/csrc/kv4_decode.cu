@@ -65,8 +65,9 @@ struct Kv4Cfg {
   // 64 ragged sequences of up to 8192 tokens / 8 of 131072, 8 kv heads; one of 700):
   // 12 warps of 48 tokens 100 / 267, 8.9; 16 of 32 (128 registers, some spilled) 100 /
   // 268, 10.2; 8 of 64 106 / 292, 9.0. At 64 (64 x 8192, 64 query over 8 kv heads): 16
-  // warps of 64 tokens 66, 12 70, 8 78. (Before the centring product was one per group:
-  // the 12 of 48 are at 97 / 263, 8.8 with it, the 16 of 64 at 65.)
+  // warps of 64 tokens 66, 12 70, 8 78. (Before the centring product was one per group and
+  // the parts of few rows were merged by more warps: the 12 of 48 are at 96 / 259, 8.2
+  // with that, the 16 of 64 at 64.)
   static constexpr int W = D == 64 ? 16 : 12;
   static constexpr int THREADS = W * 32;
   static constexpr int NG = R::NG;

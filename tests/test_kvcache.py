@@ -323,6 +323,28 @@ def test_decode4_many_sequences():
         assert ((got - o).abs() < 1e-2)[~o.isnan()].all(), b
 
 
+@pytest.mark.parametrize("weights", [False, True])
+def test_decode4_few_sequences_behind_a_full_launch(weights):
+    """2048 sequences and 52 more: the same as two calls."""
+    torch.manual_seed(3)
+    n, bs = 2100, 16
+    kc, vc = (ora.pack(torch.randn(n, 2, bs, 64).half(), v).cuda() for v in (False, True))
+    bt = torch.randperm(n).to(torch.int32).view(n, 1).cuda()
+    lens = torch.randint(0, 17, (n,), dtype=torch.int32).cuda()
+    q = torch.randn(n, 6, 64).half().cuda()
+    w, w2 = (torch.zeros(kc.shape[:3], device="cuda") for _ in range(2))
+    out = ak.paged_decode_kv4(q, kc, vc, bt, lens, 16, weights=w if weights else None)
+    for part in (slice(0, 2048), slice(2048, n)):
+        got = ak.paged_decode_kv4(q[part], kc, vc, bt[part], lens[part], 16,
+                                  weights=w2 if weights else None)
+        assert torch.equal(out[part], got)
+    assert torch.equal(w, w2)  # one add per slot
+    if weights:
+        # Of each sequence 3 heads' weights sum to 3 per kv head.
+        sums = w.sum(-1)[bt[:, 0].long()]
+        assert (sums - torch.where(lens > 0, 3.0, 0.0)[:, None]).abs().max() < 1e-4
+
+
 def test_weights_of_many_sequences():
     """Totals over more sequences than a launch takes, every page in one sequence."""
     torch.manual_seed(2)
