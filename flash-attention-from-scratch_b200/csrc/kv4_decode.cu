@@ -40,6 +40,14 @@
 //     tokens off by 0.8 %, from the tensor cores' rounding of the large sums alone.)
 //     P is two fp16 terms, P scale one, rounded once from both: the one rounding of
 //     a token's weight, like P's in fp16 attention.
+//   * P is held times 2^up, up = 14 - floor(log2(max(1, S))) with S the largest scale of V
+//     that the warp has met in the row: P scale stays below 2^15, and has fp16's 11 bits
+//     down to P scale = 2^-28 max(1, S). With a fixed factor of 4 the small weights'
+//     products with small scales were below fp16's range: for V of 1e-4, 32768 tokens and
+//     scores of deviation 2 the RMS error at bf16 output was 4.3 to 5 times that of the
+//     roundings named here. `up` only falls, once or twice a row, and the sums so far with
+//     it, by the factor that makes them follow the running maximum. (64 x 8192 at head_dim
+//     128: 96.7 -> 99.1 us, 8 x 131072: 261 -> 264; 64 x 8192 at 64: 64.7.)
 //   * q of a head is scaled by the power of two that brings its largest value into
 //     [2^7, 2^8), so that fp16 holds every bit that matters of an fp16 or bf16 q.
 #include <algorithm>
@@ -65,9 +73,9 @@ struct Kv4Cfg {
   // 64 ragged sequences of up to 8192 tokens / 8 of 131072, 8 kv heads; one of 700):
   // 12 warps of 48 tokens 100 / 267, 8.9; 16 of 32 (128 registers, some spilled) 100 /
   // 268, 10.2; 8 of 64 106 / 292, 9.0. At 64 (64 x 8192, 64 query over 8 kv heads): 16
-  // warps of 64 tokens 66, 12 70, 8 78. (Before the centring product was one per group and
-  // the parts of few rows were merged by more warps: the 12 of 48 are at 96 / 259, 8.2
-  // with that, the 16 of 64 at 64.)
+  // warps of 64 tokens 66, 12 70, 8 78. (Before the centring product was one per group,
+  // the parts of few rows were merged by more warps and P was held by V's scales: the 12
+  // of 48 are at 99 / 264, 8.2 with that, the 16 of 64 at 64.)
   static constexpr int W = D == 64 ? 16 : 12;
   static constexpr int THREADS = W * 32;
   static constexpr int NG = R::NG;
@@ -389,7 +397,8 @@ __global__ void __launch_bounds__(Kv4Cfg<D>::THREADS, 1) kv4_decode_kernel(const
   uint32_t qf[NG][4];  // b0, b1 of the codes in bits 0-3, then of those in bits 4-7
   uint32_t qs[2];      // B of the lows' product: the groups' sums of q
   float f[2];          // scale * log2(e) over q's power of two, per head
-  float m[2], l[2];    // running maximum; this lane's share of the sum, times 4
+  float m[2], l[2];    // running maximum; this lane's share of the sum, times 2^up
+  int up = 14;         // P is held times 2^up
   float acc[NG][2][4], z[4];
   float* sc = nullptr;  // SCORED: the scores of the stage's first token
   const int tok_k = (g4 & 1) ? ((g4 + 3) & 7) + 8 : g4;  // tau(g4)
@@ -461,6 +470,7 @@ __global__ void __launch_bounds__(Kv4Cfg<D>::THREADS, 1) kv4_decode_kernel(const
     const int nt = md.w & kTokens;
     if (md.w & kFirst) {
       load_q(md.x, md.y);
+      up = 14;
       m[0] = m[1] = -INFINITY;
       l[0] = l[1] = 0.f;
 #pragma unroll
@@ -475,6 +485,30 @@ __global__ void __launch_bounds__(Kv4Cfg<D>::THREADS, 1) kv4_decode_kernel(const
     const bool ok = mbar_wait(full + c_slot, c_parity, abort_flag, p.status, kSiteKv4Wait,
                               p.timeout_ns);
     if (!__all_sync(0xffffffffu, ok)) return false;
+
+    // The exponent of the largest scale of V in the stage, at least 1's. (A NaN scale is
+    // passed over: its own columns are NaN whatever the others are multiplied by.)
+    float less;  // what `up` goes down by, negative
+    {
+      __half2 top = __half2half2(__ushort_as_half(0));
+#pragma unroll
+      for (int r0 = 0; r0 < kTok; r0 += 32) {
+        if (r0 + lane < nt) {
+          uint32_t par[NG / 2];
+          load_words<NG / 2>(par, vst + (r0 + lane) * ROW + CODES);
+#pragma unroll
+          for (int w = 0; w < NG / 2; ++w) {
+            const uint32_t size = par[w] & 0x7fff7fffu;
+            top = __hmax2(top, *reinterpret_cast<const __half2*>(&size));
+          }
+        }
+      }
+      const uint32_t bits = *reinterpret_cast<const uint32_t*>(&top);
+      const uint32_t big = __reduce_max_sync(0xffffffffu, max(bits & 0xffffu, bits >> 16));
+      const int now = min(up, 14 - (max(static_cast<int>(big >> 10), 15) - 15));
+      less = static_cast<float>(now - up);
+      up = now;
+    }
 
     // Scores of the stage's tokens: s[i][0..1] token 16 i + tok_k, s[i][2..3] the
     // token after it.
@@ -550,10 +584,8 @@ __global__ void __launch_bounds__(Kv4Cfg<D>::THREADS, 1) kv4_decode_kernel(const
           }
       }
     }
-    // Online softmax: per head the maximum over the 8 lanes of its scores. P is
-    // held times 4, which keeps small P * scale in fp16's normal range longer and
-    // cannot overflow (a scale is at most 8734).
-    float alpha[2], shift[2];  // shift: 2 - m
+    // Online softmax: per head the maximum over the 8 lanes of its scores.
+    float alpha[2], shift[2];  // shift: up - m
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       float mx = fmaxf(s[0][h], s[0][h + 2]);
@@ -563,9 +595,9 @@ __global__ void __launch_bounds__(Kv4Cfg<D>::THREADS, 1) kv4_decode_kernel(const
       mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
       mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
       mx = fmaxf(mx, m[h]);
-      alpha[h] = fast_exp2(m[h] - mx);
+      alpha[h] = fast_exp2(m[h] - mx + less);
       m[h] = mx;
-      shift[h] = 2.f - mx;
+      shift[h] = static_cast<float>(up) - mx;
     }
     // P^T as B fragments: tokens of rows 2 t4, 2 t4 + 1 (+ 8), head g4; and what rounding
     // it to fp16 left over.
@@ -704,10 +736,10 @@ __global__ void __launch_bounds__(Kv4Cfg<D>::THREADS, 1) kv4_decode_kernel(const
         const float mh = l[h] != l[h] ? fmaxf(m[h], 0.f) : m[h];
         if constexpr (JOIN) {
           if (g4 == 0)
-            *reinterpret_cast<float2*>(ring + C::ML_OFF + head * 8) = make_float2(mh, 0.25f * l[h]);
+            *reinterpret_cast<float2*>(ring + C::ML_OFF + head * 8) = make_float2(mh, pow2i(-up) * l[h]);
         } else if (head < p.group && g4 == 0 && (SCORED || !(md.w & kWhole))) {
           p.m_part[pr] = mh;
-          p.l_part[pr] = 0.25f * l[h];
+          p.l_part[pr] = pow2i(-up) * l[h];
         }
       }
     }
