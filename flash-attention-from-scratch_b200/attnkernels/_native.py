@@ -118,15 +118,19 @@ def _raw_stream(idx: int):
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", _raw_stream)
 
 
+def _index(device: torch.device) -> int:
+    return device.index if device.index is not None else torch.cuda.current_device()
+
+
 def _stream(device: torch.device):
     """The current CUDA stream of `device` as an integer handle."""
-    return _raw_stream(device.index if device.index is not None else torch.cuda.current_device())
+    return _raw_stream(_index(device))
 
 
 def _on(device: torch.device):
     """Make `device` current for the call (the C ABI works on the current device);
     no device switch when it already is."""
-    idx = device.index if device.index is not None else torch.cuda.current_device()
+    idx = _index(device)
     if torch.cuda.current_device() == idx:
         return contextlib.nullcontext()
     return torch.cuda.device(idx)
@@ -165,7 +169,7 @@ class _StreamWorkspaces:
         self.launching = threading.RLock()
 
     def get(self, nbytes: int, device: torch.device, stream: int) -> torch.Tensor:
-        key = (device.index if device.index is not None else torch.cuda.current_device(), stream)
+        key = (_index(device), stream)
         buf = self._bufs.get(key)
         if buf is None or buf.numel() < nbytes:
             with self._lock:
@@ -179,28 +183,27 @@ class _StreamWorkspaces:
         """The buffer of (device, stream), or None."""
         return self._bufs.get((dev, stream))
 
+    def scratch(self, nbytes: int, dev: int, stream: int) -> torch.Tensor:
+        """The stream's kept buffer, or, while a graph is captured, scratch of the
+        capture's own: a graph must not hold an address that a later call or clear()
+        may give back, nor share it with another graph, and what a capture allocates
+        is the graph's."""
+        if torch.cuda.is_current_stream_capturing():
+            return _workspace(nbytes, torch.device("cuda", dev))
+        buf = self.kept(dev, stream)
+        if buf is not None and buf.numel() >= nbytes:
+            return buf
+        return self.get(nbytes, torch.device("cuda", dev), stream)
+
     def clear(self) -> None:
         with self._lock:
             self._bufs.clear()
 
 
 _decode_ws = _StreamWorkspaces()
-# Of the 4-bit decode and the decode with weights. Not the same buffers: a captured
-# paged_decode replays on the buffer that it was captured with, which another
-# operator's larger call must not replace.
+# Of the 4-bit decode and the decode with weights. Not the same buffers: theirs grow
+# by the scores of every token, which a paged_decode on the stream has no use for.
 _cache_ws = _StreamWorkspaces()
-
-
-def _call_workspace(nbytes: int, dev: int, stream: int) -> torch.Tensor:
-    """The stream's kept scratch, or, while a graph is captured, scratch of the
-    capture's own: a graph must not hold an address that a later call may give
-    back, nor share it with another graph."""
-    if torch.cuda.is_current_stream_capturing():
-        return _workspace(nbytes, torch.device("cuda", dev))
-    buf = _cache_ws.kept(dev, stream)
-    if buf is not None and buf.numel() >= nbytes:
-        return buf
-    return _cache_ws.get(nbytes, torch.device("cuda", dev), stream)
 
 
 @functools.lru_cache(maxsize=4096)
@@ -257,9 +260,9 @@ class Extension:
         B, H, Hkv, D, bs, nblk, maxb = self._decode_sizes(q, kc, bt)
         with _on(q.device), _decode_ws.launching:
             stream = _stream(q.device)
-            ws = _decode_ws.get(
+            ws = _decode_ws.scratch(
                 self.lib.attn_paged_decode_workspace_bytes(B, H, D, max_ctx, partition),
-                q.device, stream)
+                _index(q.device), stream)
             _check(self.lib.attn_paged_decode(
                 _ptr(q), _ptr(kc), _ptr(vc), _ptr(bt), _ptr(ctx), _ptr(out), B, H, Hkv, D, bs,
                 nblk, maxb, int(max_ctx), float(scale), int(partition), _ptr(ws), ws.numel(),
@@ -275,9 +278,9 @@ class Extension:
         l = torch.empty(B, H, **f32) if l is None else l
         with _on(q.device), _decode_ws.launching:
             stream = _stream(q.device)
-            ws = _decode_ws.get(
+            ws = _decode_ws.scratch(
                 self.lib.attn_paged_decode_workspace_bytes(B, H, D, max_ctx, partition),
-                q.device, stream)
+                _index(q.device), stream)
             _check(self.lib.attn_paged_decode_partials(
                 _ptr(q), _ptr(kc), _ptr(vc), _ptr(bt), _ptr(ctx), _ptr(o), _ptr(m), _ptr(l), B, H,
                 Hkv, D, bs, nblk, maxb, int(max_ctx), float(scale), int(partition), _ptr(ws),
@@ -317,7 +320,7 @@ class Extension:
         nbytes = _workspace_bytes("attn_paged_decode_weights_workspace_bytes", B, H, Hkv, D,
                                   max_ctx, partition)
         with _cache_ws.launching:
-            ws = _call_workspace(nbytes, dev, stream)
+            ws = _cache_ws.scratch(nbytes, dev, stream)
             _call(dev, self.lib.attn_paged_decode_weights, q.data_ptr(), kc.data_ptr(),
                   vc.data_ptr(), bt.data_ptr(), ctx.data_ptr(), out.data_ptr(),
                   weights.data_ptr(), *sizes, max_ctx, scale, partition, ws.data_ptr(),
@@ -347,7 +350,7 @@ class Extension:
         nbytes = _workspace_bytes("attn_kv4_decode_workspace_bytes", B, H, Hkv, D, max_ctx,
                                   0 if weights is None else 1)
         with _cache_ws.launching:
-            ws = _call_workspace(nbytes, dev, stream)
+            ws = _cache_ws.scratch(nbytes, dev, stream)
             _call(dev, self.lib.attn_kv4_decode, q.data_ptr(), _DTYPES[q.dtype], kc.data_ptr(),
                   vc.data_ptr(), bt.data_ptr(), ctx.data_ptr(), out.data_ptr(),
                   None if weights is None else weights.data_ptr(), *sizes, max_ctx, scale,

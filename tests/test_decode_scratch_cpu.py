@@ -1,0 +1,82 @@
+"""Which scratch the decode calls take, on CPU with a library that only looks at its arguments:
+while a graph is captured scratch of the capture's own, otherwise the stream's kept buffer."""
+import pytest
+import torch
+
+import attnkernels as ak
+from attnkernels import _native
+
+CALLS = ["paged_decode", "paged_decode_partials", "paged_decode_weights", "kv4_decode"]
+
+
+class Library:
+    """The decode entry points: each notes the address of its workspace."""
+
+    def __init__(self):
+        self.seen = []
+
+    def _decode(self, *args):
+        self.seen.append(args[-3])
+        return 0
+
+    attn_paged_decode = attn_paged_decode_partials = _decode
+    attn_paged_decode_weights = attn_kv4_decode = _decode
+
+    @staticmethod
+    def attn_paged_decode_workspace_bytes(*sizes):
+        return 1 << 16
+
+
+@pytest.fixture
+def ext(monkeypatch):
+    e = _native.Extension.__new__(_native.Extension)
+    e.lib = Library()
+    e.stream, e.capturing, e.made = 0, False, []
+
+    def workspace(nbytes, device):
+        # Held on to, so that no two have one address.
+        e.made.append(torch.empty(max(nbytes, 256), dtype=torch.uint8))
+        return e.made[-1]
+
+    monkeypatch.setattr(_native, "_raw_stream", lambda dev: e.stream)
+    monkeypatch.setattr(_native, "_workspace", workspace)
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: e.capturing)
+    ak.release_workspaces()
+    yield e
+    ak.release_workspaces()
+
+
+def call(e, name):
+    q = torch.zeros(1, 8, 64, dtype=torch.float16)
+    kc = torch.zeros(1, 8, 16, 64, dtype=torch.float16)
+    t, w, sizes = torch.zeros(1, 1, dtype=torch.int32), torch.zeros(1, 8, 16), (1, 8, 8, 64, 16, 1, 1)
+    if name.startswith("paged_decode") and name != "paged_decode_weights":
+        getattr(e, name)(q, kc, kc, t, t[0], 16, 1.0, 256)
+    elif name == "kv4_decode":
+        e.kv4_decode(0, q, kc, kc, t, t[0], None, sizes, 16, 1.0)
+    else:
+        e.paged_decode_weights(0, q, kc, kc, t, t[0], w, sizes, 16, 1.0, 256)
+    return e.lib.seen[-1]
+
+
+@pytest.mark.parametrize("name", CALLS)
+def test_a_capture_has_scratch_of_its_own(ext, name):
+    """The kept buffer is given back by a larger call or release_workspaces(), and two graphs
+    captured on one stream may replay at the same time: neither may hold it."""
+    kept = call(ext, name)
+    assert call(ext, name) == kept
+    ext.capturing = True
+    first, second = call(ext, name), call(ext, name)
+    assert len({kept, first, second}) == 3
+    ext.capturing = False
+    assert call(ext, name) == kept
+
+
+@pytest.mark.parametrize("name", CALLS)
+def test_a_capture_keeps_nothing_for_later_calls(ext, name):
+    """Scratch from a graph's private pool is the graph's: no eager call may use it."""
+    ext.capturing = True
+    captured = call(ext, name)
+    ext.capturing = False
+    assert call(ext, name) != captured
