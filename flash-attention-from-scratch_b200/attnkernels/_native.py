@@ -159,14 +159,15 @@ class _StreamWorkspaces:
     allocated while its stream is current, so the caching allocator never hands
     its memory to another stream while a kernel may still use it.
 
-    A call holds `launching` from taking the buffer to its last launch: library
-    calls run without the GIL, and a second thread's launches on the same stream
-    must not come between the launch that fills the buffer and the one that reads it."""
+    A call holds its stream's `launching` from taking the buffer to its last launch:
+    library calls run without the GIL, and a second thread's launches on the same stream
+    must not come between the launch that fills the buffer and the one that reads it.
+    Calls on other streams have other buffers and do not wait."""
 
     def __init__(self):
         self._bufs: dict[tuple[int, int], torch.Tensor] = {}
         self._lock = threading.Lock()
-        self.launching = threading.RLock()
+        self._launching: dict[tuple[int, int], threading.RLock] = {}
 
     def get(self, nbytes: int, device: torch.device, stream: int) -> torch.Tensor:
         key = (_index(device), stream)
@@ -178,6 +179,13 @@ class _StreamWorkspaces:
                     buf = _workspace(max(int(nbytes), 1 << 20), device)
                     self._bufs[key] = buf
         return buf
+
+    def launching(self, dev: int, stream: int):
+        """The lock of (device, stream), which lives on when clear() drops the buffer."""
+        key = (dev, stream)
+        lock = self._launching.get(key)
+        # setdefault() is one step: of two threads both get the first one's lock.
+        return lock if lock is not None else self._launching.setdefault(key, threading.RLock())
 
     def kept(self, dev: int, stream: int):
         """The buffer of (device, stream), or None."""
@@ -258,11 +266,12 @@ class Extension:
     def paged_decode(self, q, kc, vc, bt, ctx, max_ctx, scale, partition):
         out = torch.empty_like(q)
         B, H, Hkv, D, bs, nblk, maxb = self._decode_sizes(q, kc, bt)
-        with _on(q.device), _decode_ws.launching:
-            stream = _stream(q.device)
+        dev = _index(q.device)
+        stream = _raw_stream(dev)
+        with _on(q.device), _decode_ws.launching(dev, stream):
             ws = _decode_ws.scratch(
                 self.lib.attn_paged_decode_workspace_bytes(B, H, D, max_ctx, partition),
-                _index(q.device), stream)
+                dev, stream)
             _check(self.lib.attn_paged_decode(
                 _ptr(q), _ptr(kc), _ptr(vc), _ptr(bt), _ptr(ctx), _ptr(out), B, H, Hkv, D, bs,
                 nblk, maxb, int(max_ctx), float(scale), int(partition), _ptr(ws), ws.numel(),
@@ -276,11 +285,12 @@ class Extension:
         o = torch.empty(B, H, D, **f32) if o is None else o
         m = torch.empty(B, H, **f32) if m is None else m
         l = torch.empty(B, H, **f32) if l is None else l
-        with _on(q.device), _decode_ws.launching:
-            stream = _stream(q.device)
+        dev = _index(q.device)
+        stream = _raw_stream(dev)
+        with _on(q.device), _decode_ws.launching(dev, stream):
             ws = _decode_ws.scratch(
                 self.lib.attn_paged_decode_workspace_bytes(B, H, D, max_ctx, partition),
-                _index(q.device), stream)
+                dev, stream)
             _check(self.lib.attn_paged_decode_partials(
                 _ptr(q), _ptr(kc), _ptr(vc), _ptr(bt), _ptr(ctx), _ptr(o), _ptr(m), _ptr(l), B, H,
                 Hkv, D, bs, nblk, maxb, int(max_ctx), float(scale), int(partition), _ptr(ws),
@@ -319,7 +329,7 @@ class Extension:
         stream = _raw_stream(dev)
         nbytes = _workspace_bytes("attn_paged_decode_weights_workspace_bytes", B, H, Hkv, D,
                                   max_ctx, partition)
-        with _cache_ws.launching:
+        with _cache_ws.launching(dev, stream):
             ws = _cache_ws.scratch(nbytes, dev, stream)
             _call(dev, self.lib.attn_paged_decode_weights, q.data_ptr(), kc.data_ptr(),
                   vc.data_ptr(), bt.data_ptr(), ctx.data_ptr(), out.data_ptr(),
@@ -349,7 +359,7 @@ class Extension:
         stream = _raw_stream(dev)
         nbytes = _workspace_bytes("attn_kv4_decode_workspace_bytes", B, H, Hkv, D, max_ctx,
                                   0 if weights is None else 1)
-        with _cache_ws.launching:
+        with _cache_ws.launching(dev, stream):
             ws = _cache_ws.scratch(nbytes, dev, stream)
             _call(dev, self.lib.attn_kv4_decode, q.data_ptr(), _DTYPES[q.dtype], kc.data_ptr(),
                   vc.data_ptr(), bt.data_ptr(), ctx.data_ptr(), out.data_ptr(),

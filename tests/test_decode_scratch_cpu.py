@@ -1,5 +1,8 @@
 """Which scratch the decode calls take, on CPU with a library that only looks at its arguments:
 while a graph is captured scratch of the capture's own, otherwise the stream's kept buffer."""
+import threading
+import types
+
 import pytest
 import torch
 
@@ -80,3 +83,41 @@ def test_a_capture_keeps_nothing_for_later_calls(ext, name):
     captured = call(ext, name)
     ext.capturing = False
     assert call(ext, name) != captured
+
+
+@pytest.mark.parametrize("name", CALLS)
+@pytest.mark.parametrize("same", [False, True])
+def test_calls_wait_for_their_own_stream_alone(ext, monkeypatch, name, same):
+    """A launch that blocks (a full queue) holds back calls that share its scratch, and no call
+    on another stream."""
+    stream = threading.local()
+    monkeypatch.setattr(_native, "_raw_stream", lambda dev: stream.handle)
+    inside, leave, other = threading.Event(), threading.Event(), threading.Event()
+
+    def decode(*args):
+        if args[-1] == 1 and not inside.is_set():
+            inside.set()
+            leave.wait(20)
+        return 0
+
+    def run(handle, done=None):
+        stream.handle = handle
+        call(ext, name)
+        if done is not None:
+            done.set()
+
+    monkeypatch.setattr(ext, "lib", types.SimpleNamespace(
+        seen=[0], attn_paged_decode_workspace_bytes=Library.attn_paged_decode_workspace_bytes,
+        **{"attn_" + n: decode for n in CALLS}))
+    first = threading.Thread(target=run, args=(1,))
+    second = threading.Thread(target=run, args=(1 if same else 2, other))
+    first.start()
+    assert inside.wait(20)
+    second.start()
+    try:
+        assert other.wait(0.3 if same else 10) != same
+    finally:
+        leave.set()
+        first.join()
+        second.join()
+    assert other.is_set()
