@@ -136,6 +136,15 @@ def _on(device: torch.device):
     return torch.cuda.device(idx)
 
 
+def _capturing(dev: int) -> bool:
+    """Whether the current stream of device `dev` is being captured (torch asks the
+    current device's)."""
+    if torch.cuda.current_device() == dev:
+        return torch.cuda.is_current_stream_capturing()
+    with torch.cuda.device(dev):
+        return torch.cuda.is_current_stream_capturing()
+
+
 def _call(dev: int, fn, *args) -> None:
     """A library call with device `dev` current."""
     if torch.cuda.current_device() == dev:
@@ -196,7 +205,7 @@ class _StreamWorkspaces:
         capture's own: a graph must not hold an address that a later call or clear()
         may give back, nor share it with another graph, and what a capture allocates
         is the graph's."""
-        if torch.cuda.is_current_stream_capturing():
+        if _capturing(dev):
             return _workspace(nbytes, torch.device("cuda", dev))
         buf = self.kept(dev, stream)
         if buf is not None and buf.numel() >= nbytes:

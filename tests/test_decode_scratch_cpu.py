@@ -1,5 +1,6 @@
 """Which scratch the decode calls take, on CPU with a library that only looks at its arguments:
 while a graph is captured scratch of the capture's own, otherwise the stream's kept buffer."""
+import contextlib
 import threading
 import types
 
@@ -50,16 +51,16 @@ def ext(monkeypatch):
     ak.release_workspaces()
 
 
-def call(e, name):
+def call(e, name, dev=0):
     q = torch.zeros(1, 8, 64, dtype=torch.float16)
     kc = torch.zeros(1, 8, 16, 64, dtype=torch.float16)
     t, w, sizes = torch.zeros(1, 1, dtype=torch.int32), torch.zeros(1, 8, 16), (1, 8, 8, 64, 16, 1, 1)
     if name.startswith("paged_decode") and name != "paged_decode_weights":
         getattr(e, name)(q, kc, kc, t, t[0], 16, 1.0, 256)
     elif name == "kv4_decode":
-        e.kv4_decode(0, q, kc, kc, t, t[0], None, sizes, 16, 1.0)
+        e.kv4_decode(dev, q, kc, kc, t, t[0], None, sizes, 16, 1.0)
     else:
-        e.paged_decode_weights(0, q, kc, kc, t, t[0], w, sizes, 16, 1.0, 256)
+        e.paged_decode_weights(dev, q, kc, kc, t, t[0], w, sizes, 16, 1.0, 256)
     return e.lib.seen[-1]
 
 
@@ -121,3 +122,24 @@ def test_calls_wait_for_their_own_stream_alone(ext, monkeypatch, name, same):
         first.join()
         second.join()
     assert other.is_set()
+
+
+@pytest.mark.parametrize("capturing", [0, 1])
+@pytest.mark.parametrize("name", ["paged_decode_weights", "kv4_decode"])
+def test_the_capture_that_counts_is_the_tensors_device(ext, monkeypatch, name, capturing):
+    """Tensors on device 1, device 0 current: device 1's stream is asked, not device 0's."""
+    at = [0]
+
+    @contextlib.contextmanager
+    def device(index):
+        before, at[0] = at[0], index
+        yield
+        at[0] = before
+
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: at[0])
+    monkeypatch.setattr(torch.cuda, "device", device)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    kept = call(ext, name, dev=1)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: at[0] == capturing)
+    assert (call(ext, name, dev=1) == kept) == (capturing == 0)
+    assert at == [0]
