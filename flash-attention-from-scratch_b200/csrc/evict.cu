@@ -87,7 +87,9 @@ __global__ void __launch_bounds__(T) evict_select_kernel(const SelectParams p) {
   const int at = rank * T + tid, step = ranks * T;
   if (kvh == 0 && at == 0) p.new_lens[b] = min(len, p.keep);
   if (len <= p.keep) {  // the whole cluster alike
-    for (int j = at; j < p.keep; j += step) kept[j] = j < len ? j : -1;
+    // Unsigned: keep may be 2^31 - 1, past which j goes once more.
+    for (unsigned int j = at; j < static_cast<unsigned int>(p.keep); j += step)
+      kept[j] = j < static_cast<unsigned int>(len) ? static_cast<int>(j) : -1;
     return;
   }
   const int first = p.sinks, last = len - p.recent;  // candidates [first, last)
