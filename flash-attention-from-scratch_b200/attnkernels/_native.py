@@ -279,7 +279,7 @@ class Extension:
         stream = _raw_stream(dev)
         with _on(q.device), _decode_ws.launching(dev, stream):
             ws = _decode_ws.scratch(
-                self.lib.attn_paged_decode_workspace_bytes(B, H, D, max_ctx, partition),
+                _workspace_bytes("attn_paged_decode_workspace_bytes", B, H, D, max_ctx, partition),
                 dev, stream)
             _check(self.lib.attn_paged_decode(
                 _ptr(q), _ptr(kc), _ptr(vc), _ptr(bt), _ptr(ctx), _ptr(out), B, H, Hkv, D, bs,
@@ -298,7 +298,7 @@ class Extension:
         stream = _raw_stream(dev)
         with _on(q.device), _decode_ws.launching(dev, stream):
             ws = _decode_ws.scratch(
-                self.lib.attn_paged_decode_workspace_bytes(B, H, D, max_ctx, partition),
+                _workspace_bytes("attn_paged_decode_workspace_bytes", B, H, D, max_ctx, partition),
                 dev, stream)
             _check(self.lib.attn_paged_decode_partials(
                 _ptr(q), _ptr(kc), _ptr(vc), _ptr(bt), _ptr(ctx), _ptr(o), _ptr(m), _ptr(l), B, H,
