@@ -632,7 +632,8 @@ int attn_kv4_decode(const void* q, int dtype, const void* k_cache, const void* v
       num_heads > 0x7fffffffLL || batch * num_heads > 0x7fffffffLL)
     return fail(ATTN_ERR_UNSUPPORTED,
                 "%s: sizes must fit in 31 bits (max_context_len <= 2^30, block_size <= 65536)", name);
-  // 32-token stages of a launch (up to 2048 sequences), counted in 31 bits.
+  // Stages of a launch (up to 2048 sequences) are counted in 31 bits; one has 48 tokens or
+  // 64, of which 32 is a lower bound.
   if ((batch < 2048 ? batch : 2048) * num_kv_heads * ((max_context_len + 31) / 32) > 0x7fffffffLL)
     return fail(ATTN_ERR_UNSUPPORTED,
                 "%s: 2^36 tokens of context times kv heads, or more, in 2048 sequences", name);

@@ -163,7 +163,7 @@ __device__ __forceinline__ float part_max(float m, float l) {
 }
 
 // SCORED: every token's score is written out too, for the totals of attention
-// weights (evict.cu): 4 G bytes beside the 4 D that a token's K and V take.
+// weights (finish.cu): 4 G bytes beside the 4 D that a token's K and V take.
 template <int D, int G, bool SCORED>
 __global__ void __launch_bounds__(DecCfg<D, G>::THREADS, 1) paged_decode_kernel(const DecParams p) {
   using C = DecCfg<D, G>;

@@ -36,7 +36,7 @@ struct FinishParams {
 };
 
 // The parts of one (sequence, kv head) pair: part s of query head g is at
-// base + s * stride + g * head. Set before the decode launch has ended: false.
+// base + s * stride + g * head. An empty sequence has none.
 struct Parts {
   long long base, stride, head;
   int count;

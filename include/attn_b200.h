@@ -225,8 +225,10 @@ int attn_paged_decode_noalloc(const void* q, const void* k_cache, const void* v_
 /* ------------------------------------------------- attention weights, eviction */
 
 /*
- * Bytes of workspace attn_paged_decode_weights needs: attn_paged_decode's, and
- * fp32 scores of num_heads / num_kv_heads per (sequence, kv head, token).
+ * Bytes of workspace attn_paged_decode_weights needs; ask here, it is not a fixed
+ * amount above attn_paged_decode's. Most of it is an fp32 score per (sequence,
+ * query head, token), for max_context_len tokens of every sequence however long
+ * they are: 64 sequences of 32 heads at 131072 take 1.07 GB.
  */
 size_t attn_paged_decode_weights_workspace_bytes(int64_t batch, int64_t num_heads,
                                                  int64_t num_kv_heads, int64_t head_dim,
@@ -240,8 +242,11 @@ size_t attn_paged_decode_weights_workspace_bytes(int64_t batch, int64_t num_head
  * Totals of other slots are left as they are. A page that stands in several
  * sequences gets the adds of all of them (in no fixed order, so that such a
  * total may differ in its last bits from call to call; with every page in one
- * sequence the totals are the same each time). Lengths above max_context_len
- * are cut to it. No counterpart in the reference.
+ * sequence the totals are the same each time). A slot that is given to a new token
+ * still has the old one's total until the caller zeroes it (attn_kv4_append does
+ * for a 4-bit cache). Lengths above max_context_len are cut to it. A sequence whose
+ * scores are all NaN gives NaN, where attn_paged_decode gives zeros if it has split
+ * the sequence. No counterpart in the reference.
  */
 int attn_paged_decode_weights(const void* q, const void* k_cache, const void* v_cache,
                               const int32_t* block_tables, const int32_t* context_lens, void* out,
@@ -317,14 +322,20 @@ int attn_kv4_append(const void* k, const void* v, int dtype, void* k_cache, void
 
 /*
  * Read slots back: k, v [tokens, num_kv_heads, head_dim] of `dtype`, dense;
- * value = low + scale * code, rounded once. A negative slot, or one past the
- * cache (reported as ATTN_DEVICE_BAD_BLOCK), reads as zeros.
+ * value = low + scale * code, rounded once to fp16; for bf16 rounded to fp32
+ * first. A negative slot, or one past the cache (reported as
+ * ATTN_DEVICE_BAD_BLOCK), reads as zeros.
  */
 int attn_kv4_read(const void* k_cache, const void* v_cache, const int64_t* slots, void* k, void* v,
                   int dtype, int64_t tokens, int64_t num_kv_heads, int64_t head_dim,
                   int64_t block_size, int64_t num_blocks, void* stream);
 
-/* Bytes of workspace attn_kv4_decode needs (with_weights: `weights` is given). */
+/*
+ * Bytes of workspace attn_kv4_decode needs. with_weights: `weights` is given; then
+ * most of it is fp32 scores, num_heads / num_kv_heads of them rounded up to a power
+ * of two per (sequence, kv head, token), for max_context_len tokens of every
+ * sequence, of up to 2048 sequences.
+ */
 size_t attn_kv4_decode_workspace_bytes(int64_t batch, int64_t num_heads, int64_t num_kv_heads,
                                        int64_t head_dim, int64_t max_context_len,
                                        int with_weights);
@@ -337,7 +348,13 @@ size_t attn_kv4_decode_workspace_bytes(int64_t batch, int64_t num_heads, int64_t
  * Lengths above max_context_len are cut to it; an empty sequence gets zeros.
  * The context is split over the GPU's resident warps in equal runs, whatever the
  * lengths, so there is no partition to choose; the outputs of one sequence differ
- * by rounding with the sequences beside it.
+ * by rounding with the sequences beside it. Whether a row is split at all goes by
+ * max_context_len: the longest length, where it is known, is the fastest bound.
+ * Beside the output's own rounding two roundings to fp16 count: each softmax weight
+ * times a V scale (11 bits down to 2^-28 of the largest weight times the row's
+ * largest scale, or times 1 where that is larger; fewer below), and the middle,
+ * low + 8 scale or low + 7 scale, of each V group. Scores, sums and the softmax are
+ * fp32.
  */
 int attn_kv4_decode(const void* q, int dtype, const void* k_cache, const void* v_cache,
                     const int32_t* block_tables, const int32_t* context_lens, void* out,
