@@ -233,8 +233,8 @@ def paged_decode_weights(q, k_cache, v_cache, block_tables, context_lens, max_co
              summed over the query heads of its kv head. Totals of slots that the sequences do not
              hold stay as they are. A page that several sequences share gets the adds of all. A
              slot that is given to a new token keeps the old one's total until it is zeroed:
-             weights[slots // block_size, :, slots % block_size] = 0
-             (paged_append_kv4 does that for a 4-bit cache).
+             weights[slots // block_size, :, slots % block_size] = 0, padding's negative
+             slots left out (paged_append_kv4 does that for a 4-bit cache).
     The other arguments and the result are paged_decode's; a length above max_context_len is cut
     to it. A sequence whose keys are all NaN gives NaN, where paged_decode gives zeros if it has
     split the sequence. The scratch holds an fp32 score per sequence, head and token up to

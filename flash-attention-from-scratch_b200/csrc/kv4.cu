@@ -187,8 +187,8 @@ __device__ __forceinline__ void append_row(uint8_t* dst, uint4 raw, bool real, i
 }
 
 // A lane takes its 8 values of K and of V of one (token, head): the slot and its
-// row in the cache are found once for both. Bound by the instructions it issues (330
-// for the two, half of them the codes): 32768 tokens of 32 heads, d 128, bf16, B200:
+// row in the cache are found once for both. Mostly bound by its instructions (330 for
+// the two, half of them the codes, 0.75 issued a cycle): 32768 tokens of 32 heads, d 128, bf16, B200:
 // 200 us for 705 MB (3.5 TB/s; six CTAs per SM, 209 with five); with 64-bit divisions and
 // one tensor per thread 628.
 template <int D, typename T>

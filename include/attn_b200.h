@@ -353,8 +353,8 @@ size_t attn_kv4_decode_workspace_bytes(int64_t batch, int64_t num_heads, int64_t
  * Beside the output's own rounding two roundings to fp16 count: each softmax weight
  * times a V scale (11 bits down to 2^-28 of the largest weight times the row's
  * largest scale, or times 1 where that is larger; fewer below), and the middle,
- * low + 8 scale or low + 7 scale, of each V group. Scores, sums and the softmax are
- * fp32.
+ * low + 8 scale or low + 7 scale, of each V group. Scores (the lows' part with 22
+ * bits), sums and the softmax are fp32.
  */
 int attn_kv4_decode(const void* q, int dtype, const void* k_cache, const void* v_cache,
                     const int32_t* block_tables, const int32_t* context_lens, void* out,
